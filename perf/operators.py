@@ -373,7 +373,7 @@ def _exact_cache(x, pool_codes, pool_scales, slots, case):
     scale = (x.abs().amax(-1) / LARGEST[case["format"]]).clamp(min=SMALLEST_SCALE)
     if case["scale"] == "e8m0":
         mantissa, exponent = torch.frexp(scale)
-        scale = torch.exp2(exponent.double() - (mantissa == 0.5))
+        scale = torch.exp2(exponent.double() - (mantissa == 0.5).double())
     codes = _exact_fp8(x / scale[..., None], case["format"]).flatten(2)
     keep = slots >= 0
     out = []
