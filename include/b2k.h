@@ -338,6 +338,113 @@ B2K_API int b2k_cast(int src_format, int dst_format, int saturate, const void *i
 B2K_API int b2k_cast_ex(int src_format, int dst_format, int saturate, int rounding, const void *in_dev,
                         void *out_dev, int64_t n, void *stream);
 
+/* ---- head-wise norm and rotation; quantised paged key / value cache ---------
+ * No counterpart in the reference, whose users write such kernels over its scalar
+ * intrinsics (cvt_float_to_fp8, numba/cuda/_internal/cuda_fp8.py:3341-3374) and its
+ * 1-D reduce (numba/cuda/kernels/reduction.py:169-265); these are the same conversions
+ * and a last-axis reduction in the form a transformer's attention layer needs them.
+ *
+ * Arrays of heads are (tokens, heads, dim) with unit stride in dim and any strides in
+ * the other two; strides are in items, dim <= B2K_MAX_HEAD_DIM.  An absent array has
+ * heads = 0 (its other members are not read).  Item formats are B2K_FMT_F32,
+ * B2K_FMT_F16 and B2K_FMT_BF16, one for all arrays of heads of a call; all arithmetic
+ * is in float32, rounded once when a value is stored.  Indices (positions, slots, page
+ * numbers, offsets) are 4 or 8 byte signed integers, as *_bytes says. */
+#define B2K_MAX_HEAD_DIM 1024
+
+typedef struct b2k_heads {
+    void *data_dev;
+    int64_t token_stride, head_stride;
+    int64_t heads, dim;
+} b2k_heads;
+
+/* y = rotate(x / sqrt(mean(x^2) + eps) * weight) for every head of every token.
+ *   norm       : 0 leaves the root-mean-square norm and the weights out
+ *   *_weight   : dim items of weight_format, shared by all heads; NULL = ones
+ *   rotary_dim : the first rotary_dim items of a head are rotated (0: none), as pairs
+ *                (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved = 1, by the
+ *                angle whose cosine and sine stand in row positions[token], column i of
+ *                cos_dev and sin_dev (float32, `positions` rows of rotary_dim / 2 items,
+ *                row strides in items)
+ *   positions  : one index per token.  A token whose position is outside
+ *                [0, table_rows) is padding: the forward calls leave its rows as they
+ *                were, the backward call writes zeros. */
+typedef struct b2k_rotation {
+    int64_t format, tokens;
+    b2k_heads q, k;
+    int64_t norm;
+    double eps;
+    const void *q_weight_dev, *k_weight_dev;
+    int64_t weight_format;
+    int64_t rotary_dim, interleaved;
+    const float *cos_dev, *sin_dev;
+    int64_t cos_stride, sin_stride, table_rows;
+    const void *positions_dev;
+    int64_t position_bytes;
+} b2k_rotation;
+
+/* One side (keys or values) of the cache: codes[page][slot][head][dim] of 8 bits and
+ * scales[page][slot][head][dim / group], any strides but unit ones in the last axis. */
+typedef struct b2k_pages {
+    void *codes_dev;
+    int64_t page_stride, slot_stride, head_stride;
+    void *scales_dev;
+    int64_t scale_page_stride, scale_slot_stride, scale_head_stride;
+    int64_t heads, dim, group;
+} b2k_pages;
+
+/*   code_format  : B2K_FMT_E4M3 or B2K_FMT_E5M2
+ *   scale_format : B2K_FMT_F32, or B2K_FMT_E8M0 (a power of two)
+ *   group        : items of a head that share a scale: dim, or a divisor of dim >= 16 */
+typedef struct b2k_cache {
+    int64_t code_format, scale_format;
+    int64_t pages, page_size;
+    b2k_pages k, v;
+} b2k_cache;
+
+/* Forward.  q_out / k_out have the shapes of q / k and may be the same memory; any
+ * other overlap of an output with an input is not allowed. */
+B2K_API int b2k_norm_rotate(const b2k_rotation *r, const b2k_heads *q_out, const b2k_heads *k_out, void *stream);
+
+/* Gradients of b2k_norm_rotate at r->q, r->k for the outputs' gradients q_grad, k_grad:
+ * dq, dk (may be the same memory as q_grad, k_grad) and, where the pointers are not
+ * NULL, those of the weights (dim items of weight_format; sums over all tokens and
+ * heads in a fixed order, so equal calls give equal bits).
+ *   scratch : b2k_norm_rotate_backward_scratch_bytes() bytes, needed when a weight's
+ *             gradient is asked for; need not be cleared; its contents are of no use
+ *             after the call.  Calls that may overlap on the GPU need separate scratch. */
+B2K_API int64_t b2k_norm_rotate_backward_scratch_bytes(const b2k_rotation *r);
+B2K_API int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, const b2k_heads *k_grad,
+                                     const b2k_heads *dq, const b2k_heads *dk, void *dq_weight_dev,
+                                     void *dk_weight_dev, void *scratch_dev, int64_t scratch_bytes, void *stream);
+
+/* Quantise token t's heads of k and v into slot slots[t] = page * page_size + place.
+ * For each group: scale = max(max |finite x| / largest, 2^-126), largest = 448 (E4M3) or
+ * 57344 (E5M2), rounded up to a power of two when scale_format is E8M0; the code is
+ * x * (1 / scale) rounded to nearest even, saturating (infinities too), NaN kept.
+ * A slot outside [0, pages * page_size) skips its token.  The valid slots of one call
+ * must be distinct. */
+B2K_API int b2k_cache_write(const b2k_cache *cache, int format, int64_t tokens, const b2k_heads *k,
+                            const b2k_heads *v, const void *slots_dev, int slot_bytes, void *stream);
+
+/* Read sequences back: output row i of sequence b (offsets[b] <= i < offsets[b + 1]) is
+ * place i - offsets[b] of the pages table[b][0], table[b][1], ...:
+ * value = code * scale, saturated to the output format's finite range (NaN kept).
+ * Rows outside [offsets[0], offsets[seqs]) are left as they were; a page number outside
+ * [0, pages), or a place beyond the table's width, gives a row of zeros.
+ * offsets holds seqs + 1 indices that do not decrease. */
+B2K_API int b2k_cache_read(const b2k_cache *cache, int format, int64_t rows, const b2k_heads *k_out,
+                           const b2k_heads *v_out, const void *table_dev, int64_t table_stride,
+                           int64_t table_width, int table_bytes, const void *offsets_dev, int64_t seqs,
+                           int offset_bytes, void *stream);
+
+/* b2k_norm_rotate of q into q_out, and of k straight into the cache with v beside it, as
+ * b2k_cache_write does, from the unrounded float32 values.  A token whose position is
+ * outside the table is skipped altogether, one whose slot is outside the cache writes
+ * its q row only. */
+B2K_API int b2k_norm_rotate_write(const b2k_rotation *r, const b2k_heads *v, const b2k_heads *q_out,
+                                  const b2k_cache *cache, const void *slots_dev, int slot_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

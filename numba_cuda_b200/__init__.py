@@ -8,6 +8,8 @@ reaches for on this path::
     cuda.kernels.transpose.transpose   (numba/cuda/kernels/transpose.py)
     cuda.random.*                      (numba/cuda/random.py)
     cuda.bf16.*, cuda.fp8.*            (conversion intrinsics, bulk and scalar)
+    cuda.kernels.headnorm.*            (norm + rotation of queries and keys, with gradient; new)
+    cuda.kernels.kvcache.*             (quantised paged cache of keys and values; new)
     cuda.sharded.*                     (contiguous-shard multi-GPU wrappers; new)
 
 Host code is Python; all device work is hand-written sm_100a CUDA in
@@ -19,6 +21,7 @@ from .api import (as_cuda_array, auto_device, default_stream, device_array, devi
                   event, event_elapsed_time, external_stream, is_available, is_bfloat16_supported, is_cuda_array,
                   is_fp8_supported, pinned_array, pinned_array_like, stream, synchronize, to_device)
 from .devicearray import DeviceNDArray, Event, Stream  # noqa: F401
+from .kernels import headnorm as _headnorm, kvcache as _kvcache  # noqa: F401
 from .kernels import reduction as _reduction, transpose as _transpose  # noqa: F401
 from .kernels.reduction import Reduce
 

@@ -26,6 +26,8 @@ SOURCES = [
     "b2k_transpose.cu",
     "b2k_transpose_tma.cu",
     "b2k_assign.cu",
+    "b2k_headnorm.cu",
+    "b2k_kvcache.cu",
 ]
 
 NVCC_FLAGS = [

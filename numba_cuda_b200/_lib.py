@@ -61,6 +61,13 @@ SIGNATURES = {
     "b2k_xoroshiro128p_fill": (_i32, [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _vp]),
     "b2k_cast": (_i32, [_i32, _i32, _i32, _vp, _vp, _i64, _vp]),
     "b2k_cast_ex": (_i32, [_i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
+    # the argument structs travel as packed bytes (kernels/_operands.py)
+    "b2k_norm_rotate": (_i32, [_vp, _vp, _vp, _vp]),
+    "b2k_norm_rotate_backward_scratch_bytes": (_i64, [_vp]),
+    "b2k_norm_rotate_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "b2k_cache_write": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i32, _vp]),
+    "b2k_cache_read": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _vp]),
+    "b2k_norm_rotate_write": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _vp]),
 }
 class B2KError(RuntimeError):
     """A libb2k call failed; ``status`` is the ABI status (negative = argument

@@ -1,0 +1,560 @@
+// Norm and rotation of queries and keys, head by head, forward and backward, and the
+// argument checks and layout choices shared with the cache kernels (b2k_kvcache.cu).
+//
+//   forward   y = R(x r w),  r = 1 / sqrt(mean(x^2) + eps),  R the rotation of the
+//             position's angles
+//   backward  g = R^T dy,  h = g w,  n = x r
+//             dx = r (h - n mean(h n)),   dw = sum over tokens and heads of g n
+//
+// Both are one pass: a row is read once, stays in registers, and is written once, so
+// HBM bounds them (2 and 3 items moved per item of the rows).  The reference's users
+// would write this as a last-axis reduction of their own; its library reduce stops at
+// one axis (numba/cuda/kernels/reduction.py:217-218).
+#include "b2k_heads_forward.cuh"
+
+namespace headwise {
+
+// ---- argument checks ---------------------------------------------------------------
+int item_bytes(int64_t format) {
+    if (format == B2K_FMT_F32) return 4;
+    if (format == B2K_FMT_F16 || format == B2K_FMT_BF16) return 2;
+    return 0;
+}
+
+// Whether an array of `n` axes (outer sizes and strides, innermost run of `run` items)
+// has two items at one address; sizes <= 1 do not count.
+static bool overlapping(int n, const int64_t *size, const int64_t *stride, int64_t run) {
+    int order[4];
+    int m = 0;
+    for (int i = 0; i < n; ++i)
+        if (size[i] > 1) order[m++] = i;
+    for (int i = 1; i < m; ++i)
+        for (int j = i; j > 0 && llabs(stride[order[j]]) < llabs(stride[order[j - 1]]); --j) {
+            const int t = order[j];
+            order[j] = order[j - 1];
+            order[j - 1] = t;
+        }
+    int64_t span = run;
+    for (int i = 0; i < m; ++i) {
+        const int64_t step = llabs(stride[order[i]]);
+        if (step < span) return true;
+        span = step * (size[order[i]] - 1) + span;
+    }
+    return false;
+}
+
+int check_tokens(int64_t format, int64_t tokens, const char *name) {
+    if (item_bytes(format) == 0) return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: items must be f32, f16 or bf16", name);
+    if (tokens < 0) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: negative number of tokens", name);
+    return B2K_OK;
+}
+
+int check_heads(const b2k_heads &h, const char *name, const char *what, int64_t tokens, int itemsize, bool written) {
+    if (h.heads < 0 || h.heads > INT_MAX)
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s has an invalid number of heads", name, what);
+    if (h.heads == 0) return B2K_OK;
+    if (h.dim < 1) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s has no items in a head", name, what);
+    if (h.dim > B2K_MAX_HEAD_DIM)
+        return b2k::fail(B2K_ERR_TOO_LARGE, "%s: %s has heads of more than %d items", name, what, B2K_MAX_HEAD_DIM);
+    if (tokens == 0) return B2K_OK;
+    if (h.data_dev == nullptr) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s is a null pointer", name, what);
+    if (reinterpret_cast<uintptr_t>(h.data_dev) % itemsize)
+        return b2k::fail(B2K_ERR_ALIGNMENT, "%s: %s is not aligned to its items", name, what);
+    const int64_t size[2] = {tokens, h.heads}, stride[2] = {h.token_stride, h.head_stride};
+    if (written && overlapping(2, size, stride, h.dim))
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: rows of %s overlap", name, what);
+    return B2K_OK;
+}
+
+int check_like(const b2k_heads &h, const b2k_heads &like, const char *name, const char *what) {
+    if (h.heads != like.heads || (h.heads && h.dim != like.dim))
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s has another shape than its input", name, what);
+    return B2K_OK;
+}
+
+int check_indices(const void *p, int64_t bytes, const char *name, const char *what) {
+    if (bytes != 4 && bytes != 8)
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s must be 4 or 8 byte integers", name, what);
+    if (p == nullptr) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s is a null pointer", name, what);
+    if (reinterpret_cast<uintptr_t>(p) % bytes)
+        return b2k::fail(B2K_ERR_ALIGNMENT, "%s: %s is not aligned to its items", name, what);
+    return B2K_OK;
+}
+
+int check_rotation(const b2k_rotation *r, const char *name) {
+    if (r == nullptr) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: null arguments", name);
+    if (int rc = check_tokens(r->format, r->tokens, name)) return rc;
+    const int itemsize = item_bytes(r->format);
+    if (int rc = check_heads(r->q, name, "q", r->tokens, itemsize, false)) return rc;
+    if (int rc = check_heads(r->k, name, "k", r->tokens, itemsize, false)) return rc;
+    if (r->norm != 0 && r->norm != 1) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: norm must be 0 or 1", name);
+    if (r->norm) {
+        if (!(r->eps >= 0.0)) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: eps must not be negative", name);
+        const int wbytes = item_bytes(r->weight_format);
+        if ((r->q_weight_dev || r->k_weight_dev) && wbytes == 0)
+            return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: weights must be f32, f16 or bf16", name);
+        for (const void *w : {r->q_weight_dev, r->k_weight_dev})
+            if (w && reinterpret_cast<uintptr_t>(w) % wbytes)
+                return b2k::fail(B2K_ERR_ALIGNMENT, "%s: a weight is not aligned to its items", name);
+    }
+    if (r->interleaved != 0 && r->interleaved != 1)
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: interleaved must be 0 or 1", name);
+    if (r->rotary_dim < 0 || r->rotary_dim % 2)
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: rotary_dim must be even and not negative", name);
+    if (r->rotary_dim > 0) {
+        for (const b2k_heads *h : {&r->q, &r->k})
+            if (h->heads && r->rotary_dim > h->dim)
+                return b2k::fail(B2K_ERR_INVALID_ARG, "%s: rotary_dim is larger than a head", name);
+        if (r->table_rows < 0) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: negative table_rows", name);
+        if (r->tokens > 0) {
+            if (r->table_rows > 0 && (r->cos_dev == nullptr || r->sin_dev == nullptr))
+                return b2k::fail(B2K_ERR_INVALID_ARG, "%s: cos or sin is a null pointer", name);
+            for (const void *t : {r->cos_dev, r->sin_dev})
+                if (reinterpret_cast<uintptr_t>(t) % 4)
+                    return b2k::fail(B2K_ERR_ALIGNMENT, "%s: cos or sin is not aligned to its items", name);
+            if (int rc = check_indices(r->positions_dev, r->position_bytes, name, "positions")) return rc;
+        }
+    }
+    return B2K_OK;
+}
+
+int check_cache(const b2k_cache *c, const char *name) {
+    if (c == nullptr) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: null cache", name);
+    if (c->code_format != B2K_FMT_E4M3 && c->code_format != B2K_FMT_E5M2)
+        return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: codes must be e4m3 or e5m2", name);
+    if (c->scale_format != B2K_FMT_F32 && c->scale_format != B2K_FMT_E8M0)
+        return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: scales must be f32 or e8m0", name);
+    if (c->pages < 0 || c->page_size < 1)
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: invalid number or size of pages", name);
+    if (c->pages > 0 && c->page_size > (int64_t(1) << 62) / c->pages)
+        return b2k::fail(B2K_ERR_TOO_LARGE, "%s: too many slots", name);
+    return B2K_OK;
+}
+
+int check_side(const b2k_pages &side, const b2k_heads &like, const b2k_cache &c, const char *name, const char *what,
+               bool written) {
+    if (side.heads != like.heads || (side.heads && side.dim != like.dim))
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: the %s cache has another number of heads or head size than %s", name,
+                         what, what);
+    if (side.heads == 0) return B2K_OK;
+    if (side.group < 1 || side.dim % side.group || (side.group < 16 && side.group != side.dim))
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: the %s cache's scale group must be a head or a divisor of it >= 16",
+                         name, what);
+    if (c.pages == 0) return B2K_OK;
+    if (side.codes_dev == nullptr || side.scales_dev == nullptr)
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: the %s cache holds a null pointer", name, what);
+    if (c.scale_format == B2K_FMT_F32 && reinterpret_cast<uintptr_t>(side.scales_dev) % 4)
+        return b2k::fail(B2K_ERR_ALIGNMENT, "%s: the %s cache's scales are not aligned to their items", name, what);
+    const int64_t size[3] = {c.pages, c.page_size, side.heads};
+    const int64_t codes[3] = {side.page_stride, side.slot_stride, side.head_stride};
+    const int64_t scales[3] = {side.scale_page_stride, side.scale_slot_stride, side.scale_head_stride};
+    if (written && (overlapping(3, size, codes, side.dim) || overlapping(3, size, scales, side.dim / side.group)))
+        return b2k::fail(B2K_ERR_INVALID_ARG, "%s: rows of the %s cache overlap", name, what);
+    return B2K_OK;
+}
+
+// ---- layout ----------------------------------------------------------------------------
+// The stride of an axis of length 1 is never used: 0 keeps it out of the alignment rules.
+void set_input(Role &r, const b2k_heads &h, int64_t tokens) {
+    r.in = h.data_dev;
+    r.in_token = tokens > 1 ? h.token_stride : 0;
+    r.in_head = h.heads > 1 ? h.head_stride : 0;
+    r.heads = static_cast<int>(h.heads);
+    r.dim = static_cast<int>(h.dim);
+    r.inv_dim = h.heads ? 1.0f / static_cast<float>(h.dim) : 0.0f;
+}
+void set_output(Role &r, const b2k_heads &h, int64_t tokens) {
+    r.out = h.data_dev;
+    r.out_token = tokens > 1 ? h.token_stride : 0;
+    r.out_head = h.heads > 1 ? h.head_stride : 0;
+}
+void set_grad(Role &r, const b2k_heads &h, int64_t tokens) {
+    r.grad = h.data_dev;
+    r.grad_token = tokens > 1 ? h.token_stride : 0;
+    r.grad_head = h.heads > 1 ? h.head_stride : 0;
+}
+void set_pages(Params &p, Role &r, const b2k_cache &c, const b2k_pages &side) {
+    p.pages = c.pages;
+    p.page_size = c.page_size;
+    p.e5m2 = c.code_format == B2K_FMT_E5M2;
+    p.e8m0 = c.scale_format == B2K_FMT_E8M0;
+    r.codes = static_cast<uint8_t *>(side.codes_dev);
+    r.scales = side.scales_dev;
+    r.code_page = c.pages > 1 ? side.page_stride : 0;
+    r.code_slot = c.page_size > 1 ? side.slot_stride : 0;
+    r.code_head = side.heads > 1 ? side.head_stride : 0;
+    r.scale_page = c.pages > 1 ? side.scale_page_stride : 0;
+    r.scale_slot = c.page_size > 1 ? side.scale_slot_stride : 0;
+    r.scale_head = side.heads > 1 ? side.scale_head_stride : 0;
+    r.group = static_cast<int>(side.group);
+}
+void set_rotation(Params &p, const b2k_rotation &rot) {
+    p.norm = static_cast<int>(rot.norm);
+    p.eps = static_cast<float>(rot.eps);
+    p.interleaved = static_cast<int>(rot.interleaved);
+    p.weight_format = static_cast<int>(rot.weight_format);
+    if (rot.norm) {
+        p.role[0].weight = rot.q_weight_dev;
+        p.role[1].weight = rot.k_weight_dev;
+    }
+    if (rot.rotary_dim > 0) {
+        p.cos_table = rot.cos_dev;
+        p.sin_table = rot.sin_dev;
+        p.cos_stride = rot.table_rows > 1 ? rot.cos_stride : 0;
+        p.sin_stride = rot.table_rows > 1 ? rot.sin_stride : 0;
+        p.table_rows = rot.table_rows;
+        p.positions = rot.positions_dev;
+        p.position_bytes = static_cast<int>(rot.position_bytes);
+    }
+}
+
+static bool fits(const void *base, int64_t stride0, int64_t stride1, int itemsize, int vec) {
+    return reinterpret_cast<uintptr_t>(base) % (static_cast<uintptr_t>(itemsize) * vec) == 0 && stride0 % vec == 0 &&
+           stride1 % vec == 0;
+}
+
+// Whether every chunk of `vec` items of a role starts on a multiple of its size.
+static bool role_fits(const Params &p, const Role &r, bool rotated, int rotary, int itemsize, int vec) {
+    if (vec == 1) return true;
+    if (r.dim % vec || !fits(r.in, r.in_token, r.in_head, itemsize, vec)) return false;
+    if (r.out && !fits(r.out, r.out_token, r.out_head, itemsize, vec)) return false;
+    if (r.grad && !fits(r.grad, r.grad_token, r.grad_head, itemsize, vec)) return false;
+    if (r.weight && !fits(r.weight, 0, 0, item_bytes(p.weight_format), vec < 4 || p.weight_format != B2K_FMT_F32 ? vec : 4))
+        return false;
+    if (r.codes && (!fits(r.codes, r.code_page, r.code_slot, 1, vec) || r.code_head % vec || r.group % vec)) return false;
+    if (rotated) {
+        if (rotary % (2 * vec)) return false;
+        const int w = vec < 4 ? vec : 4;
+        if (!fits(p.cos_table, p.cos_stride, 0, 4, w) || !fits(p.sin_table, p.sin_stride, 0, 4, w)) return false;
+    }
+    return true;
+}
+
+Plan choose(Params &p, int64_t format, const b2k_rotation *rot) {
+    const int itemsize = item_bytes(format);
+    const int rotary = rot ? static_cast<int>(rot->rotary_dim) : 0;
+    Plan plan;
+    for (int vec : {1}) {
+        bool ok = true;
+        for (int i = 0; i < 3; ++i)
+            if (p.role[i].heads) ok = ok && role_fits(p, p.role[i], i < 2 && rotary, rotary, itemsize, vec);
+        if (ok) {
+            plan.vec = vec;
+            break;
+        }
+    }
+    int units = 1;
+    for (int i = 0; i < 3; ++i) {
+        Role &r = p.role[i];
+        if (r.heads == 0) continue;
+        const int turned = i < 2 ? rotary : 0;
+        // the two halves of a rotated run pair up; without a rotation of halves the pairs are
+        // the row's two halves where they are whole chunks, else neighbouring chunks
+        int paired = 0;
+        if (turned && !p.interleaved) paired = turned;
+        else if (!turned && r.dim % (2 * plan.vec) == 0) paired = r.dim;
+        r.pair_gap = paired / 2;
+        r.pair_units = paired / 2 / plan.vec;
+        r.tail = paired;
+        r.angle_units = turned / 2 / plan.vec;
+        r.units = r.pair_units + (r.dim - r.tail + 2 * plan.vec - 1) / (2 * plan.vec);
+        if (r.units > units) units = r.units;
+    }
+    p.lanes = 1;
+    while (p.lanes < 32 && p.lanes < units) p.lanes *= 2;
+    const int need = (units + p.lanes - 1) / p.lanes;
+#define B2K_HEADS_PICK(V, I) \
+    if (plan.vec == V && plan.iter == 0 && I >= need) plan.iter = I;
+    B2K_HEADS_SHAPES(B2K_HEADS_PICK)
+#undef B2K_HEADS_PICK
+    return plan;
+}
+
+int count_items(Params &p, const char *name) {
+    p.heads_per_item = 1;
+    p.items_per_token = 0;
+    int64_t per_token = 0;
+    for (Role &r : p.role) {
+        r.items = (r.heads + p.heads_per_item - 1) / p.heads_per_item;
+        per_token += r.items;
+    }
+    if (per_token > INT_MAX || (per_token && p.tokens > int64_t(UINT_MAX) / per_token))
+        return b2k::fail(B2K_ERR_TOO_LARGE, "%s: more than 2^32 - 1 rows", name);
+    p.items_per_token = static_cast<int>(per_token);
+    p.items = static_cast<uint32_t>(p.tokens * per_token);
+    return B2K_OK;
+}
+
+// ---- backward ----------------------------------------------------------------------------
+// Blocks of a role stride over its rows and keep the weight gradient's partial sums in
+// registers; each block writes one row of partials, and a second kernel adds the rows
+// in order: no atomics, so equal calls give equal bits.
+constexpr int kBackwardBlocksPerSm = 4;
+
+template <typename T, int VEC, int ITER>
+__global__ void __launch_bounds__(kThreads) heads_backward_kernel(const __grid_constant__ Params p) {
+    extern __shared__ float block_sums[];             // one row of dim floats per warp
+    const Lanes g(p.lanes);
+    const int which = static_cast<int>(blockIdx.x) < p.blocks0 ? 0 : 1;
+    const Role &r = p.role[which];
+    const uint32_t first = which ? blockIdx.x - p.blocks0 : blockIdx.x;
+    const uint32_t blocks = which ? gridDim.x - p.blocks0 : p.blocks0;
+    const uint32_t in_block = kThreads / g.n;
+    const int64_t items = p.tokens * r.items;
+    const bool summed = r.weight_grad != nullptr;
+    float sum_a[ITER][VEC] = {}, sum_b[ITER][VEC] = {};
+    float wa[ITER][VEC] = {}, wb[ITER][VEC] = {};
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        int oa, ob;
+        unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
+        if (oa < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa, wa[i]);
+        if (ob < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob, wb[i]);
+    }
+    for (int64_t item = static_cast<int64_t>(first) * in_block + threadIdx.x / g.n; item < items;
+         item += static_cast<int64_t>(blocks) * in_block) {
+        int64_t token, rest;
+        paging::divide(item, r.items, token, rest);
+        const int part = static_cast<int>(rest);
+        int64_t position = 0;
+        if (p.positions != nullptr) position = paging::load_index(p.positions, p.position_bytes, token);
+        const bool padding = p.positions != nullptr && (position < 0 || position >= p.table_rows);
+        float c[ITER][VEC] = {}, s[ITER][VEC] = {};
+        if (!padding) {
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                const int u = g.lane + i * g.n;
+                if (u < r.angle_units) {
+                    load_floats<VEC>(p.cos_table + position * p.cos_stride + u * VEC, c[i]);
+                    load_floats<VEC>(p.sin_table + position * p.sin_stride + u * VEC, s[i]);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) s[i][j] = -s[i][j];      // the inverse rotation
+                }
+            }
+        }
+        const int last = min(r.heads, (part + 1) * p.heads_per_item);
+        for (int head = part * p.heads_per_item; head < last; ++head) {
+            const T *in = static_cast<const T *>(r.in) + token * r.in_token + head * r.in_head;
+            const T *grad = static_cast<const T *>(r.grad) + token * r.grad_token + head * r.grad_head;
+            T *out = static_cast<T *>(r.out) + token * r.out_token + head * r.out_head;
+            float xa[ITER][VEC], xb[ITER][VEC], ga[ITER][VEC], gb[ITER][VEC];
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                int oa, ob;
+                unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
+                Chunk<T, VEC> ca{}, cb{}, da{}, db{};
+                if (oa < r.dim && !padding) {
+                    ca = load_chunk<T, VEC>(in + oa);
+                    da = load_chunk<T, VEC>(grad + oa);
+                }
+                if (ob < r.dim && !padding) {
+                    cb = load_chunk<T, VEC>(in + ob);
+                    db = load_chunk<T, VEC>(grad + ob);
+                }
+                widen(ca, xa[i]);
+                widen(cb, xb[i]);
+                widen(da, ga[i]);
+                widen(db, gb[i]);
+            }
+            float ss = 0.0f, dot = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                if (g.lane + i * g.n < r.angle_units) rotate<VEC>(ga[i], gb[i], c[i], s[i], p.interleaved);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    ss += xa[i][j] * xa[i][j] + xb[i][j] * xb[i][j];
+                    dot += ga[i][j] * wa[i][j] * xa[i][j] + gb[i][j] * wb[i][j] * xb[i][j];
+                }
+            }
+            if (p.norm) {
+                // mean(h n) = by * dot / dim; a padding row is all zeros (eps may be zero, too)
+                const float by = padding ? 0.0f : rsqrtf(g.sum(ss) * r.inv_dim + p.eps);
+                const float pull = g.sum(dot) * r.inv_dim * by * by;
+#pragma unroll
+                for (int i = 0; i < ITER; ++i)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        sum_a[i][j] += ga[i][j] * (xa[i][j] * by);
+                        sum_b[i][j] += gb[i][j] * (xb[i][j] * by);
+                        ga[i][j] = by * (ga[i][j] * wa[i][j] - xa[i][j] * pull);
+                        gb[i][j] = by * (gb[i][j] * wb[i][j] - xb[i][j] * pull);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                int oa, ob;
+                unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
+                if (oa < r.dim) store_chunk<T, VEC>(out + oa, ga[i]);
+                if (ob < r.dim) store_chunk<T, VEC>(out + ob, gb[i]);
+            }
+        }
+    }
+    if (!summed) return;
+    // groups of a warp, then the block's warps in order
+    const int warp = threadIdx.x / 32;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        for (int o = g.n; o < 32; o *= 2)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                sum_a[i][j] += __shfl_xor_sync(0xFFFFFFFFu, sum_a[i][j], o);
+                sum_b[i][j] += __shfl_xor_sync(0xFFFFFFFFu, sum_b[i][j], o);
+            }
+        int oa, ob;
+        unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
+        if (threadIdx.x % 32 < g.n) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (oa < r.dim) block_sums[warp * r.dim + oa + j] = sum_a[i][j];
+                if (ob < r.dim) block_sums[warp * r.dim + ob + j] = sum_b[i][j];
+            }
+        }
+    }
+    __syncthreads();
+    float *row = p.partials + static_cast<int64_t>(blockIdx.x) * B2K_MAX_HEAD_DIM;
+    for (int d = threadIdx.x; d < r.dim; d += kThreads) {
+        float v = 0.0f;
+        for (int w = 0; w < kThreads / 32; ++w) v += block_sums[w * r.dim + d];
+        row[d] = v;
+    }
+}
+
+// weight_grad[d] = sum over the role's blocks of partials[block][d], 32 columns a block:
+// eight rows of threads stride over the blocks, then a fixed tree.
+__global__ void __launch_bounds__(kThreads) weight_grad_kernel(const __grid_constant__ Params p, int blocks) {
+    __shared__ float part[kThreads / 32][32];
+    const Role &r = p.role[blockIdx.y];
+    if (r.weight_grad == nullptr) return;
+    const int d = blockIdx.x * 32 + threadIdx.x % 32, row = threadIdx.x / 32;
+    const int begin = blockIdx.y ? p.blocks0 : 0, end = blockIdx.y ? blocks : p.blocks0;
+    float v = 0.0f;
+    if (d < r.dim)
+        for (int b = begin + row; b < end; b += kThreads / 32) v += p.partials[static_cast<int64_t>(b) * B2K_MAX_HEAD_DIM + d];
+    part[row][threadIdx.x % 32] = v;
+    __syncthreads();
+    if (row || d >= r.dim) return;
+    for (int w = 1; w < kThreads / 32; ++w) v += part[w][threadIdx.x];
+    if (p.weight_format == B2K_FMT_F32) static_cast<float *>(r.weight_grad)[d] = v;
+    else if (p.weight_format == B2K_FMT_F16) static_cast<__half *>(r.weight_grad)[d] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(r.weight_grad)[d] = __float2bfloat16_rn(v);
+}
+
+static int backward_blocks() { return b2k::sm_count() * kBackwardBlocksPerSm; }
+
+template <typename T>
+static void pick_backward(const Params &p, const Plan &plan, int blocks, size_t shared, cudaStream_t stream) {
+#define B2K_HEADS_CASE(V, I)                                                              \
+    if (plan.vec == V && plan.iter == I) {                                                \
+        heads_backward_kernel<T, V, I><<<blocks, kThreads, shared, stream>>>(p);          \
+        return;                                                                           \
+    }
+    B2K_HEADS_SHAPES(B2K_HEADS_CASE)
+#undef B2K_HEADS_CASE
+}
+
+}  // namespace headwise
+
+extern "C" {
+
+using namespace headwise;
+
+int b2k_norm_rotate(const b2k_rotation *r, const b2k_heads *q_out, const b2k_heads *k_out, void *stream) {
+    B2K_RANGE("b2k_norm_rotate");
+    const char *name = "b2k_norm_rotate";
+    if (int rc = check_rotation(r, name)) return rc;
+    if (q_out == nullptr || k_out == nullptr) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: null arguments", name);
+    Params p{};
+    const b2k_heads *in[2] = {&r->q, &r->k}, *out[2] = {q_out, k_out};
+    for (int i = 0; i < 2; ++i) {
+        const char *what = i ? "k_out" : "q_out";
+        if (int rc = check_heads(*out[i], name, what, r->tokens, item_bytes(r->format), true)) return rc;
+        if (int rc = check_like(*out[i], *in[i], name, what)) return rc;
+        if (in[i]->heads == 0) continue;
+        set_input(p.role[i], *in[i], r->tokens);
+        set_output(p.role[i], *out[i], r->tokens);
+    }
+    if (r->tokens == 0) return B2K_OK;
+    p.tokens = r->tokens;
+    set_rotation(p, *r);
+    const Plan plan = choose(p, r->format, r);
+    return launch_forward<kRotate>(p, r->format, plan, b2k::as_stream(stream), name);
+}
+
+int64_t b2k_norm_rotate_backward_scratch_bytes(const b2k_rotation *r) {
+    (void)r;
+    return static_cast<int64_t>(backward_blocks()) * B2K_MAX_HEAD_DIM * 4;
+}
+
+int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, const b2k_heads *k_grad,
+                             const b2k_heads *dq, const b2k_heads *dk, void *dq_weight_dev, void *dk_weight_dev,
+                             void *scratch_dev, int64_t scratch_bytes, void *stream) {
+    B2K_RANGE("b2k_norm_rotate_backward");
+    const char *name = "b2k_norm_rotate_backward";
+    if (int rc = check_rotation(r, name)) return rc;
+    if (!q_grad || !k_grad || !dq || !dk) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: null arguments", name);
+    Params p{};
+    const b2k_heads *in[2] = {&r->q, &r->k}, *grad[2] = {q_grad, k_grad}, *out[2] = {dq, dk};
+    void *weight_grad[2] = {dq_weight_dev, dk_weight_dev};
+    const int itemsize = item_bytes(r->format);
+    for (int i = 0; i < 2; ++i) {
+        if (int rc = check_heads(*grad[i], name, i ? "k_grad" : "q_grad", r->tokens, itemsize, false)) return rc;
+        if (int rc = check_heads(*out[i], name, i ? "dk" : "dq", r->tokens, itemsize, true)) return rc;
+        if (int rc = check_like(*grad[i], *in[i], name, i ? "k_grad" : "q_grad")) return rc;
+        if (int rc = check_like(*out[i], *in[i], name, i ? "dk" : "dq")) return rc;
+        if (weight_grad[i]) {
+            const void *w = i ? r->k_weight_dev : r->q_weight_dev;
+            if (!r->norm || in[i]->heads == 0 || w == nullptr)
+                return b2k::fail(B2K_ERR_INVALID_ARG, "%s: the gradient of a weight that is not there is asked for", name);
+            if (reinterpret_cast<uintptr_t>(weight_grad[i]) % item_bytes(r->weight_format))
+                return b2k::fail(B2K_ERR_ALIGNMENT, "%s: a weight's gradient is not aligned to its items", name);
+        }
+        if (in[i]->heads == 0) continue;
+        set_input(p.role[i], *in[i], r->tokens);
+        set_grad(p.role[i], *grad[i], r->tokens);
+        set_output(p.role[i], *out[i], r->tokens);
+        p.role[i].weight_grad = weight_grad[i];
+    }
+    const bool summed = dq_weight_dev || dk_weight_dev;
+    if (r->tokens == 0 && !summed) return B2K_OK;
+    if (summed && (scratch_dev == nullptr || scratch_bytes < b2k_norm_rotate_backward_scratch_bytes(r)))
+        return b2k::fail(B2K_ERR_SCRATCH, "%s: scratch is missing or too small", name);
+    if (reinterpret_cast<uintptr_t>(scratch_dev) % 4)
+        return b2k::fail(B2K_ERR_ALIGNMENT, "%s: scratch is not aligned", name);
+    p.tokens = r->tokens;
+    p.partials = static_cast<float *>(scratch_dev);
+    set_rotation(p, *r);
+    const Plan plan = choose(p, r->format, r);
+    if (int rc = count_items(p, name)) return rc;
+    // blocks go to the two roles by their share of the rows' items, at least one to each
+    const int64_t in_block = kThreads / p.lanes;
+    int64_t need[2], most = backward_blocks();
+    for (int i = 0; i < 2; ++i) need[i] = (p.tokens * p.role[i].items + in_block - 1) / in_block;
+    if (need[0] + need[1] > most) {
+        const int64_t total = need[0] + need[1];
+        int64_t first = need[0] * most / total;
+        if (need[0] && first < 1) first = 1;
+        if (need[1] && first > most - 1) first = most - 1;
+        need[0] = first;
+        need[1] = need[1] ? most - first : 0;
+    }
+    p.blocks0 = static_cast<int>(need[0]);
+    const int blocks = static_cast<int>(need[0] + need[1]);
+    const int dim = p.role[0].dim > p.role[1].dim ? p.role[0].dim : p.role[1].dim;
+    const cudaStream_t st = b2k::as_stream(stream);
+    if (blocks > 0) {
+        const size_t shared = summed ? static_cast<size_t>(kThreads / 32) * dim * sizeof(float) : 0;
+        if (r->format == B2K_FMT_F32) pick_backward<float>(p, plan, blocks, shared, st);
+        else if (r->format == B2K_FMT_F16) pick_backward<__half>(p, plan, blocks, shared, st);
+        else pick_backward<__nv_bfloat16>(p, plan, blocks, shared, st);
+        B2K_RETURN_IF_LAUNCH_FAILED(name);
+        b2k::note_launch();
+    }
+    if (summed) {
+        weight_grad_kernel<<<dim3((dim + 31) / 32, 2), kThreads, 0, st>>>(p, blocks);
+        B2K_RETURN_IF_LAUNCH_FAILED(name);
+        b2k::note_launch();
+    }
+    return B2K_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,247 @@
+// Row arithmetic shared by the head-wise kernels (b2k_headnorm.cu, b2k_kvcache.cu).
+//
+// A row is one head of one token, dim <= 1024 items.  It is owned by a group of 1..32
+// lanes of one warp; a lane owns `units` of the row, each a pair of chunks of VEC items.
+// The two chunks of a unit are chosen so that every rotated pair (i, i + R/2) lies in
+// ONE lane: the rotation needs no exchange between lanes, and neighbouring lanes still
+// read neighbouring chunks.  The row stays in registers from its load to its store.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <float.h>
+
+#include "b2k_internal.cuh"
+#include "b2k_pages.cuh"
+
+namespace headwise {
+
+constexpr int kThreads = 256;
+
+// One array role of a launch (queries, keys or values).
+struct Role {
+    const void *in;
+    void *out;                  // null: the role is quantised into the cache
+    const void *grad;           // backward: the gradient of the role's output
+    int64_t in_token, in_head, out_token, out_head, grad_token, grad_head;
+    const void *weight;
+    void *weight_grad;
+    uint8_t *codes;
+    void *scales;
+    int64_t code_page, code_slot, code_head, scale_page, scale_slot, scale_head;
+    int heads, dim, group;
+    int items;                  // items of work a token has in this role: ceil(heads / heads_per_item)
+    int units;                  // chunk pairs of a row
+    int pair_units, pair_gap, tail;   // units below pair_units are (u, u + gap); the others lie from `tail` on
+    int angle_units;            // units below it are rotated
+    float inv_dim;
+};
+
+struct Params {
+    Role role[3];
+    int64_t tokens;
+    uint32_t items;             // all items of the launch
+    int items_per_token, heads_per_item, lanes;
+    int norm, interleaved, weight_format;
+    float eps;
+    const float *cos_table, *sin_table;
+    int64_t cos_stride, sin_stride, table_rows;
+    const void *positions;
+    int position_bytes;
+    const void *slots;
+    int slot_bytes, e5m2, e8m0;
+    int64_t pages, page_size;
+    float *partials;            // backward: weight-gradient partial sums, one row of dim floats per block
+    int blocks0;                // backward: blocks of role 0
+};
+
+template <typename T> struct Convert;
+template <> struct Convert<float> {
+    __device__ static float up(float x) { return x; }
+    __device__ static float down(float x) { return x; }
+};
+template <> struct Convert<__half> {
+    __device__ static float up(__half x) { return __half2float(x); }
+    __device__ static __half down(float x) { return __float2half_rn(x); }
+};
+template <> struct Convert<__nv_bfloat16> {
+    __device__ static float up(__nv_bfloat16 x) { return __bfloat162float(x); }
+    __device__ static __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
+};
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Chunk {
+    T e[VEC];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ Chunk<T, VEC> load_chunk(const T *p) {
+    return *reinterpret_cast<const Chunk<T, VEC> *>(p);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_chunk(T *p, const float (&v)[VEC]) {
+    Chunk<T, VEC> c;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) c.e[j] = Convert<T>::down(v[j]);
+    *reinterpret_cast<Chunk<T, VEC> *>(p) = c;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Chunk<T, VEC> &c, float (&v)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = Convert<T>::up(c.e[j]);
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_floats(const float *p, float (&v)[VEC]) {
+    constexpr int W = VEC < 4 ? VEC : 4;       // 16 bytes at most
+#pragma unroll
+    for (int j = 0; j < VEC; j += W) {
+        const Chunk<float, W> c = load_chunk<float, W>(p + j);
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[j + i] = c.e[i];
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_weight(const void *w, int format, int at, float (&v)[VEC]) {
+    if (w == nullptr) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = 1.0f;
+    } else if (format == B2K_FMT_F32) {
+        load_floats<VEC>(static_cast<const float *>(w) + at, v);
+    } else if (format == B2K_FMT_BF16) {
+        widen(load_chunk<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16 *>(w) + at), v);
+    } else {
+        widen(load_chunk<__half, VEC>(static_cast<const __half *>(w) + at), v);
+    }
+}
+
+// The lanes of a group, and where a unit's two chunks start.
+struct Lanes {
+    int n, lane;
+    unsigned mask;
+    __device__ explicit Lanes(int lanes) : n(lanes), lane(threadIdx.x & (lanes - 1)) {
+        const unsigned ones = lanes == 32 ? 0xFFFFFFFFu : (1u << lanes) - 1u;
+        mask = ones << ((threadIdx.x & 31) & ~(lanes - 1));
+    }
+    __device__ float sum(float v) const {
+        for (int o = n >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+        return v;
+    }
+    __device__ float max(float v) const {
+        for (int o = n >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
+        return v;
+    }
+};
+
+template <int VEC>
+__device__ __forceinline__ void unit_at(const Role &r, int u, int &a, int &b) {
+    if (u < r.pair_units) {
+        a = u * VEC;
+        b = a + r.pair_gap;
+    } else {
+        a = r.tail + 2 * (u - r.pair_units) * VEC;
+        b = a + VEC;
+    }
+    if (u >= r.units) a = b = r.dim;       // nothing
+}
+
+// Rotation of a unit by its angles (VEC == 1: a pair is always the unit's two items).
+template <int VEC>
+__device__ __forceinline__ void rotate(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC],
+                                       bool interleaved) {
+    if (VEC == 1 || !interleaved) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float x = a[j], y = b[j];
+            a[j] = x * c[j] - y * s[j];
+            b[j] = y * c[j] + x * s[j];
+        }
+    } else if constexpr (VEC > 1) {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+            float x = a[2 * j], y = a[2 * j + 1];
+            a[2 * j] = x * c[j] - y * s[j];
+            a[2 * j + 1] = y * c[j] + x * s[j];
+            x = b[2 * j], y = b[2 * j + 1];
+            b[2 * j] = x * c[VEC / 2 + j] - y * s[VEC / 2 + j];
+            b[2 * j + 1] = y * c[VEC / 2 + j] + x * s[VEC / 2 + j];
+        }
+    }
+}
+
+// ---- quantisation -----------------------------------------------------------------
+__device__ __forceinline__ uint32_t pack_codes2(float hi, float lo, int e5m2) {
+    uint16_t r;
+    if (e5m2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_codes(uint8_t *p, const float (&v)[VEC], float by, int e5m2) {
+    if constexpr (VEC == 1) {
+        *p = static_cast<uint8_t>(pack_codes2(0.0f, v[0] * by, e5m2));
+    } else {
+        Chunk<uint16_t, VEC / 2> c;
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) c.e[j] = pack_codes2(v[2 * j + 1] * by, v[2 * j] * by, e5m2);
+        *reinterpret_cast<Chunk<uint16_t, VEC / 2> *>(p) = c;
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ float largest_finite(const float (&v)[VEC]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const float x = fabsf(v[j]);
+        m = fmaxf(m, x <= FLT_MAX ? x : 0.0f);      // an infinity or a NaN says nothing about the scale
+    }
+    return m;
+}
+
+// Scale for a largest magnitude, and its E8M0 code.  The lower bound keeps 1 / scale
+// finite and covers a row of zeros.
+__device__ __forceinline__ float scale_for(float amax, int e5m2, int e8m0, uint8_t &code) {
+    float s = fmaxf(__fdiv_rn(amax, e5m2 ? 57344.0f : 448.0f), 0x1p-126f);
+    if (e8m0) {
+        // s is a normal number: adding all mantissa bits carries into the exponent
+        // unless they are all zero, which is the power of two not below s
+        const uint32_t e = (__float_as_uint(s) + 0x007FFFFFu) >> 23;
+        code = static_cast<uint8_t>(e);
+        s = __uint_as_float(e << 23);
+    }
+    return s;
+}
+
+// ---- host side ----------------------------------------------------------------------
+// The (items per chunk, units per lane) pairs that are compiled; choose() picks one.
+#define B2K_HEADS_SHAPES(CASE) CASE(1, 1) CASE(1, 4) CASE(1, 16)
+
+struct Plan {
+    int vec = 0, iter = 0;
+};
+
+// Argument checks; the messages start with `name`.  0 = fine.
+int item_bytes(int64_t format);                      // 0 for a format that arrays of heads cannot have
+int check_heads(const b2k_heads &h, const char *name, const char *what, int64_t tokens, int itemsize, bool written);
+int check_like(const b2k_heads &h, const b2k_heads &like, const char *name, const char *what);
+int check_tokens(int64_t format, int64_t tokens, const char *name);
+int check_rotation(const b2k_rotation *r, const char *name);
+int check_cache(const b2k_cache *c, const char *name);
+int check_side(const b2k_pages &side, const b2k_heads &like, const b2k_cache &c, const char *name, const char *what,
+               bool written);
+int check_indices(const void *p, int64_t bytes, const char *name, const char *what);
+
+void set_input(Role &r, const b2k_heads &h, int64_t tokens);
+void set_output(Role &r, const b2k_heads &h, int64_t tokens);
+void set_grad(Role &r, const b2k_heads &h, int64_t tokens);
+void set_pages(Params &p, Role &r, const b2k_cache &c, const b2k_pages &side);
+void set_rotation(Params &p, const b2k_rotation &rot);
+// Chunk width from sizes, strides and addresses; lanes and unit layout of every role.
+Plan choose(Params &p, int64_t format, const b2k_rotation *rot);
+// items and heads per item; an error when they do not fit 32 bits.
+int count_items(Params &p, const char *name);
+
+}  // namespace headwise

@@ -1,0 +1,183 @@
+"""Norm and rotation of a transformer layer's queries and keys, head by head, in one
+pass over the data: ``norm_rotate`` and its gradient ``norm_rotate_backward``.
+
+For a head ``x`` of a token at position ``p``::
+
+    y = x / sqrt(mean(x**2) + eps) * weight
+    (y[i], y[j]) -> (y[i] cos - y[j] sin, y[j] cos + y[i] sin),   cos = cos[p, i], sin = sin[p, i]
+
+over the pairs ``(i, j) = (i, i + R/2)`` of the first ``R`` items, or ``(2i, 2i + 1)`` with
+``interleaved``; the remaining items are not rotated.  All arithmetic is in float32,
+rounded once when a result is stored.
+
+The reference's users write this over their own last-axis reductions: its library
+reduce stops at one axis (numba/cuda/kernels/reduction.py:217-218).  ``kernels.kvcache``
+has the form that writes the keys straight into a quantised cache."""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from ..devicearray import _torch_stream, stream_ptr
+from ._operands import (HEAD_FORMATS, ROTATION, heads, index_bytes, indices, like, on_one_device, operand, pack_heads)
+
+
+def _weight(w, what, dim, stream):
+    if w is None:
+        return None
+    op = operand(w, what, stream=stream)
+    if op.format not in HEAD_FORMATS:
+        raise TypeError(f"{what} must be float32, float16 or bfloat16")
+    if len(op.shape) != 1 or op.shape[0] != dim or (dim > 1 and op.strides[0] != 1):
+        raise ValueError(f"{what} must be a contiguous 1-D array of {dim} items")
+    return op
+
+
+def _table(x, what, stream):
+    op = operand(x, what, stream=stream)
+    if op.format != _lib.FMT_F32:
+        raise TypeError(f"{what} must be float32")
+    if len(op.shape) != 2 or (op.shape[1] > 1 and op.strides[1] != 1):
+        raise ValueError(f"{what} must be 2-D, (positions, half the rotated items), with unit stride in its last axis")
+    return op
+
+
+def rotation(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, stream):
+    """Check the arguments that all calls share: (q, k, all operands, packed b2k_rotation)."""
+    q = heads(q, "q", stream=stream) if q is not None else None
+    k = heads(k, "k", stream=stream) if k is not None else None
+    first = q if q is not None else k
+    if first is None:
+        raise ValueError("neither q nor k is given")
+    tokens = first.shape[0]
+    ops = [q, k]
+    if q is not None and k is not None and (k.shape[0] != tokens or k.format != q.format):
+        raise ValueError("q and k must have the same number of tokens and the same type")
+    if not norm and (q_weight is not None or k_weight is not None):
+        raise ValueError("weights belong to the norm: norm=False takes none")
+    qw = _weight(q_weight, "q_weight", q.shape[2], stream) if q is not None else None
+    kw = _weight(k_weight, "k_weight", k.shape[2], stream) if k is not None else None
+    if qw is not None and kw is not None and qw.format != kw.format:
+        raise TypeError("q_weight and k_weight must have the same type")
+    ops += [qw, kw]
+    weight = qw if qw is not None else kw
+    angles = (0, 0, 0, 0, 0, 0, 0, 8)
+    if cos is not None or sin is not None or positions is not None:
+        if cos is None or sin is None or positions is None:
+            raise ValueError("cos, sin and positions go together")
+        c, s = _table(cos, "cos", stream), _table(sin, "sin", stream)
+        if c.shape != s.shape:
+            raise ValueError("cos and sin must have the same shape")
+        at = indices(positions, "positions", tokens, stream)
+        ops += [c, s, at]
+        for x in (q, k):
+            if x is not None and 2 * c.shape[1] > x.shape[2]:
+                raise ValueError("cos and sin rotate more items than a head has")
+        angles = (2 * c.shape[1], c.ptr, s.ptr, c.strides[0], s.strides[0], c.shape[0], at.ptr, index_bytes(at))
+    none = (0, 0, 0, 0, 0)
+    packed = ROTATION.pack(
+        first.format, tokens,
+        *((q.ptr, q.strides[0], q.strides[1], q.shape[1], q.shape[2]) if q is not None else none),
+        *((k.ptr, k.strides[0], k.strides[1], k.shape[1], k.shape[2]) if k is not None else none),
+        1 if norm else 0, float(eps), qw.ptr if qw is not None else 0, kw.ptr if kw is not None else 0,
+        weight.format if weight is not None else _lib.FMT_F32, angles[0], 1 if interleaved else 0, *angles[1:])
+    return q, k, ops, packed
+
+
+def result(out, source, what, stream):
+    """(array to return, operand) of an optional output with an input's shape and type."""
+    if source is None:
+        if out is not None:
+            raise ValueError(f"{what} is given without its input")
+        return None, None
+    if out is None:
+        out = like(source, stream)
+    op = heads(out, what, written=True, stream=stream)
+    if op.shape != source.shape:
+        raise ValueError(f"{what} must have the shape {source.shape}")
+    if op.format != source.format:
+        raise TypeError(f"{what} must have its input's type")
+    return out, op
+
+
+def norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, positions=None, eps=1e-6, interleaved=False,
+                norm=True, q_out=None, k_out=None, stream=0):
+    """Normalise and rotate the heads of ``q`` and ``k`` in one launch; returns
+    ``(q_out, k_out)``.
+
+    :param q, k: (tokens, heads, dim) arrays of one type, float32, float16 or bfloat16
+                 (``uint16`` items are bfloat16 bits), unit stride in ``dim``, any other
+                 strides -- views of one projection's output, or of a heads-first array.
+                 Either may be ``None``; their head counts and sizes (up to 1024) may differ.
+    :param q_weight, k_weight: ``dim`` items each, shared by all heads; ``None`` for ones.
+    :param cos, sin: float32 tables (positions, R/2); ``None`` (with ``positions``) to
+                 leave the rotation out.
+    :param positions: one int32 or int64 per token.  A token whose position is not a row of
+                 the tables is padding: its rows of the outputs are left as they were.
+    :param norm: ``False`` leaves the norm out.
+    :param q_out, k_out: outputs; new arrays when not given (padding rows are then not
+                 set).  An output may be its own input's memory; it must not overlap an
+                 input in any other way.
+    """
+    q, k, ops, packed = rotation(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, stream)
+    q_out, qo = result(q_out, q, "q_out", stream)
+    k_out, ko = result(k_out, k, "k_out", stream)
+    on_one_device([*ops, qo, ko])
+    _lib.check(_lib.lib().b2k_norm_rotate(packed, pack_heads(qo), pack_heads(ko), stream_ptr(stream)))
+    return q_out, k_out
+
+
+def norm_rotate_backward(q, k, q_weight, k_weight, cos, sin, positions, q_grad, k_grad, eps=1e-6, interleaved=False,
+                         norm=True, dq=None, dk=None, dq_weight=None, dk_weight=None, stream=0):
+    """Gradients of ``norm_rotate``: for the gradients ``q_grad``, ``k_grad`` of its outputs
+    returns ``(dq, dk, dq_weight, dk_weight)``, with ``None`` where an input was ``None``.
+
+    The weights' gradients are sums over all tokens and heads, accumulated in float32 in
+    an order that depends on the shapes only, and are stored in the weights' type.  A
+    padding token has zero gradients and adds nothing to the sums.  ``dq`` and ``dk`` may be
+    the memory of ``q_grad`` and ``k_grad``."""
+    q, k, ops, packed = rotation(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, stream)
+    grads, outs, weights = [], [], []
+    for grad, x, what in ((q_grad, q, "q_grad"), (k_grad, k, "k_grad")):
+        if (grad is None) != (x is None):
+            raise ValueError(f"{what} and its input go together")
+        op = heads(grad, what, stream=stream) if x is not None else None
+        if op is not None and (op.shape != x.shape or op.format != x.format):
+            raise ValueError(f"{what} must have its input's shape and type")
+        grads.append(op)
+    for out, x, what in ((dq, q, "dq"), (dk, k, "dk")):
+        outs.append(result(out, x, what, stream))
+    for out, w, what in ((dq_weight, ops[2], "dq_weight"), (dk_weight, ops[3], "dk_weight")):
+        if w is None:
+            if out is not None:
+                raise ValueError(f"{what} is given without its weight")
+            weights.append((None, None))
+            continue
+        if out is None:
+            out = like(w, stream)
+        op = operand(out, what, written=True, stream=stream)
+        if op.shape != w.shape or op.format != w.format or (op.shape[0] > 1 and op.strides[0] != 1):
+            raise ValueError(f"{what} must be contiguous with its weight's shape and type")
+        weights.append((out, op))
+    on_one_device([*ops, *grads, *(op for _, op in outs), *(op for _, op in weights)])
+    L = _lib.lib()
+    scratch, need = None, 0
+    if ops[2] is not None or ops[3] is not None:
+        need = int(L.b2k_norm_rotate_backward_scratch_bytes(packed))
+        # from torch's allocator on the call's stream, for this call alone: calls on other
+        # streams, and replays of captured graphs, have their own
+        ts = _torch_stream(stream)
+        if torch.cuda.current_stream() == ts:
+            scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+        else:
+            with torch.cuda.stream(ts):
+                scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    _lib.check(L.b2k_norm_rotate_backward(
+        packed, pack_heads(grads[0]), pack_heads(grads[1]), pack_heads(outs[0][1]), pack_heads(outs[1][1]),
+        weights[0][1].ptr if weights[0][1] is not None else None,
+        weights[1][1].ptr if weights[1][1] is not None else None,
+        scratch.data_ptr() if scratch is not None else None, need, stream_ptr(stream)))
+    return outs[0][0], outs[1][0], weights[0][0], weights[1][0]
+
+
+__all__ = ["norm_rotate", "norm_rotate_backward"]
