@@ -234,7 +234,8 @@ Plan choose(Params &p, int64_t format, const b2k_rotation *rot) {
     const int itemsize = item_bytes(format);
     const int rotary = rot ? static_cast<int>(rot->rotary_dim) : 0;
     Plan plan;
-    for (int vec : {1}) {
+    for (int vec : {8, 4, 1}) {
+        if (vec * itemsize > 16) continue;
         bool ok = true;
         for (int i = 0; i < 3; ++i)
             if (p.role[i].heads) ok = ok && role_fits(p, p.role[i], i < 2 && rotary, rotary, itemsize, vec);
@@ -444,7 +445,7 @@ static int backward_blocks() { return b2k::sm_count() * kBackwardBlocksPerSm; }
 template <typename T>
 static void pick_backward(const Params &p, const Plan &plan, int blocks, size_t shared, cudaStream_t stream) {
 #define B2K_HEADS_CASE(V, I)                                                              \
-    if (plan.vec == V && plan.iter == I) {                                                \
+    if constexpr (V * sizeof(T) <= 16) if (plan.vec == V && plan.iter == I) { \
         heads_backward_kernel<T, V, I><<<blocks, kThreads, shared, stream>>>(p);          \
         return;                                                                           \
     }

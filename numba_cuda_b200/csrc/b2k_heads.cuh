@@ -217,7 +217,8 @@ __device__ __forceinline__ float scale_for(float amax, int e5m2, int e8m0, uint8
 
 // ---- host side ----------------------------------------------------------------------
 // The (items per chunk, units per lane) pairs that are compiled; choose() picks one.
-#define B2K_HEADS_SHAPES(CASE) CASE(1, 1) CASE(1, 4) CASE(1, 16)
+// Chunks of 8 are for 16-bit items only (16 bytes).
+#define B2K_HEADS_SHAPES(CASE) CASE(8, 1) CASE(8, 2) CASE(4, 1) CASE(4, 4) CASE(1, 1) CASE(1, 4) CASE(1, 16)
 
 struct Plan {
     int vec = 0, iter = 0;

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
 template <typename T, int MODE>
 void pick_forward(const Params &p, const Plan &plan, unsigned blocks, cudaStream_t stream) {
 #define B2K_HEADS_CASE(V, I)                                                                 \
-    if (plan.vec == V && plan.iter == I) {                                                   \
+    if constexpr (V * sizeof(T) <= 16) if (plan.vec == V && plan.iter == I) { \
         heads_forward_kernel<T, V, I, MODE><<<blocks, kThreads, 0, stream>>>(p);             \
         return;                                                                              \
     }
