@@ -262,27 +262,51 @@ Plan choose(Params &p, int64_t format, const b2k_rotation *rot) {
         if (r.units > units) units = r.units;
     }
     p.lanes = 1;
-    while (p.lanes < 32 && p.lanes < units) p.lanes *= 2;
+    p.lane_bits = 0;
+    while (p.lanes < 32 && p.lanes < units) {
+        p.lanes *= 2;
+        p.lane_bits += 1;
+    }
     const int need = (units + p.lanes - 1) / p.lanes;
 #define B2K_HEADS_PICK(V, I) \
     if (plan.vec == V && plan.iter == 0 && I >= need) plan.iter = I;
     B2K_HEADS_SHAPES(B2K_HEADS_PICK)
 #undef B2K_HEADS_PICK
+    for (Role &r : p.role) {
+        if (r.codes == nullptr) continue;
+        r.groups_of = paging::divisor(static_cast<uint32_t>(r.group));
+        // how the chunks of a scale's group lie over the lanes; see quantise_row
+        const int run = r.pair_units ? plan.vec : 2 * plan.vec;      // neighbouring items of a lane
+        const int span = r.group / run;
+        const bool even = r.group % run == 0 && (span & (span - 1)) == 0;
+        r.scale_lanes = 0;
+        r.scale_joint = r.group == r.dim || r.pair_units == 0;
+        if (r.group == r.dim) r.scale_lanes = p.lanes;
+        else if (plan.iter == 1 && even && (r.pair_units == 0 || (r.tail == r.dim && r.pair_gap % r.group == 0)))
+            r.scale_lanes = span;
+    }
     return plan;
 }
 
-int count_items(Params &p, const char *name) {
-    p.heads_per_item = 1;
-    p.items_per_token = 0;
-    int64_t per_token = 0;
+int count_items(Params &p, int most, int threads, const char *name) {
+    // Several heads an item save loads of cosines, sines and weights, but leave a small
+    // call with fewer groups than the GPU has room for.
+    int64_t rows = 0;
+    for (const Role &r : p.role) rows += r.heads;
+    rows = rows > 0 && p.tokens > INT64_MAX / 64 / rows ? INT64_MAX / 64 : rows * p.tokens;
+    p.heads_per_item = rows * p.lanes >= static_cast<int64_t>(most) * 1024 * b2k::sm_count() ? most : 1;
+    const int64_t in_block = threads / p.lanes;
+    int64_t blocks = 0;
     for (Role &r : p.role) {
-        r.items = (r.heads + p.heads_per_item - 1) / p.heads_per_item;
-        per_token += r.items;
+        const int64_t per_token = (r.heads + p.heads_per_item - 1) / p.heads_per_item;
+        if (per_token && p.tokens > INT_MAX / per_token)
+            return b2k::fail(B2K_ERR_TOO_LARGE, "%s: more than 2^31 - 1 groups of rows", name);
+        r.items = paging::divisor(static_cast<uint32_t>(per_token ? per_token : 1));
+        r.all_items = static_cast<uint32_t>(p.tokens * per_token);
+        r.blocks = static_cast<uint32_t>((p.tokens * per_token + in_block - 1) / in_block);
+        blocks += r.blocks;
     }
-    if (per_token > INT_MAX || (per_token && p.tokens > int64_t(UINT_MAX) / per_token))
-        return b2k::fail(B2K_ERR_TOO_LARGE, "%s: more than 2^32 - 1 rows", name);
-    p.items_per_token = static_cast<int>(per_token);
-    p.items = static_cast<uint32_t>(p.tokens * per_token);
+    if (blocks > INT_MAX) return b2k::fail(B2K_ERR_TOO_LARGE, "%s: too many rows for one launch", name);
     return B2K_OK;
 }
 
@@ -300,8 +324,7 @@ __global__ void __launch_bounds__(kThreads) heads_backward_kernel(const __grid_c
     const Role &r = p.role[which];
     const uint32_t first = which ? blockIdx.x - p.blocks0 : blockIdx.x;
     const uint32_t blocks = which ? gridDim.x - p.blocks0 : p.blocks0;
-    const uint32_t in_block = kThreads / g.n;
-    const int64_t items = p.tokens * r.items;
+    const uint32_t in_block = static_cast<uint32_t>(kThreads) >> p.lane_bits;
     const bool summed = r.weight_grad != nullptr;
     float sum_a[ITER][VEC] = {}, sum_b[ITER][VEC] = {};
     float wa[ITER][VEC] = {}, wb[ITER][VEC] = {};
@@ -312,11 +335,11 @@ __global__ void __launch_bounds__(kThreads) heads_backward_kernel(const __grid_c
         if (oa < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa, wa[i]);
         if (ob < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob, wb[i]);
     }
-    for (int64_t item = static_cast<int64_t>(first) * in_block + threadIdx.x / g.n; item < items;
-         item += static_cast<int64_t>(blocks) * in_block) {
-        int64_t token, rest;
-        paging::divide(item, r.items, token, rest);
-        const int part = static_cast<int>(rest);
+    // all_items < 2^31, and a step is at most the grid's groups: no overflow
+    for (uint32_t item = first * in_block + (threadIdx.x >> p.lane_bits); item < r.all_items; item += blocks * in_block) {
+        const uint32_t at_token = r.items.quotient(item);
+        const int64_t token = at_token;
+        const int part = static_cast<int>(item - at_token * r.items.d);
         int64_t position = 0;
         if (p.positions != nullptr) position = paging::load_index(p.positions, p.position_bytes, token);
         const bool padding = p.positions != nullptr && (position < 0 || position >= p.table_rows);
@@ -525,11 +548,10 @@ int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, con
     p.partials = static_cast<float *>(scratch_dev);
     set_rotation(p, *r);
     const Plan plan = choose(p, r->format, r);
-    if (int rc = count_items(p, name)) return rc;
+    if (int rc = count_items(p, 1, kThreads, name)) return rc;
     // blocks go to the two roles by their share of the rows' items, at least one to each
-    const int64_t in_block = kThreads / p.lanes;
     int64_t need[2], most = backward_blocks();
-    for (int i = 0; i < 2; ++i) need[i] = (p.tokens * p.role[i].items + in_block - 1) / in_block;
+    for (int i = 0; i < 2; ++i) need[i] = p.role[i].blocks;
     if (need[0] + need[1] > most) {
         const int64_t total = need[0] + need[1];
         int64_t first = need[0] * most / total;

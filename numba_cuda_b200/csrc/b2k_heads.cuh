@@ -18,6 +18,11 @@ namespace headwise {
 
 constexpr int kThreads = 256;
 
+// Rows of one token that a group keeps in flight: cosines, sines and weights are loaded
+// once for all of them.  Rows that spread over several units a lane leave registers for
+// fewer.
+B2K_HD constexpr int rows_in_flight(int iter) { return iter == 1 ? 4 : iter == 2 ? 2 : 1; }
+
 // One array role of a launch (queries, keys or values).
 struct Role {
     const void *in;
@@ -30,18 +35,21 @@ struct Role {
     void *scales;
     int64_t code_page, code_slot, code_head, scale_page, scale_slot, scale_head;
     int heads, dim, group;
-    int items;                  // items of work a token has in this role: ceil(heads / heads_per_item)
+    paging::Divisor items;              // items of work a token has in this role: ceil(heads / heads_per_item)
+    paging::Divisor groups_of;          // division by `group`
+    uint32_t all_items, blocks; // of the launch
     int units;                  // chunk pairs of a row
     int pair_units, pair_gap, tail;   // units below pair_units are (u, u + gap); the others lie from `tail` on
     int angle_units;            // units below it are rotated
+    int scale_lanes, scale_joint;     // lanes that share a scale (0: found through shared memory), and whether
+                                      // a lane's two chunks do
     float inv_dim;
 };
 
 struct Params {
     Role role[3];
     int64_t tokens;
-    uint32_t items;             // all items of the launch
-    int items_per_token, heads_per_item, lanes;
+    int heads_per_item, lanes, lane_bits;
     int norm, interleaved, weight_format;
     float eps;
     const float *cos_table, *sin_table;
@@ -63,10 +71,19 @@ template <> struct Convert<float> {
 template <> struct Convert<__half> {
     __device__ static float up(__half x) { return __half2float(x); }
     __device__ static __half down(float x) { return __float2half_rn(x); }
+    using Pair = __half2;
+    __device__ static __half2 down2(float lo, float hi) { return __floats2half2_rn(lo, hi); }
 };
 template <> struct Convert<__nv_bfloat16> {
-    __device__ static float up(__nv_bfloat16 x) { return __bfloat162float(x); }
+    // a bfloat16 is the upper half of a float32: a shift.  The conversion instruction runs on
+    // the quarter-rate unit that divisions and square roots use and was what bounded the
+    // first kernels (unit busy 100%, DRAM 28%).
+    __device__ static float up(__nv_bfloat16 x) {
+        return __uint_as_float(static_cast<uint32_t>(__bfloat16_as_ushort(x)) << 16);
+    }
     __device__ static __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
+    using Pair = __nv_bfloat162;
+    __device__ static __nv_bfloat162 down2(float lo, float hi) { return __floats2bfloat162_rn(lo, hi); }
 };
 
 template <typename T, int VEC>
@@ -81,9 +98,16 @@ __device__ __forceinline__ Chunk<T, VEC> load_chunk(const T *p) {
 template <typename T, int VEC>
 __device__ __forceinline__ void store_chunk(T *p, const float (&v)[VEC]) {
     Chunk<T, VEC> c;
+    if constexpr (VEC > 1 && sizeof(T) == 2) {        // two items per conversion instruction
+        Chunk<typename Convert<T>::Pair, VEC / 2> two;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) c.e[j] = Convert<T>::down(v[j]);
-    *reinterpret_cast<Chunk<T, VEC> *>(p) = c;
+        for (int j = 0; j < VEC / 2; ++j) two.e[j] = Convert<T>::down2(v[2 * j], v[2 * j + 1]);
+        *reinterpret_cast<Chunk<typename Convert<T>::Pair, VEC / 2> *>(p) = two;
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) c.e[j] = Convert<T>::down(v[j]);
+        *reinterpret_cast<Chunk<T, VEC> *>(p) = c;
+    }
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void widen(const Chunk<T, VEC> &c, float (&v)[VEC]) {
@@ -128,8 +152,9 @@ struct Lanes {
         for (int o = n >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
         return v;
     }
-    __device__ float max(float v) const {
-        for (int o = n >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
+    // over aligned runs of `span` lanes (a power of two) of the group
+    __device__ float max(float v, int span) const {
+        for (int o = span >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
         return v;
     }
 };
@@ -201,19 +226,28 @@ __device__ __forceinline__ float largest_finite(const float (&v)[VEC]) {
     return m;
 }
 
-// Scale for a largest magnitude, and its E8M0 code.  The lower bound keeps 1 / scale
-// finite and covers a row of zeros.
-__device__ __forceinline__ float scale_for(float amax, int e5m2, int e8m0, uint8_t &code) {
-    float s = fmaxf(__fdiv_rn(amax, e5m2 ? 57344.0f : 448.0f), 0x1p-126f);
-    if (e8m0) {
-        // s is a normal number: adding all mantissa bits carries into the exponent
-        // unless they are all zero, which is the power of two not below s
-        const uint32_t e = (__float_as_uint(s) + 0x007FFFFFu) >> 23;
-        code = static_cast<uint8_t>(e);
-        s = __uint_as_float(e << 23);
+// The scale of a largest magnitude, and its reciprocal.  The lower bound keeps the
+// reciprocal finite and covers a row of zeros.
+struct Scale {
+    float value, inverse;
+    __device__ Scale(float amax, int e5m2, int e8m0) {
+        value = fmaxf(__fdiv_rn(amax, e5m2 ? 57344.0f : 448.0f), 0x1p-126f);
+        if (e8m0) {
+            // a normal number: adding all mantissa bits carries into the exponent unless
+            // they are all zero, which is the power of two not below it.  Its exponent
+            // field is at most 127 + 120, so the reciprocal is a normal number, too.
+            const uint32_t e = (__float_as_uint(value) + 0x007FFFFFu) >> 23;
+            value = __uint_as_float(e << 23);
+            inverse = __uint_as_float((254u - e) << 23);
+        } else {
+            inverse = __frcp_rn(value);
+        }
     }
-    return s;
-}
+    __device__ void store(void *scales, int64_t at, int e8m0) const {
+        if (e8m0) static_cast<uint8_t *>(scales)[at] = static_cast<uint8_t>(__float_as_uint(value) >> 23);
+        else static_cast<float *>(scales)[at] = value;
+    }
+};
 
 // ---- host side ----------------------------------------------------------------------
 // The (items per chunk, units per lane) pairs that are compiled; choose() picks one.
@@ -242,7 +276,8 @@ void set_pages(Params &p, Role &r, const b2k_cache &c, const b2k_pages &side);
 void set_rotation(Params &p, const b2k_rotation &rot);
 // Chunk width from sizes, strides and addresses; lanes and unit layout of every role.
 Plan choose(Params &p, int64_t format, const b2k_rotation *rot);
-// items and heads per item; an error when they do not fit 32 bits.
-int count_items(Params &p, const char *name);
+// Items with up to `most` heads in each, and blocks of `threads` threads, of every role; an
+// error when they do not fit 31 bits.
+int count_items(Params &p, int most, int threads, const char *name);
 
 }  // namespace headwise

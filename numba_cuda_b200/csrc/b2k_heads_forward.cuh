@@ -11,56 +11,60 @@ enum Mode { kRotate = 1, kWrite = 2, kBoth = 3 };
 
 // Quantise one row held in registers into its cache slot.
 template <int VEC, int ITER>
-__device__ __forceinline__ void quantise_row(const Params &p, const Role &r, const Lanes &g,
-                                             const paging::Place &at, int head, const float (&a)[ITER][VEC],
-                                             const float (&b)[ITER][VEC], unsigned *group_max) {
+__device__ __forceinline__ void quantise_row(const Params &p, const Role &r, const Lanes &g, const paging::Place &at,
+                                             int head, const float (&a)[ITER][VEC], const float (&b)[ITER][VEC],
+                                             unsigned *group_max) {
     uint8_t *codes = r.codes + at.page * r.code_page + at.slot * r.code_slot + head * r.code_head;
     const int64_t scale_at = at.page * r.scale_page + at.slot * r.scale_slot + head * r.scale_head;
-    const bool whole = r.group == r.dim;
-    float row_scale = 1.0f, row_by = 1.0f;
-    uint8_t code = 0;
-    if (whole) {
+    int oa[ITER], ob[ITER];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) unit_at<VEC>(r, g.lane + i * g.n, oa[i], ob[i]);
+    if (r.scale_lanes && r.scale_joint) {
         float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) m = fmaxf(m, fmaxf(largest_finite<VEC>(a[i]), largest_finite<VEC>(b[i])));
-        row_scale = scale_for(g.max(m), p.e5m2, p.e8m0, code);
-        row_by = __frcp_rn(row_scale);
-        if (g.lane == 0) {
-            if (p.e8m0) static_cast<uint8_t *>(r.scales)[scale_at] = code;
-            else static_cast<float *>(r.scales)[scale_at] = row_scale;
+        const Scale s(g.max(m, r.scale_lanes), p.e5m2, p.e8m0);
+        if ((g.lane & (r.scale_lanes - 1)) == 0 && oa[0] < r.dim) s.store(r.scales, scale_at + r.groups_of.quotient(oa[0]), p.e8m0);
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            if (oa[i] < r.dim) store_codes<VEC>(codes + oa[i], a[i], s.inverse, p.e5m2);
+            if (ob[i] < r.dim) store_codes<VEC>(codes + ob[i], b[i], s.inverse, p.e5m2);
+        }
+    } else if (ITER == 1 && r.scale_lanes) {
+        const Scale sa(g.max(largest_finite<VEC>(a[0]), r.scale_lanes), p.e5m2, p.e8m0);
+        const Scale sb(g.max(largest_finite<VEC>(b[0]), r.scale_lanes), p.e5m2, p.e8m0);
+        if ((g.lane & (r.scale_lanes - 1)) == 0 && oa[0] < r.dim) {
+            sa.store(r.scales, scale_at + r.groups_of.quotient(oa[0]), p.e8m0);
+            sb.store(r.scales, scale_at + r.groups_of.quotient(ob[0]), p.e8m0);
+        }
+        if (oa[0] < r.dim) {
+            store_codes<VEC>(codes + oa[0], a[0], sa.inverse, p.e5m2);
+            store_codes<VEC>(codes + ob[0], b[0], sb.inverse, p.e5m2);
         }
     } else {
-        // the magnitudes' bit patterns are ordered like the magnitudes
+        // any other layout of groups: the magnitudes' bit patterns are ordered like the
+        // magnitudes, so an integer maximum in shared memory finds them
+        const int groups = r.groups_of.quotient(r.dim);
         __syncwarp(g.mask);
-        for (int k = g.lane; k < r.dim / r.group; k += g.n) group_max[k] = 0u;
+        for (int k = g.lane; k < groups; k += g.n) group_max[k] = 0u;
         __syncwarp(g.mask);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            int oa, ob;
-            unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
-            if (oa < r.dim) atomicMax(&group_max[oa / r.group], __float_as_uint(largest_finite<VEC>(a[i])));
-            if (ob < r.dim) atomicMax(&group_max[ob / r.group], __float_as_uint(largest_finite<VEC>(b[i])));
+            if (oa[i] < r.dim) atomicMax(&group_max[r.groups_of.quotient(oa[i])], __float_as_uint(largest_finite<VEC>(a[i])));
+            if (ob[i] < r.dim) atomicMax(&group_max[r.groups_of.quotient(ob[i])], __float_as_uint(largest_finite<VEC>(b[i])));
         }
         __syncwarp(g.mask);
-        for (int k = g.lane; k < r.dim / r.group; k += g.n) {
-            const float s = scale_for(__uint_as_float(group_max[k]), p.e5m2, p.e8m0, code);
-            if (p.e8m0) static_cast<uint8_t *>(r.scales)[scale_at + k] = code;
-            else static_cast<float *>(r.scales)[scale_at + k] = s;
-        }
-    }
+        for (int k = g.lane; k < groups; k += g.n)
+            Scale(__uint_as_float(group_max[k]), p.e5m2, p.e8m0).store(r.scales, scale_at + k, p.e8m0);
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        int oa, ob;
-        unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
-        float by_a = row_by, by_b = row_by;
-        if (!whole) {
-            if (oa < r.dim)
-                by_a = __frcp_rn(scale_for(__uint_as_float(group_max[oa / r.group]), p.e5m2, p.e8m0, code));
-            if (ob < r.dim)
-                by_b = __frcp_rn(scale_for(__uint_as_float(group_max[ob / r.group]), p.e5m2, p.e8m0, code));
+        for (int i = 0; i < ITER; ++i) {
+            if (oa[i] < r.dim)
+                store_codes<VEC>(codes + oa[i], a[i],
+                                 Scale(__uint_as_float(group_max[r.groups_of.quotient(oa[i])]), p.e5m2, p.e8m0).inverse, p.e5m2);
+            if (ob[i] < r.dim)
+                store_codes<VEC>(codes + ob[i], b[i],
+                                 Scale(__uint_as_float(group_max[r.groups_of.quotient(ob[i])]), p.e5m2, p.e8m0).inverse, p.e5m2);
         }
-        if (oa < r.dim) store_codes<VEC>(codes + oa, a[i], by_a, p.e5m2);
-        if (ob < r.dim) store_codes<VEC>(codes + ob, b[i], by_b, p.e5m2);
     }
 }
 
@@ -68,27 +72,47 @@ template <typename T, int VEC, int ITER, int MODE>
 __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_constant__ Params p) {
     // groups of a scale are at least 16 items, so a lane's share of a row has at most this many
     constexpr int kGroupsPerLane = (2 * VEC * ITER + 15) / 16;
+    constexpr int kRows = rows_in_flight(ITER);
     __shared__ unsigned group_max[MODE == kRotate ? 1 : kThreads * kGroupsPerLane];
-    const Lanes g(p.lanes);
-    const uint32_t in_block = static_cast<uint32_t>(kThreads) / static_cast<uint32_t>(g.n);
-    const uint64_t wide = static_cast<uint64_t>(blockIdx.x) * in_block + threadIdx.x / static_cast<uint32_t>(g.n);
-    if (wide >= p.items) return;                      // whole groups
-    const uint32_t item = static_cast<uint32_t>(wide);
-    const int64_t token = item / static_cast<uint32_t>(p.items_per_token);
-    int part = static_cast<int>(item % static_cast<uint32_t>(p.items_per_token));
+    // A block works for one role, so the role's members are uniform over the block.
+    uint32_t block = blockIdx.x;
     int which = 0;
-    while (part >= p.role[which].items) part -= p.role[which++].items;
+    while (block >= p.role[which].blocks) block -= p.role[which++].blocks;
     const Role &r = p.role[which];
+    const Lanes g(p.lanes);
+    const uint32_t item = block * (static_cast<uint32_t>(kThreads) >> p.lane_bits) + (threadIdx.x >> p.lane_bits);
+    if (item >= r.all_items) return;                  // whole groups
+    const uint32_t at_token = r.items.quotient(item);
+    const int64_t token = at_token;
+    const int part = static_cast<int>(item - at_token * r.items.d);
+    const int first = part * p.heads_per_item;
+    const int rows = min(r.heads - first, p.heads_per_item);
+    int oa[ITER], ob[ITER];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) unit_at<VEC>(r, g.lane + i * g.n, oa[i], ob[i]);
 
-    int64_t position = 0;
+    // The rows' loads go first: they do not wait for the token's position and slot.
+    Chunk<T, VEC> ca[kRows][ITER], cb[kRows][ITER];
+    const T *in = static_cast<const T *>(r.in) + token * r.in_token + first * r.in_head;
+#pragma unroll
+    for (int h = 0; h < kRows; ++h)
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            ca[h][i] = cb[h][i] = Chunk<T, VEC>{};
+            if (h < rows && oa[i] < r.dim) ca[h][i] = load_chunk<T, VEC>(in + h * r.in_head + oa[i]);
+            if (h < rows && ob[i] < r.dim) cb[h][i] = load_chunk<T, VEC>(in + h * r.in_head + ob[i]);
+        }
+
+    const bool quantised = MODE == kWrite || (MODE == kBoth && r.out == nullptr);
+    int64_t position = 0, slot = 0;
+    if (quantised) slot = paging::load_index(p.slots, p.slot_bytes, token);
     if ((MODE & kRotate) && p.positions != nullptr) {
         position = paging::load_index(p.positions, p.position_bytes, token);
         if (position < 0 || position >= p.table_rows) return;
     }
-    const bool quantised = MODE == kWrite || (MODE == kBoth && r.out == nullptr);
     paging::Place at{0, 0, false};
     if (quantised) {
-        at = paging::place_of_slot(paging::load_index(p.slots, p.slot_bytes, token), p.pages, p.page_size);
+        at = paging::place_of_slot(slot, p.pages, p.page_size);
         if (!at.ok) return;
     }
     const bool normed = (MODE & kRotate) && p.norm && which < 2;
@@ -103,27 +127,20 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
                 load_floats<VEC>(p.sin_table + position * p.sin_stride + u * VEC, s[i]);
             }
             if (normed) {
-                int oa, ob;
-                unit_at<VEC>(r, u, oa, ob);
-                if (oa < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa, wa[i]);
-                if (ob < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob, wb[i]);
+                if (oa[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa[i], wa[i]);
+                if (ob[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob[i], wb[i]);
             }
         }
     }
 
-    const int last = min(r.heads, (part + 1) * p.heads_per_item);
-    for (int head = part * p.heads_per_item; head < last; ++head) {
-        const T *in = static_cast<const T *>(r.in) + token * r.in_token + head * r.in_head;
+#pragma unroll
+    for (int h = 0; h < kRows; ++h) {
+        if (h >= rows) break;
         float a[ITER][VEC], b[ITER][VEC];
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            int oa, ob;
-            unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
-            Chunk<T, VEC> ca{}, cb{};
-            if (oa < r.dim) ca = load_chunk<T, VEC>(in + oa);
-            if (ob < r.dim) cb = load_chunk<T, VEC>(in + ob);
-            widen(ca, a[i]);
-            widen(cb, b[i]);
+            widen(ca[h][i], a[i]);
+            widen(cb[h][i], b[i]);
         }
         if constexpr ((MODE & kRotate) != 0) {
             if (normed) {
@@ -146,16 +163,14 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
                 if (g.lane + i * g.n < r.angle_units) rotate<VEC>(a[i], b[i], c[i], s[i], p.interleaved);
         }
         if (!quantised) {
-            T *out = static_cast<T *>(r.out) + token * r.out_token + head * r.out_head;
+            T *out = static_cast<T *>(r.out) + token * r.out_token + (first + h) * r.out_head;
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
-                int oa, ob;
-                unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
-                if (oa < r.dim) store_chunk<T, VEC>(out + oa, a[i]);
-                if (ob < r.dim) store_chunk<T, VEC>(out + ob, b[i]);
+                if (oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a[i]);
+                if (ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b[i]);
             }
         } else if constexpr (MODE != kRotate) {
-            quantise_row<VEC, ITER>(p, r, g, at, head, a, b,
+            quantise_row<VEC, ITER>(p, r, g, at, first + h, a, b,
                                     group_max + (threadIdx.x & ~(g.n - 1)) * kGroupsPerLane);
         }
     }
@@ -176,14 +191,12 @@ void pick_forward(const Params &p, const Plan &plan, unsigned blocks, cudaStream
 // Launches over all items; the roles, tokens and tables of `p` are set.
 template <int MODE>
 int launch_forward(Params &p, int64_t format, const Plan &plan, cudaStream_t stream, const char *name) {
-    if (int rc = count_items(p, name)) return rc;
-    const int64_t in_block = kThreads / p.lanes;
-    const int64_t blocks = (static_cast<int64_t>(p.items) + in_block - 1) / in_block;
+    if (int rc = count_items(p, rows_in_flight(plan.iter), kThreads, name)) return rc;
+    const unsigned blocks = p.role[0].blocks + p.role[1].blocks + p.role[2].blocks;
     if (blocks == 0) return B2K_OK;
-    if (blocks > INT_MAX) return b2k::fail(B2K_ERR_TOO_LARGE, "%s: too many rows for one launch", name);
-    if (format == B2K_FMT_F32) pick_forward<float, MODE>(p, plan, static_cast<unsigned>(blocks), stream);
-    else if (format == B2K_FMT_F16) pick_forward<__half, MODE>(p, plan, static_cast<unsigned>(blocks), stream);
-    else pick_forward<__nv_bfloat16, MODE>(p, plan, static_cast<unsigned>(blocks), stream);
+    if (format == B2K_FMT_F32) pick_forward<float, MODE>(p, plan, blocks, stream);
+    else if (format == B2K_FMT_F16) pick_forward<__half, MODE>(p, plan, blocks, stream);
+    else pick_forward<__nv_bfloat16, MODE>(p, plan, blocks, stream);
     B2K_RETURN_IF_LAUNCH_FAILED(name);
     b2k::note_launch();
     return B2K_OK;

@@ -23,23 +23,38 @@ struct ReadParams {
     const void *table, *offsets;
     int64_t table_stride, table_width, seqs;
     int table_bytes, offset_bytes, e5m2, e8m0;
+    int tile;                       // output rows a block owns, at most kTileRows
 };
 
-template <typename T> struct Largest;
-template <> struct Largest<float> { static constexpr float value = FLT_MAX; };
-template <> struct Largest<__half> { static constexpr float value = 65504.0f; };
-template <> struct Largest<__nv_bfloat16> { static constexpr float value = 3.38953138925153547590470800371487866880e38f; };
+// ---- reading back ---------------------------------------------------------------------
+// A block owns a tile of consecutive output rows of one side.  Its first threads find
+// each row's place (a binary search over the offsets, one page-table entry); then every
+// thread keeps one chunk of CV items of a row and walks down the tile's rows with
+// kReadRows loads in flight, so index arithmetic is paid once a thread.  HBM bounds it:
+// one byte in, sizeof(T) bytes out per item.
+constexpr int kTileRows = 32;
+constexpr int kReadRows = 4;
 
-__device__ __forceinline__ float decode(uint8_t code, int e5m2) {
+template <int E5M2>
+__device__ __forceinline__ float2 decode2(uint16_t two_codes) {
     uint32_t two;
-    if (e5m2) asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(two) : "h"(static_cast<uint16_t>(code)));
-    else asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"(static_cast<uint16_t>(code)));
-    return __half2float(__ushort_as_half(static_cast<uint16_t>(two)));
+    if constexpr (E5M2) asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(two) : "h"(two_codes));
+    else asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"(two_codes));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&two));
 }
-// A value beyond the output's range is its largest one; a NaN stays.
-template <typename T>
-__device__ __forceinline__ float saturated(float v) {
-    return fabsf(v) > Largest<T>::value ? copysignf(Largest<T>::value, v) : v;
+
+// Store with saturation to the type's finite range; a NaN stays one.
+__device__ __forceinline__ float saturated(float v) { return fabsf(v) > FLT_MAX ? copysignf(FLT_MAX, v) : v; }
+template <typename T> __device__ __forceinline__ uint32_t pack2_saturated(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2_saturated<__half>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t pack2_saturated<__nv_bfloat16>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
 __device__ __forceinline__ float load_scale(const void *scales, int64_t at, int e8m0) {
@@ -49,27 +64,126 @@ __device__ __forceinline__ float load_scale(const void *scales, int64_t at, int 
     return __uint_as_float(e == 0 ? 0x00400000u : e == 255 ? 0x7FC00000u : e << 23);
 }
 
-// One warp per row of the output (a token of one side), lanes along its items.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ ReadParams p) {
-    const ReadSide &s = p.side[blockIdx.y];
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32;
-    if (row >= p.rows || s.heads == 0) return;
-    const int64_t b = paging::sequence_of_row(p.offsets, p.offset_bytes, p.seqs, row);
-    if (b < 0) return;
-    const paging::Place at = paging::place_in_sequence(row - paging::load_index(p.offsets, p.offset_bytes, b),
-                                                             p.table, p.table_stride, p.table_width, p.table_bytes, b,
-                                                             p.pages, p.page_size);
-    for (int head = 0; head < s.heads; ++head) {
-        T *out = static_cast<T *>(s.out) + row * s.out_token + head * s.out_head;
-        const uint8_t *codes = s.codes + at.page * s.code_page + at.slot * s.code_slot + head * s.code_head;
-        const int64_t scales = at.page * s.scale_page + at.slot * s.scale_slot + head * s.scale_head;
-        for (int d = threadIdx.x % 32; d < s.dim; d += 32) {
-            float v = 0.0f;
-            if (at.ok) v = saturated<T>(decode(codes[d], p.e5m2) * load_scale(s.scales, scales + d / s.group, p.e8m0));
-            out[d] = Convert<T>::down(v);
+// N consecutive items at p, N * sizeof(T) <= 32 bytes and p aligned to it.
+template <typename T, int N>
+__device__ __forceinline__ void store_items(T *p, const float (&v)[N]) {
+    if constexpr (N == 1) {
+        if constexpr (sizeof(T) == 4) *p = saturated(v[0]);
+        else *reinterpret_cast<uint16_t *>(p) = static_cast<uint16_t>(pack2_saturated<T>(v[0], 0.0f));
+    } else {
+        constexpr int W = N * sizeof(T) / 4;
+        Chunk<uint32_t, W> w;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) w.e[j] = __float_as_uint(saturated(v[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) w.e[j] = pack2_saturated<T>(v[2 * j], v[2 * j + 1]);
+        }
+        if constexpr (W == 8) {                    // sm_100's 256-bit store
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w.e[0]), "r"(w.e[1]),
+                         "r"(w.e[2]), "r"(w.e[3]), "r"(w.e[4]), "r"(w.e[5]), "r"(w.e[6]), "r"(w.e[7])
+                         : "memory");
+        } else {
+            *reinterpret_cast<Chunk<uint32_t, W> *>(p) = w;
         }
     }
+}
+
+template <typename T, int CV, int E5M2>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ ReadParams p) {
+    const ReadSide &s = p.side[blockIdx.y];
+    if (s.heads == 0) return;
+    __shared__ int64_t code_at[kTileRows], scale_at[kTileRows];
+    __shared__ int state[kTileRows];               // 0: no row of a sequence, 1: zeros, 2: codes
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tile;
+    if (threadIdx.x < p.tile) {
+        const int64_t row = first + threadIdx.x;
+        int now = 0;
+        if (row < p.rows) {
+            const int64_t b = paging::sequence_of_row(p.offsets, p.offset_bytes, p.seqs, row);
+            if (b >= 0) {
+                const paging::Place at = paging::place_in_sequence(
+                    row - paging::load_index(p.offsets, p.offset_bytes, b), p.table, p.table_stride, p.table_width,
+                    p.table_bytes, b, p.pages, p.page_size);
+                now = at.ok ? 2 : 1;
+                code_at[threadIdx.x] = at.page * s.code_page + at.slot * s.code_slot;
+                scale_at[threadIdx.x] = at.page * s.scale_page + at.slot * s.scale_slot;
+            }
+        }
+        state[threadIdx.x] = now;
+    }
+    __syncthreads();
+    const int chunks = s.dim / CV, units = s.heads * chunks;          // chunks of a row's heads
+    const int down = units < kThreads ? kThreads / units : 1;         // rows the block's threads cover at once
+    const int across = units < kThreads ? units : kThreads;
+    const int t0 = threadIdx.x / across;
+    if (t0 >= down) return;
+    for (int u = threadIdx.x - t0 * across; u < units; u += across) {
+        const int head = u / chunks, d = (u - head * chunks) * CV;
+        const uint8_t *codes = s.codes + head * s.code_head + d;
+        const int64_t scales = head * s.scale_head + d / s.group;
+        T *out = static_cast<T *>(s.out) + first * s.out_token + head * s.out_head + d;
+        for (int t = t0; t < p.tile; t += kReadRows * down) {
+            Chunk<uint8_t, CV> c[kReadRows];
+            float scale[kReadRows];
+            int now[kReadRows];
+#pragma unroll
+            for (int i = 0; i < kReadRows; ++i) {
+                const int at = t + i * down;
+                c[i] = Chunk<uint8_t, CV>{};
+                scale[i] = 0.0f;
+                now[i] = at < p.tile ? state[at] : 0;
+                if (now[i] == 2) {
+                    c[i] = load_chunk<uint8_t, CV>(codes + code_at[at]);
+                    scale[i] = load_scale(s.scales, scales + scale_at[at], p.e8m0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kReadRows; ++i) {
+                if (now[i] == 0) continue;
+                float v[CV];
+                if constexpr (CV == 1) {
+                    v[0] = decode2<E5M2>(c[i].e[0]).x * scale[i];
+                } else {
+                    const Chunk<uint16_t, CV / 2> two = *reinterpret_cast<const Chunk<uint16_t, CV / 2> *>(&c[i]);
+#pragma unroll
+                    for (int j = 0; j < CV / 2; ++j) {
+                        const float2 f = decode2<E5M2>(two.e[j]);
+                        v[2 * j] = f.x * scale[i];
+                        v[2 * j + 1] = f.y * scale[i];
+                    }
+                }
+                store_items<T, CV>(out + (t + i * down) * s.out_token, v);
+            }
+        }
+    }
+}
+
+template <typename T, int CV>
+void launch_read(const ReadParams &p, dim3 grid, cudaStream_t stream) {
+    if (p.e5m2) cache_read_kernel<T, CV, 1><<<grid, kThreads, 0, stream>>>(p);
+    else cache_read_kernel<T, CV, 0><<<grid, kThreads, 0, stream>>>(p);
+}
+
+// Widest chunk that sizes, strides and addresses of both sides allow: 32 bytes of output
+// at most.
+template <typename T>
+void pick_read(const ReadParams &p, dim3 grid, cudaStream_t stream) {
+    const auto fits = [&](int cv) {
+        for (const ReadSide &s : p.side) {
+            if (s.heads == 0) continue;
+            if (s.dim % cv || s.group % cv) return false;
+            if ((reinterpret_cast<uintptr_t>(s.codes) | s.code_page | s.code_slot | s.code_head) % cv) return false;
+            if (reinterpret_cast<uintptr_t>(s.out) % (cv * sizeof(T)) || (s.out_token | s.out_head) % cv) return false;
+        }
+        return true;
+    };
+    if constexpr (sizeof(T) == 2)
+        if (fits(16)) return launch_read<T, 16>(p, grid, stream);
+    if (fits(8)) return launch_read<T, 8>(p, grid, stream);
+    if (fits(4)) return launch_read<T, 4>(p, grid, stream);
+    launch_read<T, 1>(p, grid, stream);
 }
 
 int check_slots(const void *slots, int slot_bytes, int64_t tokens, const char *name) {
@@ -185,13 +299,16 @@ int b2k_cache_read(const b2k_cache *cache, int format, int64_t rows, const b2k_h
     p.offset_bytes = offset_bytes;
     p.e5m2 = cache->code_format == B2K_FMT_E5M2;
     p.e8m0 = cache->scale_format == B2K_FMT_E8M0;
-    const int64_t blocks = (rows + kThreads / 32 - 1) / (kThreads / 32);
+    // smaller tiles where whole ones would leave SMs without a block
+    p.tile = kTileRows;
+    while (p.tile > 4 && rows / p.tile < b2k::sm_count()) p.tile /= 2;
+    const int64_t blocks = (rows + p.tile - 1) / p.tile;
     if (blocks > INT_MAX) return b2k::fail(B2K_ERR_TOO_LARGE, "%s: too many rows for one launch", name);
-    const dim3 grid(static_cast<unsigned>(blocks), 2);
+    const dim3 grid(static_cast<unsigned>(blocks), v_out->heads ? 2 : 1);
     const cudaStream_t st = b2k::as_stream(stream);
-    if (format == B2K_FMT_F32) cache_read_kernel<float><<<grid, kThreads, 0, st>>>(p);
-    else if (format == B2K_FMT_F16) cache_read_kernel<__half><<<grid, kThreads, 0, st>>>(p);
-    else cache_read_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(p);
+    if (format == B2K_FMT_F32) pick_read<float>(p, grid, st);
+    else if (format == B2K_FMT_F16) pick_read<__half>(p, grid, st);
+    else pick_read<__nv_bfloat16>(p, grid, st);
     B2K_RETURN_IF_LAUNCH_FAILED(name);
     b2k::note_launch();
     return B2K_OK;

@@ -1,5 +1,5 @@
-// Index arithmetic of the paged cache: slot -> (page, place) and output row -> (page,
-// place).  Plain C++ apart from the function qualifiers, so that every guard below is
+// Index arithmetic of the head-wise kernels and the paged cache: division by a launch's
+// constants, slot -> (page, place) and output row -> (page, place).  Plain C++ apart from the function qualifiers, so that every guard below is
 // also compiled and tested on the host.  No function reads outside the arrays it is
 // given, whatever the indices in them say.
 #pragma once
@@ -13,6 +13,19 @@
 #endif
 
 namespace paging {
+
+// Division of n < 2^31 by a constant of the launch: with s = ceil(log2 d) and
+// m = ceil(2^(31 + s) / d), which fits 32 bits, floor(n m / 2^(31 + s)) = floor(n / d),
+// because m d - 2^(31 + s) < 2^s keeps the error of n m / 2^(31 + s) below 1 / d.
+struct Divisor {
+    uint32_t d, m, shift;
+    B2K_HD uint32_t quotient(uint32_t n) const { return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift); }
+};
+inline Divisor divisor(uint32_t d) {
+    uint32_t s = 0;
+    while (s < 31 && (1u << s) < d) ++s;
+    return Divisor{d, static_cast<uint32_t>(((uint64_t(1) << (31 + s)) + d - 1) / d), 31 + s};
+}
 
 struct Place {
     int64_t page, slot;

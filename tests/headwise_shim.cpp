@@ -38,3 +38,5 @@ int shim_place_in_sequence(int64_t position, const void *table, int64_t stride, 
     return at.ok;
 }
 }
+
+extern "C" uint32_t shim_quotient(uint32_t n, uint32_t d) { return paging::divisor(d).quotient(n); }

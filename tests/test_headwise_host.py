@@ -39,6 +39,16 @@ def test_packed_structs_have_the_layout_of_the_header(shim):
     assert shim.shim_size(3) == 13 * 8 and shim.shim_size(4) == ops.ROTATION.size - 16 and shim.shim_size(5) == 15 * 8
 
 
+def test_division_by_a_constant(shim):
+    rng = np.random.default_rng(0)
+    shim.shim_quotient.restype, shim.shim_quotient.argtypes = ctypes.c_uint32, [ctypes.c_uint32] * 2
+    for d in [*range(1, 70), 127, 128, 1000, 1023, 1024, 65535, 65537, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1]:
+        edge = [k * d + e for k in (0, 1, 2, (2 ** 31 - 1) // d) for e in (-1, 0, 1)] + [2 ** 31 - 1]
+        for n in [*edge, *rng.integers(0, 2 ** 31, 40).tolist()]:
+            if 0 <= n < 2 ** 31:
+                assert shim.shim_quotient(n, d) == n // d, (n, d)
+
+
 @pytest.mark.parametrize("pages,page_size", [(1, 1), (5, 16), (7, 17), (2 ** 20, 2 ** 14), (2 ** 33, 3), (0, 16)])
 def test_place_of_slot(shim, pages, page_size):
     page, place = ctypes.c_int64(), ctypes.c_int64()
