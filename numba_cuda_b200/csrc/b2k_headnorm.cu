@@ -289,12 +289,15 @@ Plan choose(Params &p, int64_t format, const b2k_rotation *rot) {
 }
 
 int count_items(Params &p, int most, int threads, const char *name) {
-    // Several heads an item save loads of cosines, sines and weights, but leave a small
-    // call with fewer groups than the GPU has room for.
+    // Several heads an item save loads of cosines, sines and weights and keep loads in
+    // flight behind the arithmetic, but leave a small call with fewer groups than the GPU
+    // has room for: halved until 1024 threads an SM have work.
     int64_t rows = 0;
     for (const Role &r : p.role) rows += r.heads;
     rows = rows > 0 && p.tokens > INT64_MAX / 64 / rows ? INT64_MAX / 64 : rows * p.tokens;
-    p.heads_per_item = rows * p.lanes >= static_cast<int64_t>(most) * 1024 * b2k::sm_count() ? most : 1;
+    p.heads_per_item = most;
+    while (p.heads_per_item > 1 && rows * p.lanes / p.heads_per_item < static_cast<int64_t>(1024) * b2k::sm_count())
+        p.heads_per_item /= 2;
     const int64_t in_block = threads / p.lanes;
     int64_t blocks = 0;
     for (Role &r : p.role) {
@@ -315,6 +318,16 @@ int count_items(Params &p, int most, int threads, const char *name) {
 // registers; each block writes one row of partials, and a second kernel adds the rows
 // in order: no atomics, so equal calls give equal bits.
 constexpr int kBackwardBlocksPerSm = 4;
+
+template <int VEC>
+__device__ __forceinline__ void rotate(float (&x)[VEC], float (&y)[VEC], const float (&c)[VEC], const float (&s)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const float u = x[j] * c[j] - y[j] * s[j], v = y[j] * c[j] + x[j] * s[j];
+        x[j] = u;
+        y[j] = v;
+    }
+}
 
 template <typename T, int VEC, int ITER>
 __global__ void __launch_bounds__(kThreads) heads_backward_kernel(const __grid_constant__ Params p) {
@@ -383,7 +396,16 @@ __global__ void __launch_bounds__(kThreads) heads_backward_kernel(const __grid_c
             float ss = 0.0f, dot = 0.0f;
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
-                if (g.lane + i * g.n < r.angle_units) rotate<VEC>(ga[i], gb[i], c[i], s[i], p.interleaved);
+                if (g.lane + i * g.n < r.angle_units) {
+                    if (p.interleaved) {
+                        float x[VEC], y[VEC];
+                        pair<VEC>(ga[i], gb[i], x, y);
+                        rotate<VEC>(x, y, c[i], s[i]);
+                        unpair<VEC>(x, y, ga[i], gb[i]);
+                    } else {
+                        rotate<VEC>(ga[i], gb[i], c[i], s[i]);
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     ss += xa[i][j] * xa[i][j] + xb[i][j] * xb[i][j];

@@ -16,12 +16,13 @@
 
 namespace headwise {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
-// Rows of one token that a group keeps in flight: cosines, sines and weights are loaded
-// once for all of them.  Rows that spread over several units a lane leave registers for
-// fewer.
-B2K_HD constexpr int rows_in_flight(int iter) { return iter == 1 ? 4 : iter == 2 ? 2 : 1; }
+// Rows of one token that a group has in flight at once, and in all: cosines, sines and
+// weights are loaded once for the latter.  Rows that spread over several units a lane
+// leave registers for one.
+B2K_HD constexpr int rows_in_flight(int iter) { return iter == 1 ? 2 : 1; }
+constexpr int kHeadsPerItem = 8;
 
 // One array role of a launch (queries, keys or values).
 struct Role {
@@ -63,56 +64,97 @@ struct Params {
     int blocks0;                // backward: blocks of role 0
 };
 
-template <typename T> struct Convert;
-template <> struct Convert<float> {
-    __device__ static float up(float x) { return x; }
-    __device__ static float down(float x) { return x; }
-};
-template <> struct Convert<__half> {
-    __device__ static float up(__half x) { return __half2float(x); }
-    __device__ static __half down(float x) { return __float2half_rn(x); }
-    using Pair = __half2;
-    __device__ static __half2 down2(float lo, float hi) { return __floats2half2_rn(lo, hi); }
-};
-template <> struct Convert<__nv_bfloat16> {
-    // a bfloat16 is the upper half of a float32: a shift.  The conversion instruction runs on
-    // the quarter-rate unit that divisions and square roots use and was what bounded the
-    // first kernels (unit busy 100%, DRAM 28%).
-    __device__ static float up(__nv_bfloat16 x) {
-        return __uint_as_float(static_cast<uint32_t>(__bfloat16_as_ushort(x)) << 16);
-    }
-    __device__ static __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
-    using Pair = __nv_bfloat162;
-    __device__ static __nv_bfloat162 down2(float lo, float hi) { return __floats2bfloat162_rn(lo, hi); }
-};
+// Moves go by whole words: 1, 2, 4, 8 or 16 bytes as one access.
+template <int BYTES> struct WordOf;
+template <> struct WordOf<1> { using type = uint8_t; };
+template <> struct WordOf<2> { using type = uint16_t; };
+template <> struct WordOf<4> { using type = uint32_t; };
+template <> struct WordOf<8> { using type = uint2; };
+template <> struct WordOf<16> { using type = uint4; };
 
+// VEC items of type T as loaded.
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Chunk {
-    T e[VEC];
+union Chunk {
+    using Word = typename WordOf<sizeof(T) * VEC>::type;
+    Word all;
+    uint32_t word[sizeof(T) * VEC < 4 ? 1 : sizeof(T) * VEC / 4];
 };
 
 template <typename T, int VEC>
 __device__ __forceinline__ Chunk<T, VEC> load_chunk(const T *p) {
-    return *reinterpret_cast<const Chunk<T, VEC> *>(p);
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store_chunk(T *p, const float (&v)[VEC]) {
     Chunk<T, VEC> c;
-    if constexpr (VEC > 1 && sizeof(T) == 2) {        // two items per conversion instruction
-        Chunk<typename Convert<T>::Pair, VEC / 2> two;
+    c.all = *reinterpret_cast<const typename Chunk<T, VEC>::Word *>(p);
+    return c;
+}
+
+__device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t *>(&v); }
+__device__ __forceinline__ uint32_t bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t *>(&v); }
+
+// float32 <-> T.  A bfloat16 is the upper half of a float32, so it is widened by a shift
+// or a mask.
+template <typename T> struct Convert;
+template <> struct Convert<float> {
+    __device__ static float down(float x) { return x; }
+};
+template <> struct Convert<__half> {
+    __device__ static float2 up2(uint32_t two) { return __half22float2(*reinterpret_cast<const __half2 *>(&two)); }
+    __device__ static __half down(float x) { return __float2half_rn(x); }
+    __device__ static uint32_t down2(float lo, float hi) { return bits(__floats2half2_rn(lo, hi)); }
+};
+template <> struct Convert<__nv_bfloat16> {
+    __device__ static float2 up2(uint32_t two) {
+        return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xFFFF0000u));
+    }
+    __device__ static __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
+    __device__ static uint32_t down2(float lo, float hi) { return bits(__floats2bfloat162_rn(lo, hi)); }
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Chunk<T, VEC> &c, float (&v)[VEC]) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) two.e[j] = Convert<T>::down2(v[2 * j], v[2 * j + 1]);
-        *reinterpret_cast<Chunk<typename Convert<T>::Pair, VEC / 2> *>(p) = two;
+        for (int j = 0; j < VEC; ++j) v[j] = __uint_as_float(c.word[j]);
+    } else if constexpr (VEC == 1) {
+        v[0] = Convert<T>::up2(c.all).x;
     } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) c.e[j] = Convert<T>::down(v[j]);
-        *reinterpret_cast<Chunk<T, VEC> *>(p) = c;
+        for (int j = 0; j < VEC / 2; ++j) {
+            const float2 f = Convert<T>::up2(c.word[j]);
+            v[2 * j] = f.x;
+            v[2 * j + 1] = f.y;
+        }
     }
 }
 template <typename T, int VEC>
-__device__ __forceinline__ void widen(const Chunk<T, VEC> &c, float (&v)[VEC]) {
+__device__ __forceinline__ void store_chunk(T *p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        *p = Convert<T>::down(v[0]);
+    } else {
+        Chunk<T, VEC> c;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = Convert<T>::up(c.e[j]);
+            for (int j = 0; j < VEC; ++j) c.word[j] = __float_as_uint(v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) c.word[j] = Convert<T>::down2(v[2 * j], v[2 * j + 1]);
+        }
+        *reinterpret_cast<typename Chunk<T, VEC>::Word *>(p) = c.all;
+    }
+}
+
+// Two float32 operations in one instruction (sm_100).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{.reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x;}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 x, x, y, z; "
+        "mov.b64 {%0, %1}, x;}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
 }
 
 template <int VEC>
@@ -122,7 +164,7 @@ __device__ __forceinline__ void load_floats(const float *p, float (&v)[VEC]) {
     for (int j = 0; j < VEC; j += W) {
         const Chunk<float, W> c = load_chunk<float, W>(p + j);
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[j + i] = c.e[i];
+        for (int i = 0; i < W; ++i) v[j + i] = __uint_as_float(c.word[i]);
     }
 }
 
@@ -171,27 +213,76 @@ __device__ __forceinline__ void unit_at(const Role &r, int u, int &a, int &b) {
     if (u >= r.units) a = b = r.dim;       // nothing
 }
 
-// Rotation of a unit by its angles (VEC == 1: a pair is always the unit's two items).
+// Items of a chunk pair as they meet in a rotation: pair j of a unit is (a[j], b[j]), or
+// neighbouring items of one chunk when interleaved (VEC == 1: always the unit's two
+// items).  `pair` copies the items into that order and `unpair` back; the copies are
+// register names, not instructions.
 template <int VEC>
-__device__ __forceinline__ void rotate(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC],
-                                       bool interleaved) {
-    if (VEC == 1 || !interleaved) {
+__device__ __forceinline__ void pair(const float (&a)[VEC], const float (&b)[VEC], float (&x)[VEC], float (&y)[VEC]) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float x = a[j], y = b[j];
-            a[j] = x * c[j] - y * s[j];
-            b[j] = y * c[j] + x * s[j];
-        }
-    } else if constexpr (VEC > 1) {
+    for (int j = 0; j < VEC; ++j) {
+        const float *from = 2 * j < VEC ? a : b;
+        const int at = 2 * j < VEC ? 2 * j : 2 * j - VEC;
+        x[j] = VEC == 1 ? a[0] : from[at];
+        y[j] = VEC == 1 ? b[0] : from[at + (VEC > 1)];
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void unpair(const float (&x)[VEC], const float (&y)[VEC], float (&a)[VEC], float (&b)[VEC]) {
 #pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) {
-            float x = a[2 * j], y = a[2 * j + 1];
-            a[2 * j] = x * c[j] - y * s[j];
-            a[2 * j + 1] = y * c[j] + x * s[j];
-            x = b[2 * j], y = b[2 * j + 1];
-            b[2 * j] = x * c[VEC / 2 + j] - y * s[VEC / 2 + j];
-            b[2 * j + 1] = y * c[VEC / 2 + j] + x * s[VEC / 2 + j];
+    for (int j = 0; j < VEC; ++j) {
+        float *to = 2 * j < VEC ? a : b;
+        const int at = 2 * j < VEC ? 2 * j : 2 * j - VEC;
+        if (VEC == 1) {
+            a[0] = x[0];
+            b[0] = y[0];
+        } else {
+            to[at] = x[j];
+            to[at + (VEC > 1)] = y[j];
         }
+    }
+}
+
+// (x, y) -> (x k0 - y k1, y k2 + x k3), `scale` times: rotation, weights and norm of a
+// pair in one step, with k0 = w_x cos, k1 = w_y sin, k2 = w_y cos, k3 = w_x sin.
+template <int VEC>
+__device__ __forceinline__ void turn(float (&x)[VEC], float (&y)[VEC], const float (&k0)[VEC], const float (&k1)[VEC],
+                                     const float (&k2)[VEC], const float (&k3)[VEC], float scale) {
+    if constexpr (VEC == 1) {
+        const float u = x[0] * k0[0] - y[0] * k1[0], v = y[0] * k2[0] + x[0] * k3[0];
+        x[0] = u * scale;
+        y[0] = v * scale;
+    } else {
+        const float2 by = make_float2(scale, scale);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const float2 xx = make_float2(x[j], x[j + 1]), yy = make_float2(y[j], y[j + 1]);
+            const float2 nn = make_float2(-y[j], -y[j + 1]);
+            const float2 u = fma2(xx, make_float2(k0[j], k0[j + 1]), mul2(nn, make_float2(k1[j], k1[j + 1])));
+            const float2 v = fma2(yy, make_float2(k2[j], k2[j + 1]), mul2(xx, make_float2(k3[j], k3[j + 1])));
+            const float2 us = mul2(u, by), vs = mul2(v, by);
+            x[j] = us.x;
+            x[j + 1] = us.y;
+            y[j] = vs.x;
+            y[j + 1] = vs.y;
+        }
+    }
+}
+
+// sum of the squares of a and b, on top of `sum`
+template <int VEC>
+__device__ __forceinline__ float squares(const float (&a)[VEC], const float (&b)[VEC], float sum) {
+    if constexpr (VEC == 1) {
+        return sum + (a[0] * a[0] + b[0] * b[0]);
+    } else {
+        float2 s = make_float2(sum, 0.0f);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const float2 x = make_float2(a[j], a[j + 1]), y = make_float2(b[j], b[j + 1]);
+            s = fma2(x, x, s);
+            s = fma2(y, y, s);
+        }
+        return s.x + s.y;
     }
 }
 
@@ -208,20 +299,32 @@ __device__ __forceinline__ void store_codes(uint8_t *p, const float (&v)[VEC], f
     if constexpr (VEC == 1) {
         *p = static_cast<uint8_t>(pack_codes2(0.0f, v[0] * by, e5m2));
     } else {
-        Chunk<uint16_t, VEC / 2> c;
+        Chunk<uint8_t, VEC> c;
 #pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) c.e[j] = pack_codes2(v[2 * j + 1] * by, v[2 * j] * by, e5m2);
-        *reinterpret_cast<Chunk<uint16_t, VEC / 2> *>(p) = c;
+        for (int j = 0; j < VEC / 4; ++j) {
+            const float2 by2 = make_float2(by, by);
+            const float2 x = mul2(make_float2(v[4 * j], v[4 * j + 1]), by2);
+            const float2 y = mul2(make_float2(v[4 * j + 2], v[4 * j + 3]), by2);
+            c.word[j] = pack_codes2(x.y, x.x, e5m2) | (pack_codes2(y.y, y.x, e5m2) << 16);
+        }
+        *reinterpret_cast<typename Chunk<uint8_t, VEC>::Word *>(p) = c.all;
     }
 }
 
+// Largest magnitude of a and b; NaNs do not count, infinities do.
 template <int VEC>
-__device__ __forceinline__ float largest_finite(const float (&v)[VEC]) {
-    float m = 0.0f;
+__device__ __forceinline__ float largest(const float (&a)[VEC], float m) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) m = fmaxf(m, fabsf(a[j]));
+    return m;
+}
+// The same without infinities: an infinity says nothing about the scale.
+template <int VEC>
+__device__ __forceinline__ float largest_finite(const float (&a)[VEC], float m) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        const float x = fabsf(v[j]);
-        m = fmaxf(m, x <= FLT_MAX ? x : 0.0f);      // an infinity or a NaN says nothing about the scale
+        const float x = fabsf(a[j]);
+        m = fmaxf(m, x <= FLT_MAX ? x : 0.0f);
     }
     return m;
 }

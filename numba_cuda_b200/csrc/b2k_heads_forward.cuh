@@ -22,8 +22,15 @@ __device__ __forceinline__ void quantise_row(const Params &p, const Role &r, con
     if (r.scale_lanes && r.scale_joint) {
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < ITER; ++i) m = fmaxf(m, fmaxf(largest_finite<VEC>(a[i]), largest_finite<VEC>(b[i])));
-        const Scale s(g.max(m, r.scale_lanes), p.e5m2, p.e8m0);
+        for (int i = 0; i < ITER; ++i) m = largest<VEC>(b[i], largest<VEC>(a[i], m));
+        m = g.max(m, r.scale_lanes);
+        if (__any_sync(g.mask, m > FLT_MAX)) {       // rare: again without the infinities
+            m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) m = largest_finite<VEC>(b[i], largest_finite<VEC>(a[i], m));
+            m = g.max(m, r.scale_lanes);
+        }
+        const Scale s(m, p.e5m2, p.e8m0);
         if ((g.lane & (r.scale_lanes - 1)) == 0 && oa[0] < r.dim) s.store(r.scales, scale_at + r.groups_of.quotient(oa[0]), p.e8m0);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
@@ -31,8 +38,12 @@ __device__ __forceinline__ void quantise_row(const Params &p, const Role &r, con
             if (ob[i] < r.dim) store_codes<VEC>(codes + ob[i], b[i], s.inverse, p.e5m2);
         }
     } else if (ITER == 1 && r.scale_lanes) {
-        const Scale sa(g.max(largest_finite<VEC>(a[0]), r.scale_lanes), p.e5m2, p.e8m0);
-        const Scale sb(g.max(largest_finite<VEC>(b[0]), r.scale_lanes), p.e5m2, p.e8m0);
+        float ma = g.max(largest<VEC>(a[0], 0.0f), r.scale_lanes), mb = g.max(largest<VEC>(b[0], 0.0f), r.scale_lanes);
+        if (__any_sync(g.mask, fmaxf(ma, mb) > FLT_MAX)) {
+            ma = g.max(largest_finite<VEC>(a[0], 0.0f), r.scale_lanes);
+            mb = g.max(largest_finite<VEC>(b[0], 0.0f), r.scale_lanes);
+        }
+        const Scale sa(ma, p.e5m2, p.e8m0), sb(mb, p.e5m2, p.e8m0);
         if ((g.lane & (r.scale_lanes - 1)) == 0 && oa[0] < r.dim) {
             sa.store(r.scales, scale_at + r.groups_of.quotient(oa[0]), p.e8m0);
             sb.store(r.scales, scale_at + r.groups_of.quotient(ob[0]), p.e8m0);
@@ -50,8 +61,8 @@ __device__ __forceinline__ void quantise_row(const Params &p, const Role &r, con
         __syncwarp(g.mask);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            if (oa[i] < r.dim) atomicMax(&group_max[r.groups_of.quotient(oa[i])], __float_as_uint(largest_finite<VEC>(a[i])));
-            if (ob[i] < r.dim) atomicMax(&group_max[r.groups_of.quotient(ob[i])], __float_as_uint(largest_finite<VEC>(b[i])));
+            if (oa[i] < r.dim) atomicMax(&group_max[r.groups_of.quotient(oa[i])], __float_as_uint(largest_finite<VEC>(a[i], 0.0f)));
+            if (ob[i] < r.dim) atomicMax(&group_max[r.groups_of.quotient(ob[i])], __float_as_uint(largest_finite<VEC>(b[i], 0.0f)));
         }
         __syncwarp(g.mask);
         for (int k = g.lane; k < groups; k += g.n)
@@ -68,6 +79,30 @@ __device__ __forceinline__ void quantise_row(const Params &p, const Role &r, con
     }
 }
 
+// A group's chunks of kRows rows of one token, as loaded.
+template <typename T, int VEC, int ITER, int ROWS>
+struct Batch {
+    Chunk<T, VEC> a[ROWS][ITER], b[ROWS][ITER];
+    __device__ __forceinline__ void load(const T *in, int64_t step, int rows, const int (&oa)[ITER], const int (&ob)[ITER],
+                                         int dim) {
+#pragma unroll
+        for (int h = 0; h < ROWS; ++h)
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                a[h][i] = b[h][i] = Chunk<T, VEC>{};
+                if (h < rows && oa[i] < dim) a[h][i] = load_chunk<T, VEC>(in + h * step + oa[i]);
+                if (h < rows && ob[i] < dim) b[h][i] = load_chunk<T, VEC>(in + h * step + ob[i]);
+            }
+    }
+};
+
+// What the forward kernel multiplies a row's items by: k0 .. k3 of turn() for rotated
+// units; k0 and k2 are the weights of the two chunks for the others.
+template <int VEC, int ITER>
+struct Factors {
+    float k0[ITER][VEC], k1[ITER][VEC], k2[ITER][VEC], k3[ITER][VEC];
+};
+
 template <typename T, int VEC, int ITER, int MODE>
 __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_constant__ Params p) {
     // groups of a scale are at least 16 items, so a lane's share of a row has at most this many
@@ -75,9 +110,9 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
     constexpr int kRows = rows_in_flight(ITER);
     __shared__ unsigned group_max[MODE == kRotate ? 1 : kThreads * kGroupsPerLane];
     // A block works for one role, so the role's members are uniform over the block.
-    uint32_t block = blockIdx.x;
-    int which = 0;
-    while (block >= p.role[which].blocks) block -= p.role[which++].blocks;
+    const uint32_t upto0 = p.role[0].blocks, upto1 = upto0 + p.role[1].blocks;
+    const int which = (blockIdx.x >= upto0) + (blockIdx.x >= upto1);
+    const uint32_t block = blockIdx.x - (which == 0 ? 0 : which == 1 ? upto0 : upto1);
     const Role &r = p.role[which];
     const Lanes g(p.lanes);
     const uint32_t item = block * (static_cast<uint32_t>(kThreads) >> p.lane_bits) + (threadIdx.x >> p.lane_bits);
@@ -92,16 +127,9 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
     for (int i = 0; i < ITER; ++i) unit_at<VEC>(r, g.lane + i * g.n, oa[i], ob[i]);
 
     // The rows' loads go first: they do not wait for the token's position and slot.
-    Chunk<T, VEC> ca[kRows][ITER], cb[kRows][ITER];
     const T *in = static_cast<const T *>(r.in) + token * r.in_token + first * r.in_head;
-#pragma unroll
-    for (int h = 0; h < kRows; ++h)
-#pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            ca[h][i] = cb[h][i] = Chunk<T, VEC>{};
-            if (h < rows && oa[i] < r.dim) ca[h][i] = load_chunk<T, VEC>(in + h * r.in_head + oa[i]);
-            if (h < rows && ob[i] < r.dim) cb[h][i] = load_chunk<T, VEC>(in + h * r.in_head + ob[i]);
-        }
+    Batch<T, VEC, ITER, kRows> now;
+    now.load(in, r.in_head, rows, oa, ob, r.dim);
 
     const bool quantised = MODE == kWrite || (MODE == kBoth && r.out == nullptr);
     int64_t position = 0, slot = 0;
@@ -117,62 +145,103 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
     }
     const bool normed = (MODE & kRotate) && p.norm && which < 2;
 
-    float c[ITER][VEC] = {}, s[ITER][VEC] = {}, wa[ITER][VEC] = {}, wb[ITER][VEC] = {};
+    Factors<VEC, ITER> k;
     if constexpr ((MODE & kRotate) != 0) {
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int u = g.lane + i * g.n;
+            float wa[VEC], wb[VEC], c[VEC], s[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) wa[j] = wb[j] = 1.0f;
+            if (normed && oa[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa[i], wa);
+            if (normed && ob[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob[i], wb);
             if (u < r.angle_units) {
-                load_floats<VEC>(p.cos_table + position * p.cos_stride + u * VEC, c[i]);
-                load_floats<VEC>(p.sin_table + position * p.sin_stride + u * VEC, s[i]);
-            }
-            if (normed) {
-                if (oa[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa[i], wa[i]);
-                if (ob[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob[i], wb[i]);
+                load_floats<VEC>(p.cos_table + position * p.cos_stride + u * VEC, c);
+                load_floats<VEC>(p.sin_table + position * p.sin_stride + u * VEC, s);
+                float wx[VEC], wy[VEC];
+                if (p.interleaved) {
+                    pair<VEC>(wa, wb, wx, wy);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        wx[j] = wa[j];
+                        wy[j] = wb[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    k.k0[i][j] = wx[j] * c[j];
+                    k.k1[i][j] = wy[j] * s[j];
+                    k.k2[i][j] = wy[j] * c[j];
+                    k.k3[i][j] = wx[j] * s[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    k.k0[i][j] = wa[j];
+                    k.k2[i][j] = wb[j];
+                    k.k1[i][j] = k.k3[i][j] = 0.0f;
+                }
             }
         }
     }
 
+#pragma unroll 1
+    for (int done = 0; done < rows; done += kRows) {
+        // the next rows are on their way while these are worked on
+        Batch<T, VEC, ITER, kRows> next;
+        in += kRows * r.in_head;
+        next.load(in, r.in_head, rows - done - kRows, oa, ob, r.dim);
 #pragma unroll
-    for (int h = 0; h < kRows; ++h) {
-        if (h >= rows) break;
-        float a[ITER][VEC], b[ITER][VEC];
-#pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            widen(ca[h][i], a[i]);
-            widen(cb[h][i], b[i]);
-        }
-        if constexpr ((MODE & kRotate) != 0) {
-            if (normed) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int i = 0; i < ITER; ++i)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) ss += a[i][j] * a[i][j] + b[i][j] * b[i][j];
-                const float by = rsqrtf(g.sum(ss) * r.inv_dim + p.eps);
-#pragma unroll
-                for (int i = 0; i < ITER; ++i)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        a[i][j] *= by * wa[i][j];
-                        b[i][j] *= by * wb[i][j];
-                    }
-            }
-#pragma unroll
-            for (int i = 0; i < ITER; ++i)
-                if (g.lane + i * g.n < r.angle_units) rotate<VEC>(a[i], b[i], c[i], s[i], p.interleaved);
-        }
-        if (!quantised) {
-            T *out = static_cast<T *>(r.out) + token * r.out_token + (first + h) * r.out_head;
+        for (int h = 0; h < kRows; ++h) {
+            if (done + h >= rows) break;
+            float a[ITER][VEC], b[ITER][VEC];
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
-                if (oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a[i]);
-                if (ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b[i]);
+                widen(now.a[h][i], a[i]);
+                widen(now.b[h][i], b[i]);
             }
-        } else if constexpr (MODE != kRotate) {
-            quantise_row<VEC, ITER>(p, r, g, at, first + h, a, b,
-                                    group_max + (threadIdx.x & ~(g.n - 1)) * kGroupsPerLane);
+            if constexpr ((MODE & kRotate) != 0) {
+                float by = 1.0f;
+                if (normed) {
+                    float ss = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < ITER; ++i) ss = squares<VEC>(a[i], b[i], ss);
+                    by = rsqrtf(g.sum(ss) * r.inv_dim + p.eps);
+                }
+#pragma unroll
+                for (int i = 0; i < ITER; ++i) {
+                    if (g.lane + i * g.n < r.angle_units) {
+                        if (p.interleaved) {
+                            float x[VEC], y[VEC];
+                            pair<VEC>(a[i], b[i], x, y);
+                            turn<VEC>(x, y, k.k0[i], k.k1[i], k.k2[i], k.k3[i], by);
+                            unpair<VEC>(x, y, a[i], b[i]);
+                        } else {
+                            turn<VEC>(a[i], b[i], k.k0[i], k.k1[i], k.k2[i], k.k3[i], by);
+                        }
+                    } else if (normed) {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) {
+                            a[i][j] *= by * k.k0[i][j];
+                            b[i][j] *= by * k.k2[i][j];
+                        }
+                    }
+                }
+            }
+            const int head = first + done + h;
+            if (!quantised) {
+                T *out = static_cast<T *>(r.out) + token * r.out_token + head * r.out_head;
+#pragma unroll
+                for (int i = 0; i < ITER; ++i) {
+                    if (oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a[i]);
+                    if (ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b[i]);
+                }
+            } else if constexpr (MODE != kRotate) {
+                quantise_row<VEC, ITER>(p, r, g, at, head, a, b, group_max + (threadIdx.x & ~(g.n - 1)) * kGroupsPerLane);
+            }
         }
+        now = next;
     }
 }
 
@@ -191,7 +260,7 @@ void pick_forward(const Params &p, const Plan &plan, unsigned blocks, cudaStream
 // Launches over all items; the roles, tokens and tables of `p` are set.
 template <int MODE>
 int launch_forward(Params &p, int64_t format, const Plan &plan, cudaStream_t stream, const char *name) {
-    if (int rc = count_items(p, rows_in_flight(plan.iter), kThreads, name)) return rc;
+    if (int rc = count_items(p, kHeadsPerItem, kThreads, name)) return rc;
     const unsigned blocks = p.role[0].blocks + p.role[1].blocks + p.role[2].blocks;
     if (blocks == 0) return B2K_OK;
     if (format == B2K_FMT_F32) pick_forward<float, MODE>(p, plan, blocks, stream);

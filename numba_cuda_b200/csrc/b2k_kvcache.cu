@@ -72,20 +72,23 @@ __device__ __forceinline__ void store_items(T *p, const float (&v)[N]) {
         else *reinterpret_cast<uint16_t *>(p) = static_cast<uint16_t>(pack2_saturated<T>(v[0], 0.0f));
     } else {
         constexpr int W = N * sizeof(T) / 4;
-        Chunk<uint32_t, W> w;
+        uint32_t w[W];
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) w.e[j] = __float_as_uint(saturated(v[j]));
+            for (int j = 0; j < N; ++j) w[j] = __float_as_uint(saturated(v[j]));
         } else {
 #pragma unroll
-            for (int j = 0; j < W; ++j) w.e[j] = pack2_saturated<T>(v[2 * j], v[2 * j + 1]);
+            for (int j = 0; j < W; ++j) w[j] = pack2_saturated<T>(v[2 * j], v[2 * j + 1]);
         }
         if constexpr (W == 8) {                    // sm_100's 256-bit store
-            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w.e[0]), "r"(w.e[1]),
-                         "r"(w.e[2]), "r"(w.e[3]), "r"(w.e[4]), "r"(w.e[5]), "r"(w.e[6]), "r"(w.e[7])
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
+                         "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                          : "memory");
         } else {
-            *reinterpret_cast<Chunk<uint32_t, W> *>(p) = w;
+            Chunk<uint32_t, W> c;
+#pragma unroll
+            for (int j = 0; j < W; ++j) c.word[j] = w[j];
+            *reinterpret_cast<typename Chunk<uint32_t, W>::Word *>(p) = c.all;
         }
     }
 }
@@ -144,14 +147,18 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
                 if (now[i] == 0) continue;
                 float v[CV];
                 if constexpr (CV == 1) {
-                    v[0] = decode2<E5M2>(c[i].e[0]).x * scale[i];
+                    v[0] = decode2<E5M2>(c[i].all).x * scale[i];
                 } else {
-                    const Chunk<uint16_t, CV / 2> two = *reinterpret_cast<const Chunk<uint16_t, CV / 2> *>(&c[i]);
 #pragma unroll
-                    for (int j = 0; j < CV / 2; ++j) {
-                        const float2 f = decode2<E5M2>(two.e[j]);
-                        v[2 * j] = f.x * scale[i];
-                        v[2 * j + 1] = f.y * scale[i];
+                    for (int j = 0; j < CV / 4; ++j) {
+                        const float2 f = decode2<E5M2>(static_cast<uint16_t>(c[i].word[j]));
+                        const float2 h = decode2<E5M2>(static_cast<uint16_t>(c[i].word[j] >> 16));
+                        const float2 by = make_float2(scale[i], scale[i]);
+                        const float2 x = mul2(f, by), y = mul2(h, by);
+                        v[4 * j] = x.x;
+                        v[4 * j + 1] = x.y;
+                        v[4 * j + 2] = y.x;
+                        v[4 * j + 3] = y.y;
                     }
                 }
                 store_items<T, CV>(out + (t + i * down) * s.out_token, v);
