@@ -317,152 +317,200 @@ int count_items(Params &p, int most, int threads, const char *name) {
 // Blocks of a role stride over its rows and keep the weight gradient's partial sums in
 // registers; each block writes one row of partials, and a second kernel adds the rows
 // in order: no atomics, so equal calls give equal bits.
-constexpr int kBackwardBlocksPerSm = 4;
+constexpr int kMostBlocksPerSm = 8;
+constexpr int kBackwardHeadsPerItem = 8;
 
+// The inverse rotation of a unit's pairs.
 template <int VEC>
-__device__ __forceinline__ void rotate(float (&x)[VEC], float (&y)[VEC], const float (&c)[VEC], const float (&s)[VEC]) {
+__device__ __forceinline__ void turn_back(float (&x)[VEC], float (&y)[VEC], const float (&c)[VEC], const float (&s)[VEC]) {
+    if constexpr (VEC == 1) {
+        const float u = x[0] * c[0] + y[0] * s[0], v = y[0] * c[0] - x[0] * s[0];
+        x[0] = u;
+        y[0] = v;
+    } else {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        const float u = x[j] * c[j] - y[j] * s[j], v = y[j] * c[j] + x[j] * s[j];
-        x[j] = u;
-        y[j] = v;
+        for (int j = 0; j < VEC; j += 2) {
+            const float2 a = make_float2(x[j], x[j + 1]), b = make_float2(y[j], y[j + 1]);
+            const float2 cc = make_float2(c[j], c[j + 1]), sn = make_float2(s[j], s[j + 1]);
+            const float2 u = fma2(a, cc, mul2(b, sn));
+            const float2 v = fma2(b, cc, mul2(make_float2(-a.x, -a.y), sn));
+            x[j] = u.x;
+            x[j + 1] = u.y;
+            y[j] = v.x;
+            y[j + 1] = v.y;
+        }
+    }
+}
+
+// sum of x^2 and of (g w) x over a chunk's worth of items, on top of ss and dot
+template <int VEC>
+__device__ __forceinline__ void gradient_sums(const float (&x)[VEC], const float (&g)[VEC], const float (&w)[VEC], float2 &ss,
+                                              float2 &dot) {
+    if constexpr (VEC == 1) {
+        ss.x += x[0] * x[0];
+        dot.x += g[0] * w[0] * x[0];
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const float2 xx = make_float2(x[j], x[j + 1]);
+            ss = fma2(xx, xx, ss);
+            dot = fma2(mul2(make_float2(g[j], g[j + 1]), make_float2(w[j], w[j + 1])), xx, dot);
+        }
+    }
+}
+
+// g -> by (g w) - x pull, and the weight's sum += g x by
+template <int VEC>
+__device__ __forceinline__ void gradient_of(const float (&x)[VEC], float (&g)[VEC], const float (&w)[VEC], float by,
+                                            float pull, float (&sum)[VEC]) {
+    if constexpr (VEC == 1) {
+        sum[0] += g[0] * (x[0] * by);
+        g[0] = by * (g[0] * w[0]) - x[0] * pull;
+    } else {
+        const float2 by2 = make_float2(by, by), pull2 = make_float2(-pull, -pull);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const float2 xx = make_float2(x[j], x[j + 1]), gg = make_float2(g[j], g[j + 1]);
+            const float2 t = fma2(gg, mul2(xx, by2), make_float2(sum[j], sum[j + 1]));
+            const float2 d = fma2(mul2(gg, make_float2(w[j], w[j + 1])), by2, mul2(xx, pull2));
+            sum[j] = t.x;
+            sum[j + 1] = t.y;
+            g[j] = d.x;
+            g[j + 1] = d.y;
+        }
+    }
+}
+
+template <typename T, int VEC, int ITER, int WHICH>
+__device__ __forceinline__ void backward_role(const Params &p, uint32_t first_block, uint32_t blocks, float *block_sums) {
+    const Role &r = p.role[WHICH];
+    const Lanes g(p.lanes);
+    const uint32_t in_block = static_cast<uint32_t>(kThreads) >> p.lane_bits;
+    // In the order of the pairs: w, sums and rows are kept as turn() wants them.
+    const bool swap = p.interleaved;
+    int oa[ITER], ob[ITER];
+    float wx[ITER][VEC], wy[ITER][VEC], sum_x[ITER][VEC] = {}, sum_y[ITER][VEC] = {};
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        unit_at<VEC>(r, g.lane + i * g.n, oa[i], ob[i]);
+        float wa[VEC] = {}, wb[VEC] = {};
+        if (oa[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa[i], wa);
+        if (ob[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob[i], wb);
+        in_pairs<VEC>(swap, wa, wb, wx[i], wy[i]);
+    }
+    // A warp's groups take neighbouring items and stay together: see Lanes.  all_items < 2^31,
+    // and a step is at most the grid's groups, so nothing overflows.
+    const uint32_t in_warp = 32u >> p.lane_bits;
+    for (uint32_t base = first_block * in_block + threadIdx.x / 32 * in_warp; base < r.all_items; base += blocks * in_block) {
+        const uint32_t item = base + (threadIdx.x % 32 >> p.lane_bits);
+        const bool active = item < r.all_items;
+        const uint32_t at_token = active ? r.items.quotient(item) : 0;
+        const int64_t token = at_token;
+        const int first = active ? static_cast<int>(item - at_token * r.items.d) * p.heads_per_item : 0;
+        const int rows = active ? min(r.heads - first, p.heads_per_item) : 0;
+        const T *in = static_cast<const T *>(r.in) + token * r.in_token + first * r.in_head;
+        const T *grad = static_cast<const T *>(r.grad) + token * r.grad_token + first * r.grad_head;
+        T *out = static_cast<T *>(r.out) + token * r.out_token + first * r.out_head;
+        Batch<T, VEC, ITER, 1> x_now, g_now;
+        x_now.load(in, 0, rows, oa, ob, r.dim);
+        g_now.load(grad, 0, rows, oa, ob, r.dim);
+        int64_t position = 0;
+        if (p.positions != nullptr) position = paging::load_index(p.positions, p.position_bytes, token);
+        // a padding token's rows are taken as zeros all through, with by = 0 below
+        const bool padding = p.positions != nullptr && (position < 0 || position >= p.table_rows);
+        float c[ITER][VEC] = {}, s[ITER][VEC] = {};
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int u = g.lane + i * g.n;
+            if (u < r.angle_units && !padding) {
+                load_floats<VEC>(p.cos_table + position * p.cos_stride + u * VEC, c[i]);
+                load_floats<VEC>(p.sin_table + position * p.sin_stride + u * VEC, s[i]);
+            }
+        }
+        const int most = __reduce_max_sync(0xFFFFFFFFu, rows);
+#pragma unroll 1
+        for (int h = 0; h < most; ++h) {
+            // the next row is on its way while this one is worked on
+            Batch<T, VEC, ITER, 1> x_next, g_next;
+            in += r.in_head;
+            grad += r.grad_head;
+            x_next.load(in, 0, rows - h - 1, oa, ob, r.dim);
+            g_next.load(grad, 0, rows - h - 1, oa, ob, r.dim);
+            float x[ITER][VEC], y[ITER][VEC], gx[ITER][VEC], gy[ITER][VEC];
+            float2 ss = make_float2(0.0f, 0.0f), dot = ss;
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                float a[VEC], b[VEC];
+                if (padding) x_now.a[0][i] = x_now.b[0][i] = g_now.a[0][i] = g_now.b[0][i] = Chunk<T, VEC>{};
+                widen(x_now.a[0][i], a);
+                widen(x_now.b[0][i], b);
+                in_pairs<VEC>(swap, a, b, x[i], y[i]);
+                widen(g_now.a[0][i], a);
+                widen(g_now.b[0][i], b);
+                in_pairs<VEC>(swap, a, b, gx[i], gy[i]);
+                if (g.lane + i * g.n < r.angle_units) turn_back<VEC>(gx[i], gy[i], c[i], s[i]);
+                gradient_sums<VEC>(x[i], gx[i], wx[i], ss, dot);
+                gradient_sums<VEC>(y[i], gy[i], wy[i], ss, dot);
+            }
+            if (p.norm) {
+                // dx = r (h - n mean(h n)) with n = x r:  r h - x (r^3 sum(h x) / dim)
+                const bool none = padding || h >= rows;       // eps may be zero
+                const float mean = g.sum(ss.x + ss.y) * r.inv_dim;
+                const float by = none ? 0.0f : rsqrtf(mean + p.eps);
+                const float pull = g.sum(dot.x + dot.y) * r.inv_dim * by * by * by;
+#pragma unroll
+                for (int i = 0; i < ITER; ++i) {
+                    gradient_of<VEC>(x[i], gx[i], wx[i], by, pull, sum_x[i]);
+                    gradient_of<VEC>(y[i], gy[i], wy[i], by, pull, sum_y[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                float a[VEC], b[VEC];
+                out_of_pairs<VEC>(swap, gx[i], gy[i], a, b);
+                if (h < rows && oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a);
+                if (h < rows && ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b);
+            }
+            out += r.out_head;
+            x_now = x_next;
+            g_now = g_next;
+        }
+    }
+    if (r.weight_grad == nullptr) return;
+    // groups of a warp, then the block's warps in order
+    const int warp = threadIdx.x / 32;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        float a[VEC], b[VEC];
+        out_of_pairs<VEC>(swap, sum_x[i], sum_y[i], a, b);
+        for (int o = g.n; o < 32; o *= 2)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                a[j] += __shfl_xor_sync(0xFFFFFFFFu, a[j], o);
+                b[j] += __shfl_xor_sync(0xFFFFFFFFu, b[j], o);
+            }
+        if (threadIdx.x % 32 < g.n) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (oa[i] < r.dim) block_sums[warp * r.dim + oa[i] + j] = a[j];
+                if (ob[i] < r.dim) block_sums[warp * r.dim + ob[i] + j] = b[j];
+            }
+        }
+    }
+    __syncthreads();
+    float *row = p.partials + static_cast<int64_t>(blockIdx.x) * p.partial_stride;
+    for (int d = threadIdx.x; d < r.dim; d += kThreads) {
+        float v = 0.0f;
+        for (int w = 0; w < kThreads / 32; ++w) v += block_sums[w * r.dim + d];
+        row[d] = v;
     }
 }
 
 template <typename T, int VEC, int ITER>
 __global__ void __launch_bounds__(kThreads) heads_backward_kernel(const __grid_constant__ Params p) {
     extern __shared__ float block_sums[];             // one row of dim floats per warp
-    const Lanes g(p.lanes);
-    const int which = static_cast<int>(blockIdx.x) < p.blocks0 ? 0 : 1;
-    const Role &r = p.role[which];
-    const uint32_t first = which ? blockIdx.x - p.blocks0 : blockIdx.x;
-    const uint32_t blocks = which ? gridDim.x - p.blocks0 : p.blocks0;
-    const uint32_t in_block = static_cast<uint32_t>(kThreads) >> p.lane_bits;
-    const bool summed = r.weight_grad != nullptr;
-    float sum_a[ITER][VEC] = {}, sum_b[ITER][VEC] = {};
-    float wa[ITER][VEC] = {}, wb[ITER][VEC] = {};
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        int oa, ob;
-        unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
-        if (oa < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa, wa[i]);
-        if (ob < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob, wb[i]);
-    }
-    // all_items < 2^31, and a step is at most the grid's groups: no overflow
-    for (uint32_t item = first * in_block + (threadIdx.x >> p.lane_bits); item < r.all_items; item += blocks * in_block) {
-        const uint32_t at_token = r.items.quotient(item);
-        const int64_t token = at_token;
-        const int part = static_cast<int>(item - at_token * r.items.d);
-        int64_t position = 0;
-        if (p.positions != nullptr) position = paging::load_index(p.positions, p.position_bytes, token);
-        const bool padding = p.positions != nullptr && (position < 0 || position >= p.table_rows);
-        float c[ITER][VEC] = {}, s[ITER][VEC] = {};
-        if (!padding) {
-#pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                const int u = g.lane + i * g.n;
-                if (u < r.angle_units) {
-                    load_floats<VEC>(p.cos_table + position * p.cos_stride + u * VEC, c[i]);
-                    load_floats<VEC>(p.sin_table + position * p.sin_stride + u * VEC, s[i]);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) s[i][j] = -s[i][j];      // the inverse rotation
-                }
-            }
-        }
-        const int last = min(r.heads, (part + 1) * p.heads_per_item);
-        for (int head = part * p.heads_per_item; head < last; ++head) {
-            const T *in = static_cast<const T *>(r.in) + token * r.in_token + head * r.in_head;
-            const T *grad = static_cast<const T *>(r.grad) + token * r.grad_token + head * r.grad_head;
-            T *out = static_cast<T *>(r.out) + token * r.out_token + head * r.out_head;
-            float xa[ITER][VEC], xb[ITER][VEC], ga[ITER][VEC], gb[ITER][VEC];
-#pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                int oa, ob;
-                unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
-                Chunk<T, VEC> ca{}, cb{}, da{}, db{};
-                if (oa < r.dim && !padding) {
-                    ca = load_chunk<T, VEC>(in + oa);
-                    da = load_chunk<T, VEC>(grad + oa);
-                }
-                if (ob < r.dim && !padding) {
-                    cb = load_chunk<T, VEC>(in + ob);
-                    db = load_chunk<T, VEC>(grad + ob);
-                }
-                widen(ca, xa[i]);
-                widen(cb, xb[i]);
-                widen(da, ga[i]);
-                widen(db, gb[i]);
-            }
-            float ss = 0.0f, dot = 0.0f;
-#pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                if (g.lane + i * g.n < r.angle_units) {
-                    if (p.interleaved) {
-                        float x[VEC], y[VEC];
-                        pair<VEC>(ga[i], gb[i], x, y);
-                        rotate<VEC>(x, y, c[i], s[i]);
-                        unpair<VEC>(x, y, ga[i], gb[i]);
-                    } else {
-                        rotate<VEC>(ga[i], gb[i], c[i], s[i]);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    ss += xa[i][j] * xa[i][j] + xb[i][j] * xb[i][j];
-                    dot += ga[i][j] * wa[i][j] * xa[i][j] + gb[i][j] * wb[i][j] * xb[i][j];
-                }
-            }
-            if (p.norm) {
-                // mean(h n) = by * dot / dim; a padding row is all zeros (eps may be zero, too)
-                const float by = padding ? 0.0f : rsqrtf(g.sum(ss) * r.inv_dim + p.eps);
-                const float pull = g.sum(dot) * r.inv_dim * by * by;
-#pragma unroll
-                for (int i = 0; i < ITER; ++i)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        sum_a[i][j] += ga[i][j] * (xa[i][j] * by);
-                        sum_b[i][j] += gb[i][j] * (xb[i][j] * by);
-                        ga[i][j] = by * (ga[i][j] * wa[i][j] - xa[i][j] * pull);
-                        gb[i][j] = by * (gb[i][j] * wb[i][j] - xb[i][j] * pull);
-                    }
-            }
-#pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                int oa, ob;
-                unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
-                if (oa < r.dim) store_chunk<T, VEC>(out + oa, ga[i]);
-                if (ob < r.dim) store_chunk<T, VEC>(out + ob, gb[i]);
-            }
-        }
-    }
-    if (!summed) return;
-    // groups of a warp, then the block's warps in order
-    const int warp = threadIdx.x / 32;
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        for (int o = g.n; o < 32; o *= 2)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                sum_a[i][j] += __shfl_xor_sync(0xFFFFFFFFu, sum_a[i][j], o);
-                sum_b[i][j] += __shfl_xor_sync(0xFFFFFFFFu, sum_b[i][j], o);
-            }
-        int oa, ob;
-        unit_at<VEC>(r, g.lane + i * g.n, oa, ob);
-        if (threadIdx.x % 32 < g.n) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                if (oa < r.dim) block_sums[warp * r.dim + oa + j] = sum_a[i][j];
-                if (ob < r.dim) block_sums[warp * r.dim + ob + j] = sum_b[i][j];
-            }
-        }
-    }
-    __syncthreads();
-    float *row = p.partials + static_cast<int64_t>(blockIdx.x) * B2K_MAX_HEAD_DIM;
-    for (int d = threadIdx.x; d < r.dim; d += kThreads) {
-        float v = 0.0f;
-        for (int w = 0; w < kThreads / 32; ++w) v += block_sums[w * r.dim + d];
-        row[d] = v;
-    }
+    if (static_cast<int>(blockIdx.x) < p.blocks0) backward_role<T, VEC, ITER, 0>(p, blockIdx.x, p.blocks0, block_sums);
+    else backward_role<T, VEC, ITER, 1>(p, blockIdx.x - p.blocks0, gridDim.x - p.blocks0, block_sums);
 }
 
 // weight_grad[d] = sum over the role's blocks of partials[block][d], 32 columns a block:
@@ -475,7 +523,7 @@ __global__ void __launch_bounds__(kThreads) weight_grad_kernel(const __grid_cons
     const int begin = blockIdx.y ? p.blocks0 : 0, end = blockIdx.y ? blocks : p.blocks0;
     float v = 0.0f;
     if (d < r.dim)
-        for (int b = begin + row; b < end; b += kThreads / 32) v += p.partials[static_cast<int64_t>(b) * B2K_MAX_HEAD_DIM + d];
+        for (int b = begin + row; b < end; b += kThreads / 32) v += p.partials[static_cast<int64_t>(b) * p.partial_stride + d];
     part[row][threadIdx.x % 32] = v;
     __syncthreads();
     if (row || d >= r.dim) return;
@@ -485,17 +533,44 @@ __global__ void __launch_bounds__(kThreads) weight_grad_kernel(const __grid_cons
     else static_cast<__nv_bfloat16 *>(r.weight_grad)[d] = __float2bfloat16_rn(v);
 }
 
-static int backward_blocks() { return b2k::sm_count() * kBackwardBlocksPerSm; }
+// Blocks of one instantiation that an SM holds at once: the grid is one full wave, since
+// a second, partial one would leave most SMs idle (4 blocks an SM where 3 fit: 313 us
+// instead of 226 us for 32768 tokens x 40 heads of 128 bf16 items).
+template <typename T, int VEC, int ITER>
+int resident_blocks() {
+    static b2k::PerDeviceOnce once;
+    static int found[b2k::kMaxDevices];
+    const int dev = b2k::current_device();
+    if (dev < 0 || dev >= b2k::kMaxDevices) return 1;
+    once.run([&] {
+        int n = 0;
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+            &n, heads_backward_kernel<T, VEC, ITER>, kThreads, kThreads / 32 * B2K_MAX_HEAD_DIM * sizeof(float));
+        found[dev] = n < 1 ? 1 : n > kMostBlocksPerSm ? kMostBlocksPerSm : n;
+        return e;
+    });
+    return found[dev] < 1 ? 1 : found[dev];
+}
 
+// Launches, or with `launch` off says how many blocks an SM holds.
 template <typename T>
-static void pick_backward(const Params &p, const Plan &plan, int blocks, size_t shared, cudaStream_t stream) {
-#define B2K_HEADS_CASE(V, I)                                                              \
-    if constexpr (V * sizeof(T) <= 16) if (plan.vec == V && plan.iter == I) { \
-        heads_backward_kernel<T, V, I><<<blocks, kThreads, shared, stream>>>(p);          \
-        return;                                                                           \
+static int pick_backward(const Params &p, const Plan &plan, bool launch, int blocks, size_t shared, cudaStream_t stream) {
+#define B2K_HEADS_CASE(V, I)                                                                              \
+    if constexpr (V * sizeof(T) <= 16) if (plan.vec == V && plan.iter == I) {                             \
+        if (!launch) return resident_blocks<T, V, I>();                                                   \
+        heads_backward_kernel<T, V, I><<<blocks, kThreads, shared, stream>>>(p);                          \
+        return 0;                                                                                         \
     }
     B2K_HEADS_SHAPES(B2K_HEADS_CASE)
 #undef B2K_HEADS_CASE
+    return 1;
+}
+
+static int backward_kernel(int64_t format, const Params &p, const Plan &plan, bool launch, int blocks, size_t shared,
+                           cudaStream_t stream) {
+    if (format == B2K_FMT_F32) return pick_backward<float>(p, plan, launch, blocks, shared, stream);
+    if (format == B2K_FMT_F16) return pick_backward<__half>(p, plan, launch, blocks, shared, stream);
+    return pick_backward<__nv_bfloat16>(p, plan, launch, blocks, shared, stream);
 }
 
 }  // namespace headwise
@@ -527,8 +602,10 @@ int b2k_norm_rotate(const b2k_rotation *r, const b2k_heads *q_out, const b2k_hea
 }
 
 int64_t b2k_norm_rotate_backward_scratch_bytes(const b2k_rotation *r) {
-    (void)r;
-    return static_cast<int64_t>(backward_blocks()) * B2K_MAX_HEAD_DIM * 4;
+    const int64_t dim = r == nullptr || (r->q.heads == 0 && r->k.heads == 0) ? B2K_MAX_HEAD_DIM
+                        : r->k.heads == 0 || (r->q.heads && r->q.dim > r->k.dim) ? r->q.dim : r->k.dim;
+    if (dim < 0 || dim > B2K_MAX_HEAD_DIM) return 0;
+    return static_cast<int64_t>(b2k::sm_count()) * kMostBlocksPerSm * dim * 4;
 }
 
 int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, const b2k_heads *k_grad,
@@ -570,9 +647,10 @@ int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, con
     p.partials = static_cast<float *>(scratch_dev);
     set_rotation(p, *r);
     const Plan plan = choose(p, r->format, r);
-    if (int rc = count_items(p, 1, kThreads, name)) return rc;
+    if (int rc = count_items(p, kBackwardHeadsPerItem, kThreads, name)) return rc;
     // blocks go to the two roles by their share of the rows' items, at least one to each
-    int64_t need[2], most = backward_blocks();
+    const cudaStream_t st = b2k::as_stream(stream);
+    int64_t need[2], most = b2k::sm_count() * static_cast<int64_t>(backward_kernel(r->format, p, plan, false, 0, 0, st));
     for (int i = 0; i < 2; ++i) need[i] = p.role[i].blocks;
     if (need[0] + need[1] > most) {
         const int64_t total = need[0] + need[1];
@@ -585,12 +663,10 @@ int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, con
     p.blocks0 = static_cast<int>(need[0]);
     const int blocks = static_cast<int>(need[0] + need[1]);
     const int dim = p.role[0].dim > p.role[1].dim ? p.role[0].dim : p.role[1].dim;
-    const cudaStream_t st = b2k::as_stream(stream);
+    p.partial_stride = dim;
     if (blocks > 0) {
         const size_t shared = summed ? static_cast<size_t>(kThreads / 32) * dim * sizeof(float) : 0;
-        if (r->format == B2K_FMT_F32) pick_backward<float>(p, plan, blocks, shared, st);
-        else if (r->format == B2K_FMT_F16) pick_backward<__half>(p, plan, blocks, shared, st);
-        else pick_backward<__nv_bfloat16>(p, plan, blocks, shared, st);
+        backward_kernel(r->format, p, plan, true, blocks, shared, st);
         B2K_RETURN_IF_LAUNCH_FAILED(name);
         b2k::note_launch();
     }

@@ -60,7 +60,8 @@ struct Params {
     const void *slots;
     int slot_bytes, e5m2, e8m0;
     int64_t pages, page_size;
-    float *partials;            // backward: weight-gradient partial sums, one row of dim floats per block
+    float *partials;            // backward: weight-gradient partial sums, a row per block
+    int partial_stride;
     int blocks0;                // backward: blocks of role 0
 };
 
@@ -182,25 +183,28 @@ __device__ __forceinline__ void load_weight(const void *w, int format, int at, f
     }
 }
 
-// The lanes of a group, and where a unit's two chunks start.
+// The lanes of a group.  Reductions are called by whole warps, idle groups included: a
+// shuffle under a mask known only at run time costs a warp synchronisation each, which
+// is what bounded the kernels that let idle groups leave early.
 struct Lanes {
     int n, lane;
-    unsigned mask;
-    __device__ explicit Lanes(int lanes) : n(lanes), lane(threadIdx.x & (lanes - 1)) {
-        const unsigned ones = lanes == 32 ? 0xFFFFFFFFu : (1u << lanes) - 1u;
-        mask = ones << ((threadIdx.x & 31) & ~(lanes - 1));
-    }
+    __device__ explicit Lanes(int lanes) : n(lanes), lane(threadIdx.x & (lanes - 1)) {}
     __device__ float sum(float v) const {
-        for (int o = n >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            if (o < n) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
         return v;
     }
     // over aligned runs of `span` lanes (a power of two) of the group
     __device__ float max(float v, int span) const {
-        for (int o = span >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            if (o < span) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
         return v;
     }
 };
 
+// Where a unit's two chunks start.
 template <int VEC>
 __device__ __forceinline__ void unit_at(const Role &r, int u, int &a, int &b) {
     if (u < r.pair_units) {
@@ -212,6 +216,23 @@ __device__ __forceinline__ void unit_at(const Role &r, int u, int &a, int &b) {
     }
     if (u >= r.units) a = b = r.dim;       // nothing
 }
+
+// A group's chunks of ROWS rows of one token, as loaded.
+template <typename T, int VEC, int ITER, int ROWS>
+struct Batch {
+    Chunk<T, VEC> a[ROWS][ITER], b[ROWS][ITER];
+    __device__ __forceinline__ void load(const T *in, int64_t step, int rows, const int (&oa)[ITER], const int (&ob)[ITER],
+                                         int dim) {
+#pragma unroll
+        for (int h = 0; h < ROWS; ++h)
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                a[h][i] = b[h][i] = Chunk<T, VEC>{};
+                if (h < rows && oa[i] < dim) a[h][i] = load_chunk<T, VEC>(in + h * step + oa[i]);
+                if (h < rows && ob[i] < dim) b[h][i] = load_chunk<T, VEC>(in + h * step + ob[i]);
+            }
+    }
+};
 
 // Items of a chunk pair as they meet in a rotation: pair j of a unit is (a[j], b[j]), or
 // neighbouring items of one chunk when interleaved (VEC == 1: always the unit's two
@@ -239,6 +260,33 @@ __device__ __forceinline__ void unpair(const float (&x)[VEC], const float (&y)[V
         } else {
             to[at] = x[j];
             to[at + (VEC > 1)] = y[j];
+        }
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void in_pairs(bool interleaved, const float (&a)[VEC], const float (&b)[VEC], float (&x)[VEC],
+                                         float (&y)[VEC]) {
+    if (interleaved) {
+        pair<VEC>(a, b, x, y);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            x[j] = a[j];
+            y[j] = b[j];
+        }
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void out_of_pairs(bool interleaved, const float (&x)[VEC], const float (&y)[VEC], float (&a)[VEC],
+                                             float (&b)[VEC]) {
+    if (interleaved) {
+        unpair<VEC>(x, y, a, b);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            a[j] = x[j];
+            b[j] = y[j];
         }
     }
 }
@@ -329,20 +377,23 @@ __device__ __forceinline__ float largest_finite(const float (&a)[VEC], float m) 
     return m;
 }
 
-// The scale of a largest magnitude, and its reciprocal.  The lower bound keeps the
+// The scale of a largest magnitude, and its reciprocal.  The lower bound 2^-126 keeps the
 // reciprocal finite and covers a row of zeros.
 struct Scale {
     float value, inverse;
     __device__ Scale(float amax, int e5m2, int e8m0) {
-        value = fmaxf(__fdiv_rn(amax, e5m2 ? 57344.0f : 448.0f), 0x1p-126f);
         if (e8m0) {
-            // a normal number: adding all mantissa bits carries into the exponent unless
-            // they are all zero, which is the power of two not below it.  Its exponent
-            // field is at most 127 + 120, so the reciprocal is a normal number, too.
-            const uint32_t e = (__float_as_uint(value) + 0x007FFFFFu) >> 23;
+            // amax / largest rounded up to a power of two.  largest = 1.75 * 2^8 or
+            // 1.75 * 2^15, so the quotient's power is that of amax, less 8 or 15, one more
+            // if amax's mantissa is above 1.75; the rounding of the quotient to float32
+            // cannot change this, since the float32 after 1.75 * 2^k is 1.75 * 2^k *
+            // (1 + 0.57 * 2^-23).  A field of at most 247 leaves a normal reciprocal.
+            const int field = static_cast<int>((__float_as_uint(amax) + 0x001FFFFFu) >> 23) - (e5m2 ? 15 : 8);
+            const uint32_t e = static_cast<uint32_t>(max(field, 1));
             value = __uint_as_float(e << 23);
             inverse = __uint_as_float((254u - e) << 23);
         } else {
+            value = fmaxf(__fdiv_rn(amax, e5m2 ? 57344.0f : 448.0f), 0x1p-126f);
             inverse = __frcp_rn(value);
         }
     }

@@ -9,46 +9,44 @@ namespace headwise {
 
 enum Mode { kRotate = 1, kWrite = 2, kBoth = 3 };
 
-// Quantise one row held in registers into its cache slot.
+// Quantise one row held in registers into its cache slot: `codes` and `scale_at` are the
+// row's place, oa and ob where the lane's chunks start.
 template <int VEC, int ITER>
-__device__ __forceinline__ void quantise_row(const Params &p, const Role &r, const Lanes &g, const paging::Place &at,
-                                             int head, const float (&a)[ITER][VEC], const float (&b)[ITER][VEC],
-                                             unsigned *group_max) {
-    uint8_t *codes = r.codes + at.page * r.code_page + at.slot * r.code_slot + head * r.code_head;
-    const int64_t scale_at = at.page * r.scale_page + at.slot * r.scale_slot + head * r.scale_head;
-    int oa[ITER], ob[ITER];
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) unit_at<VEC>(r, g.lane + i * g.n, oa[i], ob[i]);
+__device__ __forceinline__ void quantise_row(const Params &p, const Role &r, const Lanes &g, uint8_t *codes,
+                                             int64_t scale_at, const int (&oa)[ITER], const int (&ob)[ITER],
+                                             const float (&a)[ITER][VEC], const float (&b)[ITER][VEC],
+                                             unsigned *group_max, bool there) {
+    const int dim = there ? r.dim : 0;         // a row that is not there stores nothing
     if (r.scale_lanes && r.scale_joint) {
         float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) m = largest<VEC>(b[i], largest<VEC>(a[i], m));
         m = g.max(m, r.scale_lanes);
-        if (__any_sync(g.mask, m > FLT_MAX)) {       // rare: again without the infinities
+        if (__any_sync(0xFFFFFFFFu, m > FLT_MAX)) {       // rare: again without the infinities
             m = 0.0f;
 #pragma unroll
             for (int i = 0; i < ITER; ++i) m = largest_finite<VEC>(b[i], largest_finite<VEC>(a[i], m));
             m = g.max(m, r.scale_lanes);
         }
         const Scale s(m, p.e5m2, p.e8m0);
-        if ((g.lane & (r.scale_lanes - 1)) == 0 && oa[0] < r.dim) s.store(r.scales, scale_at + r.groups_of.quotient(oa[0]), p.e8m0);
+        if ((g.lane & (r.scale_lanes - 1)) == 0 && oa[0] < dim) s.store(r.scales, scale_at + r.groups_of.quotient(oa[0]), p.e8m0);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            if (oa[i] < r.dim) store_codes<VEC>(codes + oa[i], a[i], s.inverse, p.e5m2);
-            if (ob[i] < r.dim) store_codes<VEC>(codes + ob[i], b[i], s.inverse, p.e5m2);
+            if (oa[i] < dim) store_codes<VEC>(codes + oa[i], a[i], s.inverse, p.e5m2);
+            if (ob[i] < dim) store_codes<VEC>(codes + ob[i], b[i], s.inverse, p.e5m2);
         }
     } else if (ITER == 1 && r.scale_lanes) {
         float ma = g.max(largest<VEC>(a[0], 0.0f), r.scale_lanes), mb = g.max(largest<VEC>(b[0], 0.0f), r.scale_lanes);
-        if (__any_sync(g.mask, fmaxf(ma, mb) > FLT_MAX)) {
+        if (__any_sync(0xFFFFFFFFu, fmaxf(ma, mb) > FLT_MAX)) {
             ma = g.max(largest_finite<VEC>(a[0], 0.0f), r.scale_lanes);
             mb = g.max(largest_finite<VEC>(b[0], 0.0f), r.scale_lanes);
         }
         const Scale sa(ma, p.e5m2, p.e8m0), sb(mb, p.e5m2, p.e8m0);
-        if ((g.lane & (r.scale_lanes - 1)) == 0 && oa[0] < r.dim) {
+        if ((g.lane & (r.scale_lanes - 1)) == 0 && oa[0] < dim) {
             sa.store(r.scales, scale_at + r.groups_of.quotient(oa[0]), p.e8m0);
             sb.store(r.scales, scale_at + r.groups_of.quotient(ob[0]), p.e8m0);
         }
-        if (oa[0] < r.dim) {
+        if (oa[0] < dim) {
             store_codes<VEC>(codes + oa[0], a[0], sa.inverse, p.e5m2);
             store_codes<VEC>(codes + ob[0], b[0], sb.inverse, p.e5m2);
         }
@@ -56,45 +54,28 @@ __device__ __forceinline__ void quantise_row(const Params &p, const Role &r, con
         // any other layout of groups: the magnitudes' bit patterns are ordered like the
         // magnitudes, so an integer maximum in shared memory finds them
         const int groups = r.groups_of.quotient(r.dim);
-        __syncwarp(g.mask);
+        __syncwarp();
         for (int k = g.lane; k < groups; k += g.n) group_max[k] = 0u;
-        __syncwarp(g.mask);
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            if (oa[i] < r.dim) atomicMax(&group_max[r.groups_of.quotient(oa[i])], __float_as_uint(largest_finite<VEC>(a[i], 0.0f)));
-            if (ob[i] < r.dim) atomicMax(&group_max[r.groups_of.quotient(ob[i])], __float_as_uint(largest_finite<VEC>(b[i], 0.0f)));
+            if (oa[i] < dim) atomicMax(&group_max[r.groups_of.quotient(oa[i])], __float_as_uint(largest_finite<VEC>(a[i], 0.0f)));
+            if (ob[i] < dim) atomicMax(&group_max[r.groups_of.quotient(ob[i])], __float_as_uint(largest_finite<VEC>(b[i], 0.0f)));
         }
-        __syncwarp(g.mask);
-        for (int k = g.lane; k < groups; k += g.n)
+        __syncwarp();
+        for (int k = g.lane; k < groups && there; k += g.n)
             Scale(__uint_as_float(group_max[k]), p.e5m2, p.e8m0).store(r.scales, scale_at + k, p.e8m0);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            if (oa[i] < r.dim)
+            if (oa[i] < dim)
                 store_codes<VEC>(codes + oa[i], a[i],
                                  Scale(__uint_as_float(group_max[r.groups_of.quotient(oa[i])]), p.e5m2, p.e8m0).inverse, p.e5m2);
-            if (ob[i] < r.dim)
+            if (ob[i] < dim)
                 store_codes<VEC>(codes + ob[i], b[i],
                                  Scale(__uint_as_float(group_max[r.groups_of.quotient(ob[i])]), p.e5m2, p.e8m0).inverse, p.e5m2);
         }
     }
 }
-
-// A group's chunks of kRows rows of one token, as loaded.
-template <typename T, int VEC, int ITER, int ROWS>
-struct Batch {
-    Chunk<T, VEC> a[ROWS][ITER], b[ROWS][ITER];
-    __device__ __forceinline__ void load(const T *in, int64_t step, int rows, const int (&oa)[ITER], const int (&ob)[ITER],
-                                         int dim) {
-#pragma unroll
-        for (int h = 0; h < ROWS; ++h)
-#pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                a[h][i] = b[h][i] = Chunk<T, VEC>{};
-                if (h < rows && oa[i] < dim) a[h][i] = load_chunk<T, VEC>(in + h * step + oa[i]);
-                if (h < rows && ob[i] < dim) b[h][i] = load_chunk<T, VEC>(in + h * step + ob[i]);
-            }
-    }
-};
 
 // What the forward kernel multiplies a row's items by: k0 .. k3 of turn() for rotated
 // units; k0 and k2 are the weights of the two chunks for the others.
@@ -103,25 +84,24 @@ struct Factors {
     float k0[ITER][VEC], k1[ITER][VEC], k2[ITER][VEC], k3[ITER][VEC];
 };
 
-template <typename T, int VEC, int ITER, int MODE>
-__global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_constant__ Params p) {
+// One role's share of the launch.  WHICH is a constant so that every member of the role is
+// an operand in constant memory: indexed by a variable, each use is a load of its own,
+// and those were a quarter of all instructions.
+template <typename T, int VEC, int ITER, int MODE, int WHICH>
+__device__ __forceinline__ void forward_role(const Params &p, uint32_t block, unsigned *group_max) {
     // groups of a scale are at least 16 items, so a lane's share of a row has at most this many
     constexpr int kGroupsPerLane = (2 * VEC * ITER + 15) / 16;
     constexpr int kRows = rows_in_flight(ITER);
-    __shared__ unsigned group_max[MODE == kRotate ? 1 : kThreads * kGroupsPerLane];
-    // A block works for one role, so the role's members are uniform over the block.
-    const uint32_t upto0 = p.role[0].blocks, upto1 = upto0 + p.role[1].blocks;
-    const int which = (blockIdx.x >= upto0) + (blockIdx.x >= upto1);
-    const uint32_t block = blockIdx.x - (which == 0 ? 0 : which == 1 ? upto0 : upto1);
-    const Role &r = p.role[which];
+    constexpr bool rotates = (MODE & kRotate) != 0 && WHICH < 2;
+    constexpr bool quantised = (MODE & kWrite) != 0 && WHICH > 0;
+    const Role &r = p.role[WHICH];
     const Lanes g(p.lanes);
     const uint32_t item = block * (static_cast<uint32_t>(kThreads) >> p.lane_bits) + (threadIdx.x >> p.lane_bits);
-    if (item >= r.all_items) return;                  // whole groups
-    const uint32_t at_token = r.items.quotient(item);
+    bool active = item < r.all_items;                  // the same for a whole group
+    const uint32_t at_token = active ? r.items.quotient(item) : 0;
     const int64_t token = at_token;
-    const int part = static_cast<int>(item - at_token * r.items.d);
-    const int first = part * p.heads_per_item;
-    const int rows = min(r.heads - first, p.heads_per_item);
+    const int first = active ? static_cast<int>(item - at_token * r.items.d) * p.heads_per_item : 0;
+    int rows = active ? min(r.heads - first, p.heads_per_item) : 0;
     int oa[ITER], ob[ITER];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) unit_at<VEC>(r, g.lane + i * g.n, oa[i], ob[i]);
@@ -131,22 +111,28 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
     Batch<T, VEC, ITER, kRows> now;
     now.load(in, r.in_head, rows, oa, ob, r.dim);
 
-    const bool quantised = MODE == kWrite || (MODE == kBoth && r.out == nullptr);
     int64_t position = 0, slot = 0;
-    if (quantised) slot = paging::load_index(p.slots, p.slot_bytes, token);
+    if constexpr (quantised) slot = paging::load_index(p.slots, p.slot_bytes, token);
     if ((MODE & kRotate) && p.positions != nullptr) {
         position = paging::load_index(p.positions, p.position_bytes, token);
-        if (position < 0 || position >= p.table_rows) return;
+        active = active && position >= 0 && position < p.table_rows;
+        if (!active) position = 0;
     }
-    paging::Place at{0, 0, false};
-    if (quantised) {
-        at = paging::place_of_slot(slot, p.pages, p.page_size);
-        if (!at.ok) return;
+    uint8_t *codes = nullptr;
+    int64_t scale_at = 0;
+    T *out = nullptr;
+    if constexpr (quantised) {
+        const paging::Place at = paging::place_of_slot(slot, p.pages, p.page_size);
+        active = active && at.ok;
+        codes = r.codes + at.page * r.code_page + at.slot * r.code_slot + first * r.code_head;
+        scale_at = at.page * r.scale_page + at.slot * r.scale_slot + first * r.scale_head;
+    } else {
+        out = static_cast<T *>(r.out) + token * r.out_token + first * r.out_head;
     }
-    const bool normed = (MODE & kRotate) && p.norm && which < 2;
+    const bool normed = rotates && p.norm;
 
     Factors<VEC, ITER> k;
-    if constexpr ((MODE & kRotate) != 0) {
+    if constexpr (rotates) {
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int u = g.lane + i * g.n;
@@ -155,19 +141,11 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
             for (int j = 0; j < VEC; ++j) wa[j] = wb[j] = 1.0f;
             if (normed && oa[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa[i], wa);
             if (normed && ob[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob[i], wb);
-            if (u < r.angle_units) {
+            if (u < r.angle_units && active) {
                 load_floats<VEC>(p.cos_table + position * p.cos_stride + u * VEC, c);
                 load_floats<VEC>(p.sin_table + position * p.sin_stride + u * VEC, s);
                 float wx[VEC], wy[VEC];
-                if (p.interleaved) {
-                    pair<VEC>(wa, wb, wx, wy);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        wx[j] = wa[j];
-                        wy[j] = wb[j];
-                    }
-                }
+                in_pairs<VEC>(p.interleaved, wa, wb, wx, wy);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     k.k0[i][j] = wx[j] * c[j];
@@ -186,22 +164,24 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
         }
     }
 
+    if (!active) rows = 0;
+    const int most = __reduce_max_sync(0xFFFFFFFFu, rows);
 #pragma unroll 1
-    for (int done = 0; done < rows; done += kRows) {
+    for (int done = 0; done < most; done += kRows) {
         // the next rows are on their way while these are worked on
         Batch<T, VEC, ITER, kRows> next;
         in += kRows * r.in_head;
         next.load(in, r.in_head, rows - done - kRows, oa, ob, r.dim);
 #pragma unroll
         for (int h = 0; h < kRows; ++h) {
-            if (done + h >= rows) break;
+            const bool there = done + h < rows;
             float a[ITER][VEC], b[ITER][VEC];
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
                 widen(now.a[h][i], a[i]);
                 widen(now.b[h][i], b[i]);
             }
-            if constexpr ((MODE & kRotate) != 0) {
+            if constexpr (rotates) {
                 float by = 1.0f;
                 if (normed) {
                     float ss = 0.0f;
@@ -229,20 +209,34 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_co
                     }
                 }
             }
-            const int head = first + done + h;
-            if (!quantised) {
-                T *out = static_cast<T *>(r.out) + token * r.out_token + head * r.out_head;
+            if constexpr (quantised) {
+                quantise_row<VEC, ITER>(p, r, g, codes, scale_at, oa, ob, a, b,
+                                        group_max + (threadIdx.x & ~(g.n - 1)) * kGroupsPerLane, there);
+                codes += r.code_head;
+                scale_at += r.scale_head;
+            } else {
 #pragma unroll
                 for (int i = 0; i < ITER; ++i) {
-                    if (oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a[i]);
-                    if (ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b[i]);
+                    if (there && oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a[i]);
+                    if (there && ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b[i]);
                 }
-            } else if constexpr (MODE != kRotate) {
-                quantise_row<VEC, ITER>(p, r, g, at, head, a, b, group_max + (threadIdx.x & ~(g.n - 1)) * kGroupsPerLane);
+                out += r.out_head;
             }
         }
         now = next;
     }
+}
+
+template <typename T, int VEC, int ITER, int MODE>
+__global__ void __launch_bounds__(kThreads) heads_forward_kernel(const __grid_constant__ Params p) {
+    __shared__ unsigned group_max[MODE == kRotate ? 1 : kThreads * ((2 * VEC * ITER + 15) / 16)];
+    uint32_t block = blockIdx.x;
+    if constexpr ((MODE & kRotate) != 0) {                 // a cache write has no queries
+        if (block < p.role[0].blocks) return forward_role<T, VEC, ITER, MODE, 0>(p, block, group_max);
+        block -= p.role[0].blocks;
+    }
+    if (MODE == kRotate || block < p.role[1].blocks) return forward_role<T, VEC, ITER, MODE, 1>(p, block, group_max);
+    if constexpr (MODE != kRotate) forward_role<T, VEC, ITER, MODE, 2>(p, block - p.role[1].blocks, group_max);
 }
 
 // ---- launch --------------------------------------------------------------------------

@@ -245,6 +245,28 @@ def test_special_values_stay_in_their_rows():
     assert got[2, 1, 5].isnan() and got[3, 0].eq(0).all()
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dtype,dim", [("bfloat16", 128), ("float32", 64), ("float16", 20)])
+def test_an_infinity_reaches_its_own_pair_only(dtype, dim, inter):
+    """Without the norm, nothing but the two items of a pair meet."""
+    _, q, _, _, _, cos, sin, pos = setup(3, 2, 1, dim, dim // 4 * 2, dtype, "contiguous", None, 0)
+    i, j = ref.pairs(dim // 4 * 2, inter)
+    for at in (1, dim // 2 + 1, dim - 1):
+        x = q.clone()
+        x[1, 1, at] = float("inf")
+        partner = int(j[list(i).index(at)]) if at in i else int(i[list(j).index(at)]) if at in j else at
+        for got in (headnorm.norm_rotate(x, None, None, None, cos, sin, pos, interleaved=inter, norm=False)[0],
+                    headnorm.norm_rotate_backward(q, None, None, None, cos, sin, pos, x, None, interleaved=inter, norm=False)[0]):
+            bad = ~torch.isfinite(got.as_torch())
+            assert set(bad.nonzero()[:, 2].tolist()) <= {at, partner} and bad[1, 1, at]
+    # with the norm: a weight's sum is spoilt where the infinite gradient's pair is, and there only
+    g = q.clone()
+    g[1, 1, dim - 1] = float("inf")
+    w = torch.ones(dim, device="cuda", dtype=q.dtype)
+    dw = headnorm.norm_rotate_backward(q, None, w, None, cos, sin, pos, g, None, interleaved=inter)[2].as_torch()
+    assert (~torch.isfinite(dw)).nonzero().flatten().tolist() == [dim - 1]
+
+
 def test_device_arrays_host_arrays_and_raw_bf16():
     rng = np.random.default_rng(5)
     q, w = rng.standard_normal((10, 4, 64)).astype(np.float32), rng.standard_normal(64).astype(np.float32)
