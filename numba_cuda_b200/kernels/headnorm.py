@@ -15,72 +15,67 @@ reduce stops at one axis (numba/cuda/kernels/reduction.py:217-218).  ``kernels.k
 has the form that writes the keys straight into a quantised cache."""
 from __future__ import annotations
 
-import torch
-
 from .. import _lib
-from ..devicearray import _torch_stream, stream_ptr
-from ._operands import (HEAD_FORMATS, ROTATION, heads, index_bytes, indices, like, on_one_device, operand, pack_heads)
-
-
-def _weight(w, what, dim, stream):
-    if w is None:
-        return None
-    op = operand(w, what, stream=stream)
-    if op.format not in HEAD_FORMATS:
-        raise TypeError(f"{what} must be float32, float16 or bfloat16")
-    if len(op.shape) != 1 or op.shape[0] != dim or (dim > 1 and op.strides[0] != 1):
-        raise ValueError(f"{what} must be a contiguous 1-D array of {dim} items")
-    return op
+from ..devicearray import stream_ptr
+from ._operands import (HEAD_FORMATS, ROTATION, heads, index_bytes, indices, like, on_one_device, operand, pack_heads,
+                        vector, workspace)
 
 
 def _table(x, what, stream):
     op = operand(x, what, stream=stream)
-    if op.format != _lib.FMT_F32:
+    if op[3] != _lib.FMT_F32:
         raise TypeError(f"{what} must be float32")
-    if len(op.shape) != 2 or (op.shape[1] > 1 and op.strides[1] != 1):
+    if len(op[1]) != 2 or (op[2][1] != 1 and op[1][1] > 1):
         raise ValueError(f"{what} must be 2-D, (positions, half the rotated items), with unit stride in its last axis")
     return op
 
 
+_NO_ANGLES = (0, 0, 0, 0, 0, 0, 0, 8)
+_NO_ARRAY = (0, 0, 0, 0, 0)
+
+
 def rotation(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, stream):
     """Check the arguments that all calls share: (q, k, all operands, packed b2k_rotation)."""
-    q = heads(q, "q", stream=stream) if q is not None else None
-    k = heads(k, "k", stream=stream) if k is not None else None
+    given = []                           # (operand, members of b2k_heads, its weight's operand)
+    for x, w, what in ((q, q_weight, "q"), (k, k_weight, "k")):
+        if x is None:
+            given.append((None, _NO_ARRAY, None))
+            continue
+        op = heads(x, what, stream=stream)
+        ptr, (_, n, dim), (token, head, _), _, _, _ = op
+        if w is not None:
+            if not norm:
+                raise ValueError("weights belong to the norm: norm=False takes none")
+            w = vector(w, what + "_weight", dim, HEAD_FORMATS, "float32, float16 or bfloat16", False, stream)
+        given.append((op, (ptr, token, head, n, dim), w))
+    (q, q_members, qw), (k, k_members, kw) = given
     first = q if q is not None else k
     if first is None:
         raise ValueError("neither q nor k is given")
-    tokens = first.shape[0]
-    ops = [q, k]
-    if q is not None and k is not None and (k.shape[0] != tokens or k.format != q.format):
+    tokens, fmt = first[1][0], first[3]
+    if k is not None and (k[1][0] != tokens or k[3] != fmt):
         raise ValueError("q and k must have the same number of tokens and the same type")
-    if not norm and (q_weight is not None or k_weight is not None):
-        raise ValueError("weights belong to the norm: norm=False takes none")
-    qw = _weight(q_weight, "q_weight", q.shape[2], stream) if q is not None else None
-    kw = _weight(k_weight, "k_weight", k.shape[2], stream) if k is not None else None
-    if qw is not None and kw is not None and qw.format != kw.format:
-        raise TypeError("q_weight and k_weight must have the same type")
-    ops += [qw, kw]
     weight = qw if qw is not None else kw
-    angles = (0, 0, 0, 0, 0, 0, 0, 8)
+    if kw is not None and kw[3] != weight[3]:
+        raise TypeError("q_weight and k_weight must have the same type")
+    ops = [q, k, qw, kw]
+    rotary, *angles = _NO_ANGLES
     if cos is not None or sin is not None or positions is not None:
         if cos is None or sin is None or positions is None:
             raise ValueError("cos, sin and positions go together")
         c, s = _table(cos, "cos", stream), _table(sin, "sin", stream)
-        if c.shape != s.shape:
+        if c[1] != s[1]:
             raise ValueError("cos and sin must have the same shape")
+        rows, half = c[1]
         at = indices(positions, "positions", tokens, stream)
         ops += [c, s, at]
-        for x in (q, k):
-            if x is not None and 2 * c.shape[1] > x.shape[2]:
-                raise ValueError("cos and sin rotate more items than a head has")
-        angles = (2 * c.shape[1], c.ptr, s.ptr, c.strides[0], s.strides[0], c.shape[0], at.ptr, index_bytes(at))
-    none = (0, 0, 0, 0, 0)
-    packed = ROTATION.pack(
-        first.format, tokens,
-        *((q.ptr, q.strides[0], q.strides[1], q.shape[1], q.shape[2]) if q is not None else none),
-        *((k.ptr, k.strides[0], k.strides[1], k.shape[1], k.shape[2]) if k is not None else none),
-        1 if norm else 0, float(eps), qw.ptr if qw is not None else 0, kw.ptr if kw is not None else 0,
-        weight.format if weight is not None else _lib.FMT_F32, angles[0], 1 if interleaved else 0, *angles[1:])
+        rotary = 2 * half
+        if (q is not None and rotary > q_members[4]) or (k is not None and rotary > k_members[4]):
+            raise ValueError("cos and sin rotate more items than a head has")
+        angles = c[0], s[0], c[2][0], s[2][0], rows, at[0], index_bytes(at)
+    packed = ROTATION.pack(fmt, tokens, *q_members, *k_members, 1 if norm else 0, float(eps), qw[0] if qw is not None else 0,
+                           kw[0] if kw is not None else 0, weight[3] if weight is not None else _lib.FMT_F32, rotary,
+                           1 if interleaved else 0, *angles)
     return q, k, ops, packed
 
 
@@ -92,11 +87,13 @@ def result(out, source, what, stream):
         return None, None
     if out is None:
         out = like(source, stream)
-    op = heads(out, what, written=True, stream=stream)
-    if op.shape != source.shape:
-        raise ValueError(f"{what} must have the shape {source.shape}")
-    if op.format != source.format:
+    op = operand(out, what, True, stream)
+    if op[1] != source[1]:
+        raise ValueError(f"{what} must have the shape {tuple(source[1])}")
+    if op[3] != source[3]:
         raise TypeError(f"{what} must have its input's type")
+    if op[2][2] != 1 and op[1][2] > 1:
+        raise ValueError(f"{what} must have unit stride in its last axis")
     return out, op
 
 
@@ -142,7 +139,7 @@ def norm_rotate_backward(q, k, q_weight, k_weight, cos, sin, positions, q_grad, 
         if (grad is None) != (x is None):
             raise ValueError(f"{what} and its input go together")
         op = heads(grad, what, stream=stream) if x is not None else None
-        if op is not None and (op.shape != x.shape or op.format != x.format):
+        if op is not None and (op[1] != x[1] or op[3] != x[3]):
             raise ValueError(f"{what} must have its input's shape and type")
         grads.append(op)
     for out, x, what in ((dq, q, "dq"), (dk, k, "dk")):
@@ -155,27 +152,17 @@ def norm_rotate_backward(q, k, q_weight, k_weight, cos, sin, positions, q_grad, 
             continue
         if out is None:
             out = like(w, stream)
-        op = operand(out, what, written=True, stream=stream)
-        if op.shape != w.shape or op.format != w.format or (op.shape[0] > 1 and op.strides[0] != 1):
-            raise ValueError(f"{what} must be contiguous with its weight's shape and type")
-        weights.append((out, op))
+        weights.append((out, vector(out, what, w[1][0], (w[3],), "of its weight's type", True, stream)))
     on_one_device([*ops, *grads, *(op for _, op in outs), *(op for _, op in weights)])
     L = _lib.lib()
     scratch, need = None, 0
     if ops[2] is not None or ops[3] is not None:
         need = int(L.b2k_norm_rotate_backward_scratch_bytes(packed))
-        # from torch's allocator on the call's stream, for this call alone: calls on other
-        # streams, and replays of captured graphs, have their own
-        ts = _torch_stream(stream)
-        if torch.cuda.current_stream() == ts:
-            scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
-        else:
-            with torch.cuda.stream(ts):
-                scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+        scratch = workspace(need, stream)
     _lib.check(L.b2k_norm_rotate_backward(
         packed, pack_heads(grads[0]), pack_heads(grads[1]), pack_heads(outs[0][1]), pack_heads(outs[1][1]),
-        weights[0][1].ptr if weights[0][1] is not None else None,
-        weights[1][1].ptr if weights[1][1] is not None else None,
+        weights[0][1][0] if weights[0][1] is not None else None,
+        weights[1][1][0] if weights[1][1] is not None else None,
         scratch.data_ptr() if scratch is not None else None, need, stream_ptr(stream)))
     return outs[0][0], outs[1][0], weights[0][0], weights[1][0]
 

@@ -23,69 +23,89 @@ from __future__ import annotations
 from .. import _lib
 from ..casts import _format_code
 from ..devicearray import stream_ptr
-from ._operands import (CACHE, heads, index_bytes, indices, on_one_device, operand, pack_heads)
+from ._operands import CACHE, INDEX_FORMATS, heads, index_bytes, indices, on_one_device, operand, pack_heads
 from .headnorm import result, rotation
 
-_CODES = {_lib.FMT_E4M3, _lib.FMT_E5M2}
+_CODES = (_lib.FMT_E4M3, _lib.FMT_E5M2)
+_CODE_TYPES = (_lib.FMT_E4M3, _lib.FMT_E5M2, _lib.FMT_U8)
+_SCALE_TYPES = (_lib.FMT_F32, _lib.FMT_E8M0, _lib.FMT_U8)
+_NO_SIDE = (0,) * 11
 
 
 def _side(codes, scales, what, written, stream):
-    """Checked (codes, scales, heads, dim, group) of keys or values."""
-    c = operand(codes, f"{what}_codes", written, stream)
-    s = operand(scales, f"{what}_scales", written, stream)
-    if len(c.shape) != 4 or len(s.shape) != 4 or c.shape[:3] != s.shape[:3]:
+    """Checked operands of keys' or values' codes and scales, and the members of b2k_pages."""
+    c = operand(codes, what + "_codes", written, stream)
+    s = operand(scales, what + "_scales", written, stream)
+    c_ptr, c_shape, c_strides, c_type, _, _ = c
+    s_ptr, s_shape, s_strides, s_type, _, _ = s
+    if len(c_shape) != 4 or len(s_shape) != 4 or c_shape[:3] != s_shape[:3]:
         raise ValueError(f"{what}_codes and {what}_scales must have the axes (pages, page_size, heads, dim) and "
                          "(pages, page_size, heads, groups)")
-    if (c.shape[3] > 1 and c.strides[3] != 1) or (s.shape[3] > 1 and s.strides[3] != 1):
+    _, _, n, dim = c_shape
+    groups = s_shape[3]
+    if (c_strides[3] != 1 and dim > 1) or (s_strides[3] != 1 and groups > 1):
         raise ValueError(f"{what}_codes and {what}_scales must have unit stride in their last axis")
-    if c.format not in _CODES and c.format != _lib.FMT_U8:
+    if c_type not in _CODE_TYPES:
         raise TypeError(f"{what}_codes must be fp8 codes (uint8, float8_e4m3fn or float8_e5m2)")
-    if s.format not in (_lib.FMT_F32, _lib.FMT_U8, _lib.FMT_E8M0):
+    if s_type not in _SCALE_TYPES:
         raise TypeError(f"{what}_scales must be float32 or E8M0 codes (uint8, float8_e8m0fnu)")
-    groups = s.shape[3]
-    if groups < 1 or c.shape[3] % groups:
+    if groups < 1 or dim % groups:
         raise ValueError(f"{what}_scales: the groups must divide the head")
-    return c, s
+    return c, s, (c_ptr, c_strides[0], c_strides[1], c_strides[2], s_ptr, s_strides[0], s_strides[1], s_strides[2], n, dim,
+                  dim // groups)
 
 
 def cache(k_codes, k_scales, v_codes, v_scales, format, written, stream):
-    """Check the cache's arrays: (k codes operand, v codes operand, operands, packed b2k_cache)."""
+    """Check the cache's arrays: (shape of k_codes, of v_codes, operands, packed b2k_cache)."""
     if (k_codes is None) != (k_scales is None) or (v_codes is None) != (v_scales is None):
         raise ValueError("codes and scales go together")
-    sides = [None if k_codes is None else _side(k_codes, k_scales, "k", written, stream),
-             None if v_codes is None else _side(v_codes, v_scales, "v", written, stream)]
-    there = [x for x in sides if x is not None]
-    if not there:
+    code = None
+    if format is not None:
+        code = _format_code(format)
+        if code not in _CODES:
+            raise ValueError("format must be e4m3 or e5m2")
+    k_shape = v_shape = pages = scale = None
+    k_members = v_members = _NO_SIDE
+    ops = []
+    if k_codes is not None:
+        c, s, k_members = _side(k_codes, k_scales, "k", written, stream)
+        ops += [c, s]
+        k_shape = c[1]
+    if v_codes is not None:
+        c, s, v_members = _side(v_codes, v_scales, "v", written, stream)
+        ops += [c, s]
+        v_shape = c[1]
+    for at in range(0, len(ops), 2):
+        told, kind = ops[at][3], ops[at + 1][3]
+        if told != _lib.FMT_U8:
+            if code is not None and code != told:
+                raise TypeError("the codes' types and format disagree")
+            code = told
+        kind = _lib.FMT_F32 if kind == _lib.FMT_F32 else _lib.FMT_E8M0
+        if scale is not None and scale != kind:
+            raise TypeError("the key and the value scales must have the same type")
+        scale = kind
+        if pages is not None and pages != ops[at][1][:2]:
+            raise ValueError("the key and the value cache must have the same pages")
+        pages = ops[at][1][:2]
+    if not ops:
         raise ValueError("neither a key nor a value cache is given")
-    if any(c.shape[:2] != there[0][0].shape[:2] for c, _ in there):
-        raise ValueError("the key and the value cache must have the same pages")
-    told = {c.format for c, _ in there} - {_lib.FMT_U8}
-    code = _format_code(format) if format is not None else None
-    if code is not None and code not in _CODES:
-        raise ValueError("format must be e4m3 or e5m2")
-    if len(told) > 1 or (told and code is not None and code not in told):
-        raise TypeError("the codes' types and format disagree")
-    if code is None:
-        code = told.pop() if told else _lib.FMT_E4M3
-    scale = {_lib.FMT_F32 if s.format == _lib.FMT_F32 else _lib.FMT_E8M0 for _, s in there}
-    if len(scale) > 1:
-        raise TypeError("the key and the value scales must have the same type")
-    values = [code, scale.pop(), there[0][0].shape[0], there[0][0].shape[1]]
-    for side in sides:
-        if side is None:
-            values += [0] * 11
-        else:
-            c, s = side
-            values += [c.ptr, *c.strides[:3], s.ptr, *s.strides[:3], c.shape[2], c.shape[3], c.shape[3] // s.shape[3]]
-    return (sides[0][0] if sides[0] else None, sides[1][0] if sides[1] else None,
-            [op for side in there for op in side], CACHE.pack(*values))
+    return k_shape, v_shape, ops, CACHE.pack(_lib.FMT_E4M3 if code is None else code, scale, *pages, *k_members, *v_members)
 
 
-def _fits(x, codes, what):
-    if (x is None) != (codes is None):
+def _fits(op, shape, what):
+    if (op is None) != (shape is None):
         raise ValueError(f"{what} and its cache go together")
-    if x is not None and x.shape[1:] != codes.shape[2:]:
-        raise ValueError(f"{what} has heads of the shape {x.shape[1:]}, its cache {codes.shape[2:]}")
+    if op is not None and op[1][1:] != shape[2:]:
+        raise ValueError(f"{what} has heads of the shape {tuple(op[1][1:])}, its cache {tuple(shape[2:])}")
+
+
+def _pair(k, v, what):
+    """The number of tokens (rows) and the type of k and v, of which one may be missing."""
+    first = k if k is not None else v
+    if k is not None and v is not None and (k[1][0] != v[1][0] or k[3] != v[3]):
+        raise ValueError(f"{what} and the same type")
+    return first[1][0], first[3]
 
 
 def write(k, v, k_codes, k_scales, v_codes, v_scales, slots, format=None, stream=0):
@@ -103,13 +123,11 @@ def write(k, v, k_codes, k_scales, v_codes, v_scales, slots, format=None, stream
     kc, vc, ops, packed = cache(k_codes, k_scales, v_codes, v_scales, format, True, stream)
     _fits(k, kc, "k")
     _fits(v, vc, "v")
-    first = k if k is not None else v
-    if k is not None and v is not None and (k.shape[0] != v.shape[0] or k.format != v.format):
-        raise ValueError("k and v must have the same number of tokens and the same type")
-    at = indices(slots, "slots", first.shape[0], stream)
-    on_one_device([k, v, at, *ops])
-    _lib.check(_lib.lib().b2k_cache_write(packed, first.format, first.shape[0], pack_heads(k), pack_heads(v), at.ptr,
-                                          index_bytes(at), stream_ptr(stream)))
+    tokens, fmt = _pair(k, v, "k and v must have the same number of tokens")
+    at = indices(slots, "slots", tokens, stream)
+    on_one_device((k, v, at, *ops))
+    _lib.check(_lib.lib().b2k_cache_write(packed, fmt, tokens, pack_heads(k), pack_heads(v), at[0], index_bytes(at),
+                                          stream_ptr(stream)))
 
 
 def read(k_codes, k_scales, v_codes, v_scales, page_table, offsets, k_out, v_out, format=None, stream=0):
@@ -129,19 +147,17 @@ def read(k_codes, k_scales, v_codes, v_scales, page_table, offsets, k_out, v_out
     kc, vc, ops, packed = cache(k_codes, k_scales, v_codes, v_scales, format, False, stream)
     _fits(ko, kc, "k_out")
     _fits(vo, vc, "v_out")
-    first = ko if ko is not None else vo
-    if ko is not None and vo is not None and (ko.shape[0] != vo.shape[0] or ko.format != vo.format):
-        raise ValueError("k_out and v_out must have the same number of rows and the same type")
+    rows, fmt = _pair(ko, vo, "k_out and v_out must have the same number of rows")
     table = operand(page_table, "page_table", stream=stream)
-    if table.format not in (_lib.FMT_I32, _lib.FMT_I64):
+    if table[3] not in INDEX_FORMATS:
         raise TypeError("page_table must be int32 or int64")
-    if len(table.shape) != 2 or (table.shape[1] > 1 and table.strides[1] != 1):
+    if len(table[1]) != 2 or (table[2][1] != 1 and table[1][1] > 1):
         raise ValueError("page_table must be 2-D, (sequences, width), with unit stride in its last axis")
-    at = indices(offsets, "offsets", table.shape[0] + 1, stream)
-    on_one_device([ko, vo, table, at, *ops])
-    _lib.check(_lib.lib().b2k_cache_read(packed, first.format, first.shape[0], pack_heads(ko), pack_heads(vo), table.ptr,
-                                         table.strides[0], table.shape[1], index_bytes(table), at.ptr, table.shape[0],
-                                         index_bytes(at), stream_ptr(stream)))
+    sequences, width = table[1]
+    at = indices(offsets, "offsets", sequences + 1, stream)
+    on_one_device((ko, vo, table, at, *ops))
+    _lib.check(_lib.lib().b2k_cache_read(packed, fmt, rows, pack_heads(ko), pack_heads(vo), table[0], table[2][0], width,
+                                         index_bytes(table), at[0], sequences, index_bytes(at), stream_ptr(stream)))
     return k_out, v_out
 
 
@@ -160,12 +176,12 @@ def norm_rotate_write(q, k, v, q_weight, k_weight, cos, sin, positions, k_codes,
     _fits(k, kc, "k")
     _fits(v, vc, "v")
     first = q if q is not None else k
-    if v is not None and (v.shape[0] != first.shape[0] or v.format != first.format):
+    if v is not None and (v[1][0] != first[1][0] or v[3] != first[3]):
         raise ValueError("v must have the tokens and the type of q and k")
-    at = indices(slots, "slots", first.shape[0], stream)
-    on_one_device([*ops, v, qo, at, *more])
-    _lib.check(_lib.lib().b2k_norm_rotate_write(packed, pack_heads(v), pack_heads(qo), packed_cache, at.ptr,
-                                                index_bytes(at), stream_ptr(stream)))
+    at = indices(slots, "slots", first[1][0], stream)
+    on_one_device((*ops, v, qo, at, *more))
+    _lib.check(_lib.lib().b2k_norm_rotate_write(packed, pack_heads(v), pack_heads(qo), packed_cache, at[0], index_bytes(at),
+                                                stream_ptr(stream)))
     return q_out
 
 
