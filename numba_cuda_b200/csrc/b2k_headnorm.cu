@@ -223,7 +223,7 @@ static bool role_fits(const Params &p, const Role &r, bool rotated, int rotary, 
         return false;
     if (r.codes && (!fits(r.codes, r.code_page, r.code_slot, 1, vec) || r.code_head % vec || r.group % vec)) return false;
     if (rotated) {
-        if (rotary % (2 * vec)) return false;
+        if (rotary % (p.interleaved ? vec : 2 * vec)) return false;
         const int w = vec < 4 ? vec : 4;
         if (!fits(p.cos_table, p.cos_stride, 0, 4, w) || !fits(p.sin_table, p.sin_stride, 0, 4, w)) return false;
     }
@@ -248,17 +248,23 @@ Plan choose(Params &p, int64_t format, const b2k_rotation *rot) {
     for (int i = 0; i < 3; ++i) {
         Role &r = p.role[i];
         if (r.heads == 0) continue;
-        const int turned = i < 2 ? rotary : 0;
-        // the two halves of a rotated run pair up; without a rotation of halves the pairs are
-        // the row's two halves where they are whole chunks, else neighbouring chunks
-        int paired = 0;
-        if (turned && !p.interleaved) paired = turned;
-        else if (!turned && r.dim % (2 * plan.vec) == 0) paired = r.dim;
-        r.pair_gap = paired / 2;
-        r.pair_units = paired / 2 / plan.vec;
-        r.tail = paired;
-        r.angle_units = turned / 2 / plan.vec;
-        r.units = r.pair_units + (r.dim - r.tail + 2 * plan.vec - 1) / (2 * plan.vec);
+        const int turned = i < 2 ? rotary : 0, vec = plan.vec;
+        // The halves of a rotated run pair up, and what lies behind it lies in pairs of
+        // neighbouring chunks.  Without a rotation of halves the two halves of the row pair
+        // up; single interleaved items (vec == 1) pair with their neighbours.
+        if (turned && !p.interleaved) {
+            r.pair_gap = turned / 2;
+            r.tail = turned;
+        } else if (turned && vec == 1) {
+            r.pair_gap = r.tail = 0;
+        } else {
+            r.pair_gap = (r.dim / vec + 1) / 2 * vec;
+            r.tail = r.dim;
+        }
+        r.pair_units = r.pair_gap / vec;
+        r.angle_units = turned / 2 / vec;
+        r.angle_items = turned;
+        r.units = r.pair_units + (r.dim - r.tail + 2 * vec - 1) / (2 * vec);
         if (r.units > units) units = r.units;
     }
     p.lanes = 1;
@@ -276,13 +282,12 @@ Plan choose(Params &p, int64_t format, const b2k_rotation *rot) {
         if (r.codes == nullptr) continue;
         r.groups_of = paging::divisor(static_cast<uint32_t>(r.group));
         // how the chunks of a scale's group lie over the lanes; see quantise_row
-        const int run = r.pair_units ? plan.vec : 2 * plan.vec;      // neighbouring items of a lane
-        const int span = r.group / run;
-        const bool even = r.group % run == 0 && (span & (span - 1)) == 0;
+        const int span = r.group / plan.vec;
+        const bool even = r.group % plan.vec == 0 && (span & (span - 1)) == 0;
         r.scale_lanes = 0;
-        r.scale_joint = r.group == r.dim || r.pair_units == 0;
-        if (r.group == r.dim) r.scale_lanes = p.lanes;
-        else if (plan.iter == 1 && even && (r.pair_units == 0 || (r.tail == r.dim && r.pair_gap % r.group == 0)))
+        r.scale_joint = r.group == r.dim;
+        if (r.scale_joint) r.scale_lanes = p.lanes;
+        else if (plan.iter == 1 && even && r.tail == r.dim && r.dim == 2 * r.pair_gap && r.pair_gap % r.group == 0)
             r.scale_lanes = span;
     }
     return plan;
@@ -295,13 +300,12 @@ int count_items(Params &p, int most, int threads, const char *name) {
     int64_t rows = 0;
     for (const Role &r : p.role) rows += r.heads;
     rows = rows > 0 && p.tokens > INT64_MAX / 64 / rows ? INT64_MAX / 64 : rows * p.tokens;
-    p.heads_per_item = most;
-    while (p.heads_per_item > 1 && rows * p.lanes / p.heads_per_item < static_cast<int64_t>(1024) * b2k::sm_count())
-        p.heads_per_item /= 2;
+    while (most > 1 && rows * p.lanes / most < static_cast<int64_t>(1024) * b2k::sm_count()) most /= 2;
     const int64_t in_block = threads / p.lanes;
     int64_t blocks = 0;
     for (Role &r : p.role) {
-        const int64_t per_token = (r.heads + p.heads_per_item - 1) / p.heads_per_item;
+        const int64_t per_token = (r.heads + most - 1) / most;
+        r.heads_per_item = per_token ? static_cast<int>((r.heads + per_token - 1) / per_token) : 1;      // even shares
         if (per_token && p.tokens > INT_MAX / per_token)
             return b2k::fail(B2K_ERR_TOO_LARGE, "%s: more than 2^31 - 1 groups of rows", name);
         r.items = paging::divisor(static_cast<uint32_t>(per_token ? per_token : 1));
@@ -321,7 +325,7 @@ constexpr int kMostBlocksPerSm = 8;
 constexpr int kBackwardHeadsPerItem = 8;
 
 // The inverse rotation of a unit's pairs.
-template <int VEC>
+template <int FROM, int TO, int VEC>
 __device__ __forceinline__ void turn_back(float (&x)[VEC], float (&y)[VEC], const float (&c)[VEC], const float (&s)[VEC]) {
     if constexpr (VEC == 1) {
         const float u = x[0] * c[0] + y[0] * s[0], v = y[0] * c[0] - x[0] * s[0];
@@ -329,7 +333,7 @@ __device__ __forceinline__ void turn_back(float (&x)[VEC], float (&y)[VEC], cons
         y[0] = v;
     } else {
 #pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
+        for (int j = FROM; j < TO; j += 2) {
             const float2 a = make_float2(x[j], x[j + 1]), b = make_float2(y[j], y[j + 1]);
             const float2 cc = make_float2(c[j], c[j + 1]), sn = make_float2(s[j], s[j + 1]);
             const float2 u = fma2(a, cc, mul2(b, sn));
@@ -406,8 +410,8 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
         const bool active = item < r.all_items;
         const uint32_t at_token = active ? r.items.quotient(item) : 0;
         const int64_t token = at_token;
-        const int first = active ? static_cast<int>(item - at_token * r.items.d) * p.heads_per_item : 0;
-        const int rows = active ? min(r.heads - first, p.heads_per_item) : 0;
+        const int first = active ? static_cast<int>(item - at_token * r.items.d) * r.heads_per_item : 0;
+        const int rows = active ? min(r.heads - first, r.heads_per_item) : 0;
         const T *in = static_cast<const T *>(r.in) + token * r.in_token + first * r.in_head;
         const T *grad = static_cast<const T *>(r.grad) + token * r.grad_token + first * r.grad_head;
         T *out = static_cast<T *>(r.out) + token * r.out_token + first * r.out_head;
@@ -418,14 +422,15 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
         if (p.positions != nullptr) position = paging::load_index(p.positions, p.position_bytes, token);
         // a padding token's rows are taken as zeros all through, with by = 0 below
         const bool padding = p.positions != nullptr && (position < 0 || position >= p.table_rows);
-        float c[ITER][VEC] = {}, s[ITER][VEC] = {};
+        float c[ITER][VEC], s[ITER][VEC];
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int u = g.lane + i * g.n;
-            if (u < r.angle_units && !padding) {
-                load_floats<VEC>(p.cos_table + position * p.cos_stride + u * VEC, c[i]);
-                load_floats<VEC>(p.sin_table + position * p.sin_stride + u * VEC, s[i]);
-            }
+            Turned t = turned_of<VEC>(r, swap, u, oa[i], ob[i]);
+            t.lo = t.lo && !padding;
+            t.hi = t.hi && !padding;
+            load_angles<VEC>(p.cos_table + position * p.cos_stride, swap, u, oa[i], ob[i], t, c[i]);
+            load_angles<VEC>(p.sin_table + position * p.sin_stride, swap, u, oa[i], ob[i], t, s[i]);
         }
         const int most = __reduce_max_sync(0xFFFFFFFFu, rows);
 #pragma unroll 1
@@ -448,7 +453,9 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
                 widen(g_now.a[0][i], a);
                 widen(g_now.b[0][i], b);
                 in_pairs<VEC>(swap, a, b, gx[i], gy[i]);
-                if (g.lane + i * g.n < r.angle_units) turn_back<VEC>(gx[i], gy[i], c[i], s[i]);
+                const Turned t = turned_of<VEC>(r, swap, g.lane + i * g.n, oa[i], ob[i]);
+                if (VEC > 1 && t.lo) turn_back<0, VEC / 2, VEC>(gx[i], gy[i], c[i], s[i]);
+                if (t.hi) turn_back<VEC / 2, VEC, VEC>(gx[i], gy[i], c[i], s[i]);
                 gradient_sums<VEC>(x[i], gx[i], wx[i], ss, dot);
                 gradient_sums<VEC>(y[i], gy[i], wy[i], ss, dot);
             }
@@ -506,8 +513,10 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
     }
 }
 
+// Four blocks an SM where a row takes one unit a lane (128 registers; 32768 tokens x 40
+// heads of 128 bf16 items: 208 us, with three blocks of 146 registers 234 us).
 template <typename T, int VEC, int ITER>
-__global__ void __launch_bounds__(kThreads) heads_backward_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, ITER == 1 ? 4 : 1) heads_backward_kernel(const __grid_constant__ Params p) {
     extern __shared__ float block_sums[];             // one row of dim floats per warp
     if (static_cast<int>(blockIdx.x) < p.blocks0) backward_role<T, VEC, ITER, 0>(p, blockIdx.x, p.blocks0, block_sums);
     else backward_role<T, VEC, ITER, 1>(p, blockIdx.x - p.blocks0, gridDim.x - p.blocks0, block_sums);

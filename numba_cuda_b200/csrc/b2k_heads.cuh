@@ -22,7 +22,7 @@ constexpr int kThreads = 128;
 // weights are loaded once for the latter.  Rows that spread over several units a lane
 // leave registers for one.
 B2K_HD constexpr int rows_in_flight(int iter) { return iter == 1 ? 2 : 1; }
-constexpr int kHeadsPerItem = 8;
+constexpr int kHeadsPerItem = 16;
 
 // One array role of a launch (queries, keys or values).
 struct Role {
@@ -41,7 +41,9 @@ struct Role {
     uint32_t all_items, blocks; // of the launch
     int units;                  // chunk pairs of a row
     int pair_units, pair_gap, tail;   // units below pair_units are (u, u + gap); the others lie from `tail` on
-    int angle_units;            // units below it are rotated
+    int angle_units;            // units below it are rotated (pairs of halves, or of single items)
+    int angle_items;            // chunks below it are rotated (interleaved pairs)
+    int heads_per_item;
     int scale_lanes, scale_joint;     // lanes that share a scale (0: found through shared memory), and whether
                                       // a lane's two chunks do
     float inv_dim;
@@ -50,7 +52,7 @@ struct Role {
 struct Params {
     Role role[3];
     int64_t tokens;
-    int heads_per_item, lanes, lane_bits;
+    int lanes, lane_bits;
     int norm, interleaved, weight_format;
     float eps;
     const float *cos_table, *sin_table;
@@ -291,28 +293,64 @@ __device__ __forceinline__ void out_of_pairs(bool interleaved, const float (&x)[
     }
 }
 
-// (x, y) -> (x k0 - y k1, y k2 + x k3), `scale` times: rotation, weights and norm of a
-// pair in one step, with k0 = w_x cos, k1 = w_y sin, k2 = w_y cos, k3 = w_x sin.
+// Which half of a unit's pairs is rotated: all or none for pairs of halves, one chunk's
+// pairs each when interleaved.
+struct Turned {
+    bool lo, hi;
+};
 template <int VEC>
-__device__ __forceinline__ void turn(float (&x)[VEC], float (&y)[VEC], const float (&k0)[VEC], const float (&k1)[VEC],
-                                     const float (&k2)[VEC], const float (&k3)[VEC], float scale) {
+__device__ __forceinline__ Turned turned_of(const Role &r, bool interleaved, int u, int oa, int ob) {
+    if (VEC > 1 && interleaved) return Turned{oa < r.angle_items, ob < r.angle_items};
+    return Turned{u < r.angle_units, u < r.angle_units};
+}
+
+// A unit's cosines or sines, from its position's row of the table; zeros where nothing is rotated.
+template <int VEC>
+__device__ __forceinline__ void load_angles(const float *row, bool interleaved, int u, int oa, int ob, Turned t,
+                                            float (&v)[VEC]) {
     if constexpr (VEC == 1) {
-        const float u = x[0] * k0[0] - y[0] * k1[0], v = y[0] * k2[0] + x[0] * k3[0];
+        v[0] = t.lo ? row[u] : 0.0f;
+    } else {
+        constexpr int H = VEC / 2;
+        float lo[H] = {}, hi[H] = {};
+        if (t.lo) load_floats<H>(row + (interleaved ? oa / 2 : u * VEC), lo);
+        if (t.hi) load_floats<H>(row + (interleaved ? ob / 2 : u * VEC + H), hi);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            v[j] = lo[j];
+            v[H + j] = hi[j];
+        }
+    }
+}
+
+// (x, y) -> scale (x k0 - y k1, y k2 + x k3): rotation, weights and norm of a pair in one
+// step, with k0 = w_x cos, k1 = w_y sin, k2 = w_y cos, k3 = w_x sin.  Pairs that are not
+// rotated are scaled by their weights k0, k2 alone: a product with a zero sine would
+// carry an infinity over to the partner.
+template <int FROM, int TO, int VEC>
+__device__ __forceinline__ void turn(float (&x)[VEC], float (&y)[VEC], const float (&k0)[VEC], const float (&k1)[VEC],
+                                     const float (&k2)[VEC], const float (&k3)[VEC], float scale, bool turned) {
+    if constexpr (VEC == 1) {
+        const float u = turned ? x[0] * k0[0] - y[0] * k1[0] : x[0] * k0[0];
+        const float v = turned ? y[0] * k2[0] + x[0] * k3[0] : y[0] * k2[0];
         x[0] = u * scale;
         y[0] = v * scale;
     } else {
         const float2 by = make_float2(scale, scale);
 #pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
+        for (int j = FROM; j < TO; j += 2) {
             const float2 xx = make_float2(x[j], x[j + 1]), yy = make_float2(y[j], y[j + 1]);
-            const float2 nn = make_float2(-y[j], -y[j + 1]);
-            const float2 u = fma2(xx, make_float2(k0[j], k0[j + 1]), mul2(nn, make_float2(k1[j], k1[j + 1])));
-            const float2 v = fma2(yy, make_float2(k2[j], k2[j + 1]), mul2(xx, make_float2(k3[j], k3[j + 1])));
-            const float2 us = mul2(u, by), vs = mul2(v, by);
-            x[j] = us.x;
-            x[j + 1] = us.y;
-            y[j] = vs.x;
-            y[j + 1] = vs.y;
+            float2 u = mul2(xx, make_float2(k0[j], k0[j + 1])), v = mul2(yy, make_float2(k2[j], k2[j + 1]));
+            if (turned) {
+                u = fma2(make_float2(-yy.x, -yy.y), make_float2(k1[j], k1[j + 1]), u);
+                v = fma2(xx, make_float2(k3[j], k3[j + 1]), v);
+            }
+            u = mul2(u, by);
+            v = mul2(v, by);
+            x[j] = u.x;
+            x[j + 1] = u.y;
+            y[j] = v.x;
+            y[j + 1] = v.y;
         }
     }
 }
