@@ -78,6 +78,8 @@ B2K_API int b2k_version(void);
 B2K_API const char *b2k_last_error(void);
 /* number of kernels this library has launched in the calling process */
 B2K_API int64_t b2k_launch_count(void);
+/* ordinal of the current device, -1 without one */
+B2K_API int b2k_current_device(void);
 
 /* ---- reduce -------------------------------------------------------------
  * Replaces the three launches + partials allocation of Reduce.__call__

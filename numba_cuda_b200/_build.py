@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -95,6 +96,22 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+PYFAST = os.path.join(HERE, "_pyfast" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_pyfast(force: bool = False) -> str:
+    """Compile the Python extension ``csrc/b2k_pyfast.cpp`` (host code only) in-tree."""
+    src = os.path.join(CSRC, "b2k_pyfast.cpp")
+    if force or _stale(PYFAST, _deps(src)):
+        cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared",
+               "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"], src, "-o", PYFAST]
+        p = subprocess.run(cmd, capture_output=True, text=True)
+        if p.returncode != 0:
+            sys.stderr.write(p.stdout + p.stderr)
+            raise RuntimeError("building _pyfast failed")
+    return PYFAST
+
+
 EXAMPLES_LIB = os.path.join(CSRC, "examples", "libb2k_examples.so")
 
 
@@ -113,5 +130,6 @@ def build_examples(force: bool = False) -> str:
 
 
 if __name__ == "__main__":
+    build_pyfast(force="--force" in sys.argv)
     build_examples(force="--force" in sys.argv)
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))

@@ -31,6 +31,7 @@ SIGNATURES = {
     "b2k_version": (_i32, []),
     "b2k_last_error": (ctypes.c_char_p, []),
     "b2k_launch_count": (_i64, []),
+    "b2k_current_device": (_i32, []),
     "b2k_reduce_scratch_bytes": (_i64, []),
     "b2k_reduce": (_i32, [_i32, _i32, _vp, _i64, _vp, _vp, _vp, _i64, _vp]),
     "b2k_reduce_ex": (_i32, [_i32, _i32, _vp, _i64, _vp, _vp, _vp, _i64, ctypes.c_uint, _vp]),

@@ -73,4 +73,6 @@ const char *b2k_last_error(void) { return b2k::g_error; }
 
 int64_t b2k_launch_count(void) { return b2k::g_launches.load(std::memory_order_relaxed); }
 
+int b2k_current_device(void) { return b2k::current_device(); }
+
 }  // extern "C"

@@ -7,6 +7,7 @@ exports the CUDA Array Interface; host arrays are copied to the device where the
 only read."""
 from __future__ import annotations
 
+import ctypes
 import struct
 
 import numpy as np
@@ -131,4 +132,35 @@ def workspace(nbytes, stream):
         return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
 
 
-__all__ = ["operand", "heads", "vector", "indices", "pack_heads", "index_bytes", "on_one_device", "like", "workspace"]
+class _NoFast:
+    """Stands for the extension where it was not built: every call takes the Python code."""
+
+    @staticmethod
+    def _pass(*args):
+        return None
+
+    norm_rotate = norm_rotate_backward = cache_write = cache_read = norm_rotate_write = _pass
+
+
+class _Fast:
+    """The extension ``_pyfast``, set up when it is first used (it needs the library)."""
+
+    def __getattr__(self, name):
+        try:
+            from .. import _pyfast as module
+        except ImportError:
+            module = _NoFast
+        else:
+            L = _lib.lib()
+            names = ("b2k_norm_rotate", "b2k_norm_rotate_backward_scratch_bytes", "b2k_norm_rotate_backward",
+                     "b2k_cache_write", "b2k_cache_read", "b2k_norm_rotate_write", "b2k_current_device")
+            module.setup(torch.Tensor, _TORCH, {n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names},
+                         stream_ptr, workspace)
+        for entry in ("norm_rotate", "norm_rotate_backward", "cache_write", "cache_read", "norm_rotate_write"):
+            setattr(self, entry, getattr(module, entry))
+        return self.__dict__[name]
+
+
+fast = _Fast()
+
+__all__ = ["operand", "heads", "vector", "indices", "pack_heads", "index_bytes", "on_one_device", "like", "workspace", "fast"]

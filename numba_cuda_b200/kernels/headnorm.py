@@ -17,7 +17,7 @@ from __future__ import annotations
 
 from .. import _lib
 from ..devicearray import stream_ptr
-from ._operands import (HEAD_FORMATS, ROTATION, heads, index_bytes, indices, like, on_one_device, operand, pack_heads,
+from ._operands import (HEAD_FORMATS, ROTATION, fast, heads, index_bytes, indices, like, on_one_device, operand, pack_heads,
                         vector, workspace)
 
 
@@ -116,6 +116,10 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, position
                  set).  An output may be its own input's memory; it must not overlap an
                  input in any other way.
     """
+    status = fast.norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, q_out, k_out, stream)
+    if status is not None:
+        _lib.check(status)
+        return q_out, k_out
     q, k, ops, packed = rotation(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, stream)
     q_out, qo = result(q_out, q, "q_out", stream)
     k_out, ko = result(k_out, k, "k_out", stream)
@@ -133,6 +137,11 @@ def norm_rotate_backward(q, k, q_weight, k_weight, cos, sin, positions, q_grad, 
     an order that depends on the shapes only, and are stored in the weights' type.  A
     padding token has zero gradients and adds nothing to the sums.  ``dq`` and ``dk`` may be
     the memory of ``q_grad`` and ``k_grad``."""
+    status = fast.norm_rotate_backward(q, k, q_weight, k_weight, cos, sin, positions, q_grad, k_grad, eps, interleaved,
+                                       norm, dq, dk, dq_weight, dk_weight, stream)
+    if status is not None:
+        _lib.check(status)
+        return dq, dk, dq_weight, dk_weight
     q, k, ops, packed = rotation(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, stream)
     grads, outs, weights = [], [], []
     for grad, x, what in ((q_grad, q, "q_grad"), (k_grad, k, "k_grad")):

@@ -23,7 +23,7 @@ from __future__ import annotations
 from .. import _lib
 from ..casts import _format_code
 from ..devicearray import stream_ptr
-from ._operands import CACHE, INDEX_FORMATS, heads, index_bytes, indices, on_one_device, operand, pack_heads
+from ._operands import CACHE, INDEX_FORMATS, fast, heads, index_bytes, indices, on_one_device, operand, pack_heads
 from .headnorm import result, rotation
 
 _CODES = (_lib.FMT_E4M3, _lib.FMT_E5M2)
@@ -118,6 +118,9 @@ def write(k, v, k_codes, k_scales, v_codes, v_scales, slots, format=None, stream
                  and scales a slot gets is not defined when two share it.
     :param format: ``"e4m3"`` (the default for untyped codes) or ``"e5m2"``.
     """
+    status = fast.cache_write(k, v, k_codes, k_scales, v_codes, v_scales, slots, format, stream)
+    if status is not None:
+        return _lib.check(status)
     k = heads(k, "k", stream=stream) if k is not None else None
     v = heads(v, "v", stream=stream) if v is not None else None
     kc, vc, ops, packed = cache(k_codes, k_scales, v_codes, v_scales, format, True, stream)
@@ -142,6 +145,10 @@ def read(k_codes, k_scales, v_codes, v_scales, page_table, offsets, k_out, v_out
     :param k_out, v_out: (rows, heads, dim) arrays, float32, float16 or bfloat16; either may
                  be ``None``, with its cache.  Values beyond the type's range saturate.
     """
+    status = fast.cache_read(k_codes, k_scales, v_codes, v_scales, page_table, offsets, k_out, v_out, format, stream)
+    if status is not None:
+        _lib.check(status)
+        return k_out, v_out
     ko = heads(k_out, "k_out", True, stream) if k_out is not None else None
     vo = heads(v_out, "v_out", True, stream) if v_out is not None else None
     kc, vc, ops, packed = cache(k_codes, k_scales, v_codes, v_scales, format, False, stream)
@@ -169,6 +176,11 @@ def norm_rotate_write(q, k, v, q_weight, k_weight, cos, sin, positions, k_codes,
     beside it.  Arguments as for ``headnorm.norm_rotate`` and ``write``; a token whose
     position is no row of the tables is skipped altogether, one whose slot is outside
     the cache writes its row of ``q_out`` only."""
+    status = fast.norm_rotate_write(q, k, q_weight, k_weight, cos, sin, positions, v, k_codes, k_scales, v_codes, v_scales,
+                                    slots, eps, interleaved, norm, format, q_out, stream)
+    if status is not None:
+        _lib.check(status)
+        return q_out
     q, k, ops, packed = rotation(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, stream)
     v = heads(v, "v", stream=stream) if v is not None else None
     q_out, qo = result(q_out, q, "q_out", stream)
