@@ -522,24 +522,35 @@ __global__ void __launch_bounds__(kThreads, ITER == 1 ? 4 : 1) heads_backward_ke
     else backward_role<T, VEC, ITER, 1>(p, blockIdx.x - p.blocks0, gridDim.x - p.blocks0, block_sums);
 }
 
-// weight_grad[d] = sum over the role's blocks of partials[block][d], 32 columns a block:
-// eight rows of threads stride over the blocks, then a fixed tree.
-__global__ void __launch_bounds__(kThreads) weight_grad_kernel(const __grid_constant__ Params p, int blocks) {
-    __shared__ float part[kThreads / 32][32];
+// weight_grad[d] = sum over the role's blocks of partials[block][d], 32 columns a block: 32
+// warps stride over the partial rows with four loads in flight, then one warp a column
+// folds their sums.  The order depends on the grid alone.  (With 4 warps and one load in
+// flight this took 25 us for 592 rows of 128.)
+constexpr int kSumThreads = 1024;
+
+__global__ void __launch_bounds__(kSumThreads) weight_grad_kernel(const __grid_constant__ Params p, int blocks) {
+    __shared__ float part[32][33];
     const Role &r = p.role[blockIdx.y];
     if (r.weight_grad == nullptr) return;
-    const int d = blockIdx.x * 32 + threadIdx.x % 32, row = threadIdx.x / 32;
+    const int column = threadIdx.x % 32, row = threadIdx.x / 32;
     const int begin = blockIdx.y ? p.blocks0 : 0, end = blockIdx.y ? blocks : p.blocks0;
-    float v = 0.0f;
+    const int d = blockIdx.x * 32 + column;
+    float v[4] = {};
     if (d < r.dim)
-        for (int b = begin + row; b < end; b += kThreads / 32) v += p.partials[static_cast<int64_t>(b) * p.partial_stride + d];
-    part[row][threadIdx.x % 32] = v;
+        for (int b = begin + row; b < end; b += 4 * 32)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (b + i * 32 < end) v[i] += p.partials[static_cast<int64_t>(b + i * 32) * p.partial_stride + d];
+    part[row][column] = (v[0] + v[1]) + (v[2] + v[3]);
     __syncthreads();
-    if (row || d >= r.dim) return;
-    for (int w = 1; w < kThreads / 32; ++w) v += part[w][threadIdx.x];
-    if (p.weight_format == B2K_FMT_F32) static_cast<float *>(r.weight_grad)[d] = v;
-    else if (p.weight_format == B2K_FMT_F16) static_cast<__half *>(r.weight_grad)[d] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16 *>(r.weight_grad)[d] = __float2bfloat16_rn(v);
+    float sum = part[column][row];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    const int at = blockIdx.x * 32 + row;
+    if (column || at >= r.dim) return;
+    if (p.weight_format == B2K_FMT_F32) static_cast<float *>(r.weight_grad)[at] = sum;
+    else if (p.weight_format == B2K_FMT_F16) static_cast<__half *>(r.weight_grad)[at] = __float2half_rn(sum);
+    else static_cast<__nv_bfloat16 *>(r.weight_grad)[at] = __float2bfloat16_rn(sum);
 }
 
 // Blocks of one instantiation that an SM holds at once: the grid is one full wave, since
@@ -680,7 +691,7 @@ int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, con
         b2k::note_launch();
     }
     if (summed) {
-        weight_grad_kernel<<<dim3((dim + 31) / 32, 2), kThreads, 0, st>>>(p, blocks);
+        weight_grad_kernel<<<dim3((dim + 31) / 32, 2), kSumThreads, 0, st>>>(p, blocks);
         B2K_RETURN_IF_LAUNCH_FAILED(name);
         b2k::note_launch();
     }
