@@ -50,7 +50,8 @@ def operand(x, what, written=False, stream=0):
             raise ValueError(f"{what} requires grad: the call is not recorded for autograd, pass x.detach()")
         if written:
             raise ValueError(f"{what} must be in device memory")
-        x = x.cuda()
+        with torch.cuda.stream(_torch_stream(stream)):      # its memory goes back in this stream's order
+            x = x.cuda()
         return x.data_ptr(), x.shape, x.stride(), fmt, x.get_device(), x
     if not isinstance(x, DeviceNDArray):
         if written and not is_cuda_array(x):

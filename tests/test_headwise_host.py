@@ -360,6 +360,16 @@ def test_python_refusals_of_the_cache():
             f(k, v, kc, ks, vc, vs, slots)
 
 
+def test_arrays_of_another_device_are_refused(monkeypatch):
+    """The launch goes to the current device: arrays that live elsewhere are an error."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    q = _fake((3, 4, 16), np.float32)                   # "device" -1
+    with pytest.raises(ValueError, match="current device is 0"):
+        headnorm.norm_rotate(q, None, q_out=q)
+    with pytest.raises(ValueError, match="current device is 0"):
+        kvcache.write(q, None, _fake((2, 4, 4, 16), np.uint8), _fake((2, 4, 4, 1), np.float32), None, None, _fake((3,), np.int32))
+
+
 def test_names_are_reachable_from_the_package():
     assert cuda.kernels.headnorm.norm_rotate is headnorm.norm_rotate
     assert cuda.kernels.kvcache.read is kvcache.read

@@ -411,6 +411,23 @@ def test_captured_step_follows_its_inputs():
             assert torch.equal(a, b)
 
 
+def test_host_tensors_on_a_stream_of_their_own():
+    """What a call copies to the device belongs to the call's stream: work that other
+    streams start meanwhile does not get its memory."""
+    rng = np.random.default_rng(0)
+    x = torch.randn(4000, 4, 128)
+    slots = torch.arange(4000)
+    want, got = (pool(250, 16, 4, 128, 128, "e4m3", "f32", rng) for _ in range(2))
+    kvcache.write(x.cuda(), None, *want, None, None, slots.cuda())
+    st = cuda.stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        kvcache.write(x, None, *got, None, None, slots, stream=st)
+        torch.full((4000, 4, 128), 9.0, device="cuda")            # the default stream takes memory at once
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_streams_of_the_package():
     rng = np.random.default_rng(0)
     x = layout((500, 4, 128), "contiguous", "bfloat16", rng)
