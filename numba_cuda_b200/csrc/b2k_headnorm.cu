@@ -385,13 +385,12 @@ __device__ __forceinline__ void gradient_of(const float (&x)[VEC], float (&g)[VE
     }
 }
 
-template <typename T, int VEC, int ITER, int WHICH>
+template <typename T, int VEC, int ITER, int WHICH, bool INTER>
 __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_block, uint32_t blocks, float *block_sums) {
     const Role &r = p.role[WHICH];
     const Lanes g(p.lanes);
     const uint32_t in_block = static_cast<uint32_t>(kThreads) >> p.lane_bits;
-    // In the order of the pairs: w, sums and rows are kept as turn() wants them.
-    const bool swap = p.interleaved;
+    // w, sums and rows are kept in the order of the pairs
     int oa[ITER], ob[ITER];
     float wx[ITER][VEC], wy[ITER][VEC], sum_x[ITER][VEC] = {}, sum_y[ITER][VEC] = {};
 #pragma unroll
@@ -400,7 +399,7 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
         float wa[VEC] = {}, wb[VEC] = {};
         if (oa[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa[i], wa);
         if (ob[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob[i], wb);
-        in_pairs<VEC>(swap, wa, wb, wx[i], wy[i]);
+        in_pairs<VEC, INTER>(wa, wb, wx[i], wy[i]);
     }
     // A warp's groups take neighbouring items and stay together: see Lanes.  all_items < 2^31,
     // and a step is at most the grid's groups, so nothing overflows.
@@ -422,15 +421,20 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
         if (p.positions != nullptr) position = paging::load_index(p.positions, p.position_bytes, token);
         // a padding token's rows are taken as zeros all through, with by = 0 below
         const bool padding = p.positions != nullptr && (position < 0 || position >= p.table_rows);
+        if (padding) {
+            x_now = Batch<T, VEC, ITER, 1>{};
+            g_now = Batch<T, VEC, ITER, 1>{};
+        }
+        const int loads = padding ? 0 : rows;
         float c[ITER][VEC], s[ITER][VEC];
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int u = g.lane + i * g.n;
-            Turned t = turned_of<VEC>(r, swap, u, oa[i], ob[i]);
+            Turned t = turned_of<VEC, INTER>(r, u, oa[i], ob[i]);
             t.lo = t.lo && !padding;
             t.hi = t.hi && !padding;
-            load_angles<VEC>(p.cos_table + position * p.cos_stride, swap, u, oa[i], ob[i], t, c[i]);
-            load_angles<VEC>(p.sin_table + position * p.sin_stride, swap, u, oa[i], ob[i], t, s[i]);
+            load_angles<VEC, INTER>(p.cos_table + position * p.cos_stride, u, oa[i], ob[i], t, c[i]);
+            load_angles<VEC, INTER>(p.sin_table + position * p.sin_stride, u, oa[i], ob[i], t, s[i]);
         }
         const int most = __reduce_max_sync(0xFFFFFFFFu, rows);
 #pragma unroll 1
@@ -439,21 +443,20 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
             Batch<T, VEC, ITER, 1> x_next, g_next;
             in += r.in_head;
             grad += r.grad_head;
-            x_next.load(in, 0, rows - h - 1, oa, ob, r.dim);
-            g_next.load(grad, 0, rows - h - 1, oa, ob, r.dim);
+            x_next.load(in, 0, loads - h - 1, oa, ob, r.dim);
+            g_next.load(grad, 0, loads - h - 1, oa, ob, r.dim);
             float x[ITER][VEC], y[ITER][VEC], gx[ITER][VEC], gy[ITER][VEC];
             float2 ss = make_float2(0.0f, 0.0f), dot = ss;
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
                 float a[VEC], b[VEC];
-                if (padding) x_now.a[0][i] = x_now.b[0][i] = g_now.a[0][i] = g_now.b[0][i] = Chunk<T, VEC>{};
                 widen(x_now.a[0][i], a);
                 widen(x_now.b[0][i], b);
-                in_pairs<VEC>(swap, a, b, x[i], y[i]);
+                in_pairs<VEC, INTER>(a, b, x[i], y[i]);
                 widen(g_now.a[0][i], a);
                 widen(g_now.b[0][i], b);
-                in_pairs<VEC>(swap, a, b, gx[i], gy[i]);
-                const Turned t = turned_of<VEC>(r, swap, g.lane + i * g.n, oa[i], ob[i]);
+                in_pairs<VEC, INTER>(a, b, gx[i], gy[i]);
+                const Turned t = turned_of<VEC, INTER>(r, g.lane + i * g.n, oa[i], ob[i]);
                 if (VEC > 1 && t.lo) turn_back<0, VEC / 2, VEC>(gx[i], gy[i], c[i], s[i]);
                 if (t.hi) turn_back<VEC / 2, VEC, VEC>(gx[i], gy[i], c[i], s[i]);
                 gradient_sums<VEC>(x[i], gx[i], wx[i], ss, dot);
@@ -474,7 +477,7 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
                 float a[VEC], b[VEC];
-                out_of_pairs<VEC>(swap, gx[i], gy[i], a, b);
+                out_of_pairs<VEC, INTER>(gx[i], gy[i], a, b);
                 if (h < rows && oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a);
                 if (h < rows && ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b);
             }
@@ -489,7 +492,7 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         float a[VEC], b[VEC];
-        out_of_pairs<VEC>(swap, sum_x[i], sum_y[i], a, b);
+        out_of_pairs<VEC, INTER>(sum_x[i], sum_y[i], a, b);
         for (int o = g.n; o < 32; o *= 2)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
@@ -518,8 +521,14 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
 template <typename T, int VEC, int ITER>
 __global__ void __launch_bounds__(kThreads, ITER == 1 ? 4 : 1) heads_backward_kernel(const __grid_constant__ Params p) {
     extern __shared__ float block_sums[];             // one row of dim floats per warp
-    if (static_cast<int>(blockIdx.x) < p.blocks0) backward_role<T, VEC, ITER, 0>(p, blockIdx.x, p.blocks0, block_sums);
-    else backward_role<T, VEC, ITER, 1>(p, blockIdx.x - p.blocks0, gridDim.x - p.blocks0, block_sums);
+    const uint32_t blocks0 = p.blocks0, blocks1 = gridDim.x - blocks0;
+    if (VEC > 1 && p.interleaved) {
+        if (blockIdx.x < blocks0) backward_role<T, VEC, ITER, 0, true>(p, blockIdx.x, blocks0, block_sums);
+        else backward_role<T, VEC, ITER, 1, true>(p, blockIdx.x - blocks0, blocks1, block_sums);
+    } else {
+        if (blockIdx.x < blocks0) backward_role<T, VEC, ITER, 0, false>(p, blockIdx.x, blocks0, block_sums);
+        else backward_role<T, VEC, ITER, 1, false>(p, blockIdx.x - blocks0, blocks1, block_sums);
+    }
 }
 
 // weight_grad[d] = sum over the role's blocks of partials[block][d], 32 columns a block: 32

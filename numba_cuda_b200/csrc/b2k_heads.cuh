@@ -266,10 +266,10 @@ __device__ __forceinline__ void unpair(const float (&x)[VEC], const float (&y)[V
     }
 }
 
-template <int VEC>
-__device__ __forceinline__ void in_pairs(bool interleaved, const float (&a)[VEC], const float (&b)[VEC], float (&x)[VEC],
-                                         float (&y)[VEC]) {
-    if (interleaved) {
+// INTER is a constant because a choice at run time costs a move per item.
+template <int VEC, bool INTER>
+__device__ __forceinline__ void in_pairs(const float (&a)[VEC], const float (&b)[VEC], float (&x)[VEC], float (&y)[VEC]) {
+    if constexpr (INTER) {
         pair<VEC>(a, b, x, y);
     } else {
 #pragma unroll
@@ -279,10 +279,9 @@ __device__ __forceinline__ void in_pairs(bool interleaved, const float (&a)[VEC]
         }
     }
 }
-template <int VEC>
-__device__ __forceinline__ void out_of_pairs(bool interleaved, const float (&x)[VEC], const float (&y)[VEC], float (&a)[VEC],
-                                             float (&b)[VEC]) {
-    if (interleaved) {
+template <int VEC, bool INTER>
+__device__ __forceinline__ void out_of_pairs(const float (&x)[VEC], const float (&y)[VEC], float (&a)[VEC], float (&b)[VEC]) {
+    if constexpr (INTER) {
         unpair<VEC>(x, y, a, b);
     } else {
 #pragma unroll
@@ -298,23 +297,22 @@ __device__ __forceinline__ void out_of_pairs(bool interleaved, const float (&x)[
 struct Turned {
     bool lo, hi;
 };
-template <int VEC>
-__device__ __forceinline__ Turned turned_of(const Role &r, bool interleaved, int u, int oa, int ob) {
-    if (VEC > 1 && interleaved) return Turned{oa < r.angle_items, ob < r.angle_items};
+template <int VEC, bool INTER>
+__device__ __forceinline__ Turned turned_of(const Role &r, int u, int oa, int ob) {
+    if (VEC > 1 && INTER) return Turned{oa < r.angle_items, ob < r.angle_items};
     return Turned{u < r.angle_units, u < r.angle_units};
 }
 
 // A unit's cosines or sines, from its position's row of the table; zeros where nothing is rotated.
-template <int VEC>
-__device__ __forceinline__ void load_angles(const float *row, bool interleaved, int u, int oa, int ob, Turned t,
-                                            float (&v)[VEC]) {
+template <int VEC, bool INTER>
+__device__ __forceinline__ void load_angles(const float *row, int u, int oa, int ob, Turned t, float (&v)[VEC]) {
     if constexpr (VEC == 1) {
         v[0] = t.lo ? row[u] : 0.0f;
     } else {
         constexpr int H = VEC / 2;
         float lo[H] = {}, hi[H] = {};
-        if (t.lo) load_floats<H>(row + (interleaved ? oa / 2 : u * VEC), lo);
-        if (t.hi) load_floats<H>(row + (interleaved ? ob / 2 : u * VEC + H), hi);
+        if (t.lo) load_floats<H>(row + (INTER ? oa / 2 : u * VEC), lo);
+        if (t.hi) load_floats<H>(row + (INTER ? ob / 2 : u * VEC + H), hi);
 #pragma unroll
         for (int j = 0; j < H; ++j) {
             v[j] = lo[j];

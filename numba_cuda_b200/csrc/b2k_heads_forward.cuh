@@ -86,7 +86,7 @@ struct Factors {
 // One role's share of the launch.  WHICH is a constant so that every member of the role is
 // an operand in constant memory: indexed by a variable, each use is a load of its own,
 // and those were a quarter of all instructions.
-template <typename T, int VEC, int ITER, int MODE, int WHICH>
+template <typename T, int VEC, int ITER, int MODE, int WHICH, bool INTER>
 __device__ __forceinline__ void forward_role(const Params &p, uint32_t block, unsigned *group_max) {
     // groups of a scale are at least 16 items, so a lane's share of a row has at most this many
     constexpr int kGroupsPerLane = (2 * VEC * ITER + 15) / 16;
@@ -135,16 +135,16 @@ __device__ __forceinline__ void forward_role(const Params &p, uint32_t block, un
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int u = g.lane + i * g.n;
-            const Turned t = turned_of<VEC>(r, p.interleaved, u, oa[i], ob[i]);
+            const Turned t = turned_of<VEC, INTER>(r, u, oa[i], ob[i]);
             float wa[VEC], wb[VEC], wx[VEC], wy[VEC], c[VEC], s[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) wa[j] = wb[j] = 1.0f;
             if (normed && oa[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa[i], wa);
             if (normed && ob[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob[i], wb);
-            in_pairs<VEC>(p.interleaved, wa, wb, wx, wy);
+            in_pairs<VEC, INTER>(wa, wb, wx, wy);
             const Turned load{t.lo && active, t.hi && active};
-            load_angles<VEC>(p.cos_table + position * p.cos_stride, p.interleaved, u, oa[i], ob[i], load, c);
-            load_angles<VEC>(p.sin_table + position * p.sin_stride, p.interleaved, u, oa[i], ob[i], load, s);
+            load_angles<VEC, INTER>(p.cos_table + position * p.cos_stride, u, oa[i], ob[i], load, c);
+            load_angles<VEC, INTER>(p.sin_table + position * p.sin_stride, u, oa[i], ob[i], load, s);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 const bool turned = j < VEC / 2 ? t.lo : t.hi;
@@ -183,12 +183,12 @@ __device__ __forceinline__ void forward_role(const Params &p, uint32_t block, un
                 }
 #pragma unroll
                 for (int i = 0; i < ITER; ++i) {
-                    const Turned t = turned_of<VEC>(r, p.interleaved, g.lane + i * g.n, oa[i], ob[i]);
+                    const Turned t = turned_of<VEC, INTER>(r, g.lane + i * g.n, oa[i], ob[i]);
                     float x[VEC], y[VEC];
-                    in_pairs<VEC>(p.interleaved, a[i], b[i], x, y);
+                    in_pairs<VEC, INTER>(a[i], b[i], x, y);
                     if (VEC > 1) turn<0, VEC / 2, VEC>(x, y, k.k0[i], k.k1[i], k.k2[i], k.k3[i], by, t.lo);
                     turn<VEC / 2, VEC, VEC>(x, y, k.k0[i], k.k1[i], k.k2[i], k.k3[i], by, t.hi);
-                    out_of_pairs<VEC>(p.interleaved, x, y, a[i], b[i]);
+                    out_of_pairs<VEC, INTER>(x, y, a[i], b[i]);
                 }
             }
             if constexpr (quantised) {
@@ -209,19 +209,27 @@ __device__ __forceinline__ void forward_role(const Params &p, uint32_t block, un
     }
 }
 
+template <typename T, int VEC, int ITER, int MODE, bool INTER>
+__device__ __forceinline__ void forward_roles(const Params &p, unsigned *group_max) {
+    uint32_t block = blockIdx.x;
+    if constexpr ((MODE & kRotate) != 0) {                 // a cache write has no queries
+        if (block < p.role[0].blocks) return forward_role<T, VEC, ITER, MODE, 0, INTER>(p, block, group_max);
+        block -= p.role[0].blocks;
+    }
+    if (MODE == kRotate || block < p.role[1].blocks) return forward_role<T, VEC, ITER, MODE, 1, INTER>(p, block, group_max);
+    if constexpr (MODE != kRotate) forward_role<T, VEC, ITER, MODE, 2, INTER>(p, block - p.role[1].blocks, group_max);
+}
+
 // Five blocks an SM where a row takes one unit a lane (102 registers): left alone the
 // compiler takes a few more and four fit (rotation of 16384 tokens x 40 heads of 128 bf16
 // items 66.5 us instead of 63.6 us).
 template <typename T, int VEC, int ITER, int MODE>
 __global__ void __launch_bounds__(kThreads, ITER == 1 ? 5 : 1) heads_forward_kernel(const __grid_constant__ Params p) {
     __shared__ unsigned group_max[MODE == kRotate ? 1 : kThreads * ((2 * VEC * ITER + 15) / 16)];
-    uint32_t block = blockIdx.x;
-    if constexpr ((MODE & kRotate) != 0) {                 // a cache write has no queries
-        if (block < p.role[0].blocks) return forward_role<T, VEC, ITER, MODE, 0>(p, block, group_max);
-        block -= p.role[0].blocks;
+    if constexpr ((MODE & kRotate) != 0 && VEC > 1) {
+        if (p.interleaved) return forward_roles<T, VEC, ITER, MODE, true>(p, group_max);
     }
-    if (MODE == kRotate || block < p.role[1].blocks) return forward_role<T, VEC, ITER, MODE, 1>(p, block, group_max);
-    if constexpr (MODE != kRotate) forward_role<T, VEC, ITER, MODE, 2>(p, block - p.role[1].blocks, group_max);
+    forward_roles<T, VEC, ITER, MODE, false>(p, group_max);
 }
 
 // ---- launch --------------------------------------------------------------------------
