@@ -10,13 +10,58 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <initializer_list>
+
 #include "../../include/b2k.h"
 
 namespace {
 
 // Set once by setup().
-PyObject *g_tensor_type, *g_formats, *g_stream_ptr, *g_workspace;
-PyObject *s_dtype, *s_shape, *s_stride, *s_data_ptr, *s_get_device, *s_requires_grad;
+PyObject *g_tensor_type, *g_formats, *g_stream_ptr, *g_workspace, *g_no_arguments;
+
+// An attribute or a method without arguments of the tensor type.  Where it is implemented
+// in C, its function is called directly: looking six of them up for each of ten tensors
+// was a fifth of a call's host time.
+struct Member {
+    const char *name;
+    PyObject *key = nullptr;
+    bool called = false;                  // a method
+    getter get = nullptr;
+    void *closure = nullptr;
+    PyCFunction plain = nullptr;          // METH_NOARGS
+    PyCFunctionWithKeywords keyed = nullptr;
+
+    bool find(PyObject *type) {
+        Py_XSETREF(key, PyUnicode_InternFromString(name));
+        PyObject *d = key ? PyObject_GetAttr(type, key) : nullptr;       // held for good: the pointers live in it
+        if (d == nullptr) return false;
+        get = nullptr;
+        plain = nullptr;
+        keyed = nullptr;
+        called = !Py_IS_TYPE(d, &PyGetSetDescr_Type) && PyCallable_Check(d);
+        if (Py_IS_TYPE(d, &PyGetSetDescr_Type)) {
+            const PyGetSetDef *def = reinterpret_cast<PyGetSetDescrObject *>(d)->d_getset;
+            get = def->get;
+            closure = def->closure;
+        } else if (Py_IS_TYPE(d, &PyMethodDescr_Type)) {
+            const PyMethodDef *def = reinterpret_cast<PyMethodDescrObject *>(d)->d_method;
+            if (def->ml_flags == METH_NOARGS) plain = def->ml_meth;
+            else if (def->ml_flags == (METH_VARARGS | METH_KEYWORDS))
+                keyed = reinterpret_cast<PyCFunctionWithKeywords>(reinterpret_cast<void (*)()>(def->ml_meth));
+        }
+        return true;
+    }
+    PyObject *operator()(PyObject *o) const {
+        if (get) return get(o, closure);
+        if (plain) return plain(o, nullptr);
+        if (keyed) return keyed(o, g_no_arguments, nullptr);
+        if (!called) return PyObject_GetAttr(o, key);
+        PyObject *args[1] = {o};
+        return PyObject_VectorcallMethod(key, args, 1 | PY_VECTORCALL_ARGUMENTS_OFFSET, nullptr);
+    }
+};
+Member m_dtype{"dtype"}, m_shape{"shape"}, m_stride{"stride"}, m_data_ptr{"data_ptr"}, m_get_device{"get_device"},
+    m_requires_grad{"requires_grad"};
 
 struct Entry {
     decltype(&b2k_norm_rotate) norm_rotate;
@@ -41,11 +86,6 @@ bool as_integer(PyObject *o, long long &v) {            // takes the reference
     return !(v == -1 && PyErr_Occurred());
 }
 
-bool method_integer(PyObject *o, PyObject *name, long long &v) {
-    PyObject *args[1] = {o};
-    return as_integer(PyObject_VectorcallMethod(name, args, 1 | PY_VECTORCALL_ARGUMENTS_OFFSET, nullptr), v);
-}
-
 bool integers(PyObject *tuple, long long *out, int &n) {  // takes the reference
     if (tuple == nullptr) return false;
     bool ok = PyTuple_Check(tuple) && PyTuple_GET_SIZE(tuple) <= 4;
@@ -64,28 +104,25 @@ bool integers(PyObject *tuple, long long *out, int &n) {  // takes the reference
 // Python error behind; the entry points clear it.
 bool read(PyObject *o, int device, Array &a) {
     if (reinterpret_cast<PyObject *>(Py_TYPE(o)) != g_tensor_type) return false;
-    PyObject *dtype = PyObject_GetAttr(o, s_dtype);
+    PyObject *dtype = m_dtype(o);
     if (dtype == nullptr) return false;
     PyObject *format = PyDict_GetItemWithError(g_formats, dtype);      // borrowed
     Py_DECREF(dtype);
     if (format == nullptr) return false;
     a.format = static_cast<int>(PyLong_AsLong(format));
-    PyObject *grad = PyObject_GetAttr(o, s_requires_grad);
+    PyObject *grad = m_requires_grad(o);
     if (grad == nullptr) return false;
     const bool plain = grad == Py_False;
     Py_DECREF(grad);
     if (!plain) return false;
     long long v;
-    if (!method_integer(o, s_get_device, v) || v != device) return false;
+    if (!as_integer(m_get_device(o), v) || v != device) return false;
     a.device = device;
-    if (!method_integer(o, s_data_ptr, v)) return false;
+    if (!as_integer(m_data_ptr(o), v)) return false;
     a.data = reinterpret_cast<void *>(v);
     int strides = 0;
-    if (!integers(PyObject_GetAttr(o, s_shape), a.size, a.ndim)) return false;
-    PyObject *args[1] = {o};
-    if (!integers(PyObject_VectorcallMethod(s_stride, args, 1 | PY_VECTORCALL_ARGUMENTS_OFFSET, nullptr), a.stride, strides))
-        return false;
-    return strides == a.ndim;
+    if (!integers(m_shape(o), a.size, a.ndim)) return false;
+    return integers(m_stride(o), a.stride, strides) && strides == a.ndim;
 }
 
 bool is_float(int format) { return format == B2K_FMT_F32 || format == B2K_FMT_F16 || format == B2K_FMT_BF16; }
@@ -270,7 +307,7 @@ PyObject *norm_rotate_backward(PyObject *, PyObject *const *args, Py_ssize_t n) 
     }
     PyObject *held = nullptr;
     void *scratch = nullptr;
-    long long bytes = 0, at;
+    long long bytes = 0;
     if (sums[0] || sums[1]) {
         bytes = g_call.scratch_bytes(&t.r);
         PyObject *size = PyLong_FromLongLong(bytes);
@@ -279,11 +316,13 @@ PyObject *norm_rotate_backward(PyObject *, PyObject *const *args, Py_ssize_t n) 
         held = PyObject_Vectorcall(g_workspace, two, 2, nullptr);
         Py_DECREF(size);
         if (held == nullptr) return nullptr;                            // out of memory, say
-        if (!method_integer(held, s_data_ptr, at)) {
+        Array scratch_of;
+        if (!read(held, device, scratch_of)) {
+            if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "no workspace tensor");
             Py_DECREF(held);
             return nullptr;
         }
-        scratch = reinterpret_cast<void *>(at);
+        scratch = scratch_of.data;
     }
     const int status =
         g_call.norm_rotate_backward(&t.r, &q_grad, &k_grad, &dq, &dk, sums[0], sums[1], scratch, bytes, stream);
@@ -377,6 +416,8 @@ PyObject *setup(PyObject *, PyObject *args) {
         !address(addresses, "b2k_norm_rotate_write", e.norm_rotate_write) ||
         !address(addresses, "b2k_current_device", e.current_device))
         return nullptr;
+    for (Member *m : {&m_dtype, &m_shape, &m_stride, &m_data_ptr, &m_get_device, &m_requires_grad})
+        if (!m->find(type)) return nullptr;
     g_call = e;
     Py_INCREF(formats);
     Py_XSETREF(g_formats, formats);
@@ -404,12 +445,7 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_pyfast", nullptr, -1, g_methods
 }  // namespace
 
 PyMODINIT_FUNC PyInit__pyfast(void) {
-    s_dtype = PyUnicode_InternFromString("dtype");
-    s_shape = PyUnicode_InternFromString("shape");
-    s_stride = PyUnicode_InternFromString("stride");
-    s_data_ptr = PyUnicode_InternFromString("data_ptr");
-    s_get_device = PyUnicode_InternFromString("get_device");
-    s_requires_grad = PyUnicode_InternFromString("requires_grad");
-    if (!s_dtype || !s_shape || !s_stride || !s_data_ptr || !s_get_device || !s_requires_grad) return nullptr;
+    g_no_arguments = PyTuple_New(0);
+    if (g_no_arguments == nullptr) return nullptr;
     return PyModule_Create(&g_module);
 }

@@ -124,10 +124,16 @@ def like(op, stream):
     return device_array(op[1], dtype, stream=stream)
 
 
+def _current_stream_ptr() -> int:
+    """cudaStream_t of torch's current stream; the object for it would cost 3 us."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(torch.cuda.current_device()) if raw is not None else torch.cuda.current_stream().cuda_stream
+
+
 def workspace(nbytes, stream):
     """Device memory for one call, from torch's allocator on the call's stream: calls on
     other streams and replays of captured graphs have their own."""
-    if torch.cuda.current_stream().cuda_stream == stream_ptr(stream):
+    if _current_stream_ptr() == stream_ptr(stream):
         return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
     with torch.cuda.stream(_torch_stream(stream)):
         return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
