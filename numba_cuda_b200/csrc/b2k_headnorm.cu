@@ -10,6 +10,8 @@
 // HBM bounds them (2 and 3 items moved per item of the rows).  The reference's users
 // would write this as a last-axis reduction of their own; its library reduce stops at
 // one axis (numba/cuda/kernels/reduction.py:217-218).
+#include <algorithm>
+
 #include "b2k_heads_forward.cuh"
 
 namespace headwise {
@@ -224,47 +226,63 @@ static bool role_fits(const Params &p, const Role &r, bool rotated, int rotary, 
     if (r.codes && (!fits(r.codes, r.code_page, r.code_slot, 1, vec) || r.code_head % vec || r.group % vec)) return false;
     if (rotated) {
         if (rotary % (p.interleaved ? vec : 2 * vec)) return false;
-        const int w = vec < 4 ? vec : 4;
+        const int w = vec / 2;                 // a chunk's pairs, or half a chunk of one table row
         if (!fits(p.cos_table, p.cos_stride, 0, 4, w) || !fits(p.sin_table, p.sin_stride, 0, 4, w)) return false;
     }
     return true;
 }
 
-Plan choose(Params &p, int64_t format, const b2k_rotation *rot) {
-    const int itemsize = item_bytes(format);
-    const int rotary = rot ? static_cast<int>(rot->rotary_dim) : 0;
-    Plan plan;
-    for (int vec : {8, 4, 1}) {
-        if (vec * itemsize > 16) continue;
-        bool ok = true;
-        for (int i = 0; i < 3; ++i)
-            if (p.role[i].heads) ok = ok && role_fits(p, p.role[i], i < 2 && rotary, rotary, itemsize, vec);
-        if (ok) {
-            plan.vec = vec;
-            break;
-        }
+// How chunks of `vec` items pair up in a role's rows; `turned` items are rotated.
+static void pair_up(Role &r, int vec, int turned, bool interleaved) {
+    // The halves of a rotated run pair up, and what lies behind it lies in pairs of
+    // neighbouring chunks.  Without a rotation of halves the two halves of the row pair
+    // up; single interleaved items (vec == 1) pair with their neighbours.
+    if (turned && !interleaved) {
+        r.pair_gap = turned / 2;
+        r.tail = turned;
+    } else if (turned && vec == 1) {
+        r.pair_gap = r.tail = 0;
+    } else {
+        r.pair_gap = (r.dim / vec + 1) / 2 * vec;
+        r.tail = r.dim;
     }
+    r.pair_units = r.pair_gap / vec;
+    r.angle_units = turned / 2 / vec;
+    r.angle_items = turned;
+    r.units = r.pair_units + (r.dim - r.tail + 2 * vec - 1) / (2 * vec);
+}
+
+// Units a lane holds in the smallest compiled shape for chunks of `vec` items; 0 if none
+// takes so many.
+static int units_a_lane(int vec, int units, int lanes) {
+    const int need = (units + lanes - 1) / lanes;
+#define B2K_HEADS_PICK(V, I) \
+    if (vec == V && I >= need) return I;
+    B2K_HEADS_SHAPES(B2K_HEADS_PICK)
+#undef B2K_HEADS_PICK
+    return 0;
+}
+
+int widest(const Params &p, int which, int64_t format, const b2k_rotation *rot) {
+    const int itemsize = item_bytes(format);
+    const int rotary = rot && which < 2 ? static_cast<int>(rot->rotary_dim) : 0;
+    for (int vec : {8, 4, 2}) {
+        if (vec * itemsize > 16 || !role_fits(p, p.role[which], rotary > 0, rotary, itemsize, vec)) continue;
+        Role r = p.role[which];
+        pair_up(r, vec, rotary, p.interleaved);
+        if (units_a_lane(vec, r.units, 32)) return vec;
+    }
+    return 1;
+}
+
+Plan lay_out(Params &p, int vec, const b2k_rotation *rot) {
+    Plan plan;
+    plan.vec = vec;
     int units = 1;
     for (int i = 0; i < 3; ++i) {
         Role &r = p.role[i];
         if (r.heads == 0) continue;
-        const int turned = i < 2 ? rotary : 0, vec = plan.vec;
-        // The halves of a rotated run pair up, and what lies behind it lies in pairs of
-        // neighbouring chunks.  Without a rotation of halves the two halves of the row pair
-        // up; single interleaved items (vec == 1) pair with their neighbours.
-        if (turned && !p.interleaved) {
-            r.pair_gap = turned / 2;
-            r.tail = turned;
-        } else if (turned && vec == 1) {
-            r.pair_gap = r.tail = 0;
-        } else {
-            r.pair_gap = (r.dim / vec + 1) / 2 * vec;
-            r.tail = r.dim;
-        }
-        r.pair_units = r.pair_gap / vec;
-        r.angle_units = turned / 2 / vec;
-        r.angle_items = turned;
-        r.units = r.pair_units + (r.dim - r.tail + 2 * vec - 1) / (2 * vec);
+        pair_up(r, vec, rot && i < 2 ? static_cast<int>(rot->rotary_dim) : 0, p.interleaved);
         if (r.units > units) units = r.units;
     }
     p.lanes = 1;
@@ -273,11 +291,9 @@ Plan choose(Params &p, int64_t format, const b2k_rotation *rot) {
         p.lanes *= 2;
         p.lane_bits += 1;
     }
-    const int need = (units + p.lanes - 1) / p.lanes;
-#define B2K_HEADS_PICK(V, I) \
-    if (plan.vec == V && plan.iter == 0 && I >= need) plan.iter = I;
-    B2K_HEADS_SHAPES(B2K_HEADS_PICK)
-#undef B2K_HEADS_PICK
+    plan.iter = units_a_lane(vec, units, p.lanes);
+    // another role's narrow chunks may be too many for a long row: narrower ones have a shape
+    if (plan.iter == 0 && vec > 1) return lay_out(p, vec / 2, rot);
     for (Role &r : p.role) {
         if (r.codes == nullptr) continue;
         r.groups_of = paging::divisor(static_cast<uint32_t>(r.group));
@@ -327,10 +343,10 @@ constexpr int kBackwardHeadsPerItem = 8;
 // The inverse rotation of a unit's pairs.
 template <int FROM, int TO, int VEC>
 __device__ __forceinline__ void turn_back(float (&x)[VEC], float (&y)[VEC], const float (&c)[VEC], const float (&s)[VEC]) {
-    if constexpr (VEC == 1) {
-        const float u = x[0] * c[0] + y[0] * s[0], v = y[0] * c[0] - x[0] * s[0];
-        x[0] = u;
-        y[0] = v;
+    if constexpr (TO - FROM == 1) {
+        const float u = x[FROM] * c[FROM] + y[FROM] * s[FROM], v = y[FROM] * c[FROM] - x[FROM] * s[FROM];
+        x[FROM] = u;
+        y[FROM] = v;
     } else {
 #pragma unroll
         for (int j = FROM; j < TO; j += 2) {
@@ -626,8 +642,7 @@ int b2k_norm_rotate(const b2k_rotation *r, const b2k_heads *q_out, const b2k_hea
     if (r->tokens == 0) return B2K_OK;
     p.tokens = r->tokens;
     set_rotation(p, *r);
-    const Plan plan = choose(p, r->format, r);
-    return launch_forward<kRotate>(p, r->format, plan, b2k::as_stream(stream), name);
+    return launch_forward<kRotate>(p, r->format, r, b2k::as_stream(stream), name);
 }
 
 int64_t b2k_norm_rotate_backward_scratch_bytes(const b2k_rotation *r) {
@@ -675,7 +690,11 @@ int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, con
     p.tokens = r->tokens;
     p.partials = static_cast<float *>(scratch_dev);
     set_rotation(p, *r);
-    const Plan plan = choose(p, r->format, r);
+    int vec = 8;
+    for (int i = 0; i < 2; ++i)
+        if (p.role[i].heads) vec = std::min(vec, widest(p, i, r->format, r));
+    const Plan plan = lay_out(p, vec, r);
+    if (plan.iter == 0) return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: no kernel for this head size", name);
     if (int rc = count_items(p, kBackwardHeadsPerItem, kThreads, name)) return rc;
     // blocks go to the two roles by their share of the rows' items, at least one to each
     const cudaStream_t st = b2k::as_stream(stream);

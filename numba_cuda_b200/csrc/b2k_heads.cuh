@@ -328,11 +328,11 @@ __device__ __forceinline__ void load_angles(const float *row, int u, int oa, int
 template <int FROM, int TO, int VEC>
 __device__ __forceinline__ void turn(float (&x)[VEC], float (&y)[VEC], const float (&k0)[VEC], const float (&k1)[VEC],
                                      const float (&k2)[VEC], const float (&k3)[VEC], float scale, bool turned) {
-    if constexpr (VEC == 1) {
-        const float u = turned ? x[0] * k0[0] - y[0] * k1[0] : x[0] * k0[0];
-        const float v = turned ? y[0] * k2[0] + x[0] * k3[0] : y[0] * k2[0];
-        x[0] = u * scale;
-        y[0] = v * scale;
+    if constexpr (TO - FROM == 1) {
+        const float u = turned ? x[FROM] * k0[FROM] - y[FROM] * k1[FROM] : x[FROM] * k0[FROM];
+        const float v = turned ? y[FROM] * k2[FROM] + x[FROM] * k3[FROM] : y[FROM] * k2[FROM];
+        x[FROM] = u * scale;
+        y[FROM] = v * scale;
     } else {
         const float2 by = make_float2(scale, scale);
 #pragma unroll
@@ -384,12 +384,17 @@ __device__ __forceinline__ void store_codes(uint8_t *p, const float (&v)[VEC], f
         *p = static_cast<uint8_t>(pack_codes2(0.0f, v[0] * by, e5m2));
     } else {
         Chunk<uint8_t, VEC> c;
+        const float2 by2 = make_float2(by, by);
+        if constexpr (VEC == 2) {
+            const float2 x = mul2(make_float2(v[0], v[1]), by2);
+            c.all = static_cast<uint16_t>(pack_codes2(x.y, x.x, e5m2));
+        } else {
 #pragma unroll
-        for (int j = 0; j < VEC / 4; ++j) {
-            const float2 by2 = make_float2(by, by);
-            const float2 x = mul2(make_float2(v[4 * j], v[4 * j + 1]), by2);
-            const float2 y = mul2(make_float2(v[4 * j + 2], v[4 * j + 3]), by2);
-            c.word[j] = pack_codes2(x.y, x.x, e5m2) | (pack_codes2(y.y, y.x, e5m2) << 16);
+            for (int j = 0; j < VEC / 4; ++j) {
+                const float2 x = mul2(make_float2(v[4 * j], v[4 * j + 1]), by2);
+                const float2 y = mul2(make_float2(v[4 * j + 2], v[4 * j + 3]), by2);
+                c.word[j] = pack_codes2(x.y, x.x, e5m2) | (pack_codes2(y.y, y.x, e5m2) << 16);
+            }
         }
         *reinterpret_cast<typename Chunk<uint8_t, VEC>::Word *>(p) = c.all;
     }
@@ -447,7 +452,8 @@ struct Scale {
 // ---- host side ----------------------------------------------------------------------
 // The (items per chunk, units per lane) pairs that are compiled; choose() picks one.
 // Chunks of 8 are for 16-bit items only (16 bytes).
-#define B2K_HEADS_SHAPES(CASE) CASE(8, 1) CASE(8, 2) CASE(4, 1) CASE(4, 4) CASE(1, 1) CASE(1, 4) CASE(1, 16)
+#define B2K_HEADS_SHAPES(CASE) \
+    CASE(8, 1) CASE(8, 2) CASE(4, 1) CASE(4, 4) CASE(2, 1) CASE(2, 4) CASE(1, 1) CASE(1, 4) CASE(1, 16)
 
 struct Plan {
     int vec = 0, iter = 0;
@@ -469,8 +475,10 @@ void set_output(Role &r, const b2k_heads &h, int64_t tokens);
 void set_grad(Role &r, const b2k_heads &h, int64_t tokens);
 void set_pages(Params &p, Role &r, const b2k_cache &c, const b2k_pages &side);
 void set_rotation(Params &p, const b2k_rotation &rot);
-// Chunk width from sizes, strides and addresses; lanes and unit layout of every role.
-Plan choose(Params &p, int64_t format, const b2k_rotation *rot);
+// Widest chunks that a role's sizes, strides and addresses allow.
+int widest(const Params &p, int which, int64_t format, const b2k_rotation *rot);
+// Lanes and unit layout of every role for chunks of `vec` items, or fewer.
+Plan lay_out(Params &p, int vec, const b2k_rotation *rot);
 // Items with up to `most` heads in each, and blocks of `threads` threads, of every role; an
 // error when they do not fit 31 bits.
 int count_items(Params &p, int most, int threads, const char *name);

@@ -244,17 +244,44 @@ void pick_forward(const Params &p, const Plan &plan, unsigned blocks, cudaStream
 #undef B2K_HEADS_CASE
 }
 
+// Roles whose sizes or strides allow different chunks get launches of their own when they
+// hold at least this many items together: a launch costs some 2.5 us of the host, single
+// items instead of chunks of 8 about 3 us for 2^20 items.
+constexpr int64_t kItemsToSplit = int64_t(1) << 20;
+
 // Launches over all items; the roles, tokens and tables of `p` are set.
 template <int MODE>
-int launch_forward(Params &p, int64_t format, const Plan &plan, cudaStream_t stream, const char *name) {
-    if (int rc = count_items(p, kHeadsPerItem, kThreads, name)) return rc;
-    const unsigned blocks = p.role[0].blocks + p.role[1].blocks + p.role[2].blocks;
-    if (blocks == 0) return B2K_OK;
-    if (format == B2K_FMT_F32) pick_forward<float, MODE>(p, plan, blocks, stream);
-    else if (format == B2K_FMT_F16) pick_forward<__half, MODE>(p, plan, blocks, stream);
-    else pick_forward<__nv_bfloat16, MODE>(p, plan, blocks, stream);
-    B2K_RETURN_IF_LAUNCH_FAILED(name);
-    b2k::note_launch();
+int launch_forward(const Params &all, int64_t format, const b2k_rotation *rot, cudaStream_t stream, const char *name) {
+    int vec[3] = {}, least = 8, most = 0;
+    double items = 0;
+    for (int i = 0; i < 3; ++i) {
+        const Role &r = all.role[i];
+        if (r.heads == 0) continue;
+        vec[i] = widest(all, i, format, rot);
+        if (vec[i] < least) least = vec[i];
+        if (vec[i] > most) most = vec[i];
+        items += static_cast<double>(all.tokens) * r.heads * r.dim;
+    }
+    const bool split = least != most && items >= kItemsToSplit;
+    for (int width : {8, 4, 2, 1}) {
+        Params p = all;
+        bool any = false;
+        for (int i = 0; i < 3; ++i) {
+            const bool here = vec[i] && (split ? vec[i] == width : width == least);
+            if (!here) p.role[i].heads = 0;
+            any = any || here;
+        }
+        if (!any) continue;
+        const Plan plan = lay_out(p, width, rot);
+        if (plan.iter == 0) return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: no kernel for this head size", name);
+        if (int rc = count_items(p, kHeadsPerItem, kThreads, name)) return rc;
+        const unsigned blocks = p.role[0].blocks + p.role[1].blocks + p.role[2].blocks;
+        if (format == B2K_FMT_F32) pick_forward<float, MODE>(p, plan, blocks, stream);
+        else if (format == B2K_FMT_F16) pick_forward<__half, MODE>(p, plan, blocks, stream);
+        else pick_forward<__nv_bfloat16, MODE>(p, plan, blocks, stream);
+        B2K_RETURN_IF_LAUNCH_FAILED(name);
+        b2k::note_launch();
+    }
     return B2K_OK;
 }
 

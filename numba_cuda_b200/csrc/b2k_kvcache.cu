@@ -96,7 +96,6 @@ __device__ __forceinline__ void store_items(T *p, const float (&v)[N]) {
 template <typename T, int CV, int E5M2>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ ReadParams p) {
     const ReadSide &s = p.side[blockIdx.y];
-    if (s.heads == 0) return;
     __shared__ int64_t code_at[kTileRows], scale_at[kTileRows];
     __shared__ int state[kTileRows];               // 0: no row of a sequence, 1: zeros, 2: codes
     const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tile;
@@ -173,23 +172,23 @@ void launch_read(const ReadParams &p, dim3 grid, cudaStream_t stream) {
     else cache_read_kernel<T, CV, 0><<<grid, kThreads, 0, stream>>>(p);
 }
 
-// Widest chunk that sizes, strides and addresses of both sides allow: 32 bytes of output
-// at most.
+// Widest chunk that a side's sizes, strides and addresses allow: 32 bytes of output at most.
+int widest_read(const ReadSide &s, int itemsize) {
+    for (int cv : {16, 8, 4}) {
+        if (cv * itemsize > 32 || s.dim % cv || s.group % cv) continue;
+        if ((reinterpret_cast<uintptr_t>(s.codes) | s.code_page | s.code_slot | s.code_head) % cv) continue;
+        if (reinterpret_cast<uintptr_t>(s.out) % (cv * itemsize) || (s.out_token | s.out_head) % cv) continue;
+        return cv;
+    }
+    return 1;
+}
+
 template <typename T>
-void pick_read(const ReadParams &p, dim3 grid, cudaStream_t stream) {
-    const auto fits = [&](int cv) {
-        for (const ReadSide &s : p.side) {
-            if (s.heads == 0) continue;
-            if (s.dim % cv || s.group % cv) return false;
-            if ((reinterpret_cast<uintptr_t>(s.codes) | s.code_page | s.code_slot | s.code_head) % cv) return false;
-            if (reinterpret_cast<uintptr_t>(s.out) % (cv * sizeof(T)) || (s.out_token | s.out_head) % cv) return false;
-        }
-        return true;
-    };
+void pick_read(const ReadParams &p, int cv, dim3 grid, cudaStream_t stream) {
     if constexpr (sizeof(T) == 2)
-        if (fits(16)) return launch_read<T, 16>(p, grid, stream);
-    if (fits(8)) return launch_read<T, 8>(p, grid, stream);
-    if (fits(4)) return launch_read<T, 4>(p, grid, stream);
+        if (cv == 16) return launch_read<T, 16>(p, grid, stream);
+    if (cv == 8) return launch_read<T, 8>(p, grid, stream);
+    if (cv == 4) return launch_read<T, 4>(p, grid, stream);
     launch_read<T, 1>(p, grid, stream);
 }
 
@@ -224,8 +223,7 @@ int b2k_cache_write(const b2k_cache *cache, int format, int64_t tokens, const b2
     p.tokens = tokens;
     p.slots = slots_dev;
     p.slot_bytes = slot_bytes;
-    const Plan plan = choose(p, format, nullptr);
-    return launch_forward<kWrite>(p, format, plan, b2k::as_stream(stream), name);
+    return launch_forward<kWrite>(p, format, nullptr, b2k::as_stream(stream), name);
 }
 
 int b2k_norm_rotate_write(const b2k_rotation *r, const b2k_heads *v, const b2k_heads *q_out, const b2k_cache *cache,
@@ -260,8 +258,7 @@ int b2k_norm_rotate_write(const b2k_rotation *r, const b2k_heads *v, const b2k_h
     p.slots = slots_dev;
     p.slot_bytes = slot_bytes;
     set_rotation(p, *r);
-    const Plan plan = choose(p, r->format, r);
-    return launch_forward<kBoth>(p, r->format, plan, b2k::as_stream(stream), name);
+    return launch_forward<kBoth>(p, r->format, r, b2k::as_stream(stream), name);
 }
 
 int b2k_cache_read(const b2k_cache *cache, int format, int64_t rows, const b2k_heads *k_out, const b2k_heads *v_out,
@@ -311,13 +308,27 @@ int b2k_cache_read(const b2k_cache *cache, int format, int64_t rows, const b2k_h
     while (p.tile > 4 && rows / p.tile < b2k::sm_count()) p.tile /= 2;
     const int64_t blocks = (rows + p.tile - 1) / p.tile;
     if (blocks > INT_MAX) return b2k::fail(B2K_ERR_TOO_LARGE, "%s: too many rows for one launch", name);
-    const dim3 grid(static_cast<unsigned>(blocks), v_out->heads ? 2 : 1);
     const cudaStream_t st = b2k::as_stream(stream);
-    if (format == B2K_FMT_F32) pick_read<float>(p, grid, st);
-    else if (format == B2K_FMT_F16) pick_read<__half>(p, grid, st);
-    else pick_read<__nv_bfloat16>(p, grid, st);
-    B2K_RETURN_IF_LAUNCH_FAILED(name);
-    b2k::note_launch();
+    int sides = 0, cv[2] = {};
+    double items = 0;
+    for (ReadSide &side : p.side) {                     // the sides that are there come first
+        if (side.heads == 0) continue;
+        items += static_cast<double>(rows) * side.heads * side.dim;
+        cv[sides] = widest_read(side, item_bytes(format));
+        p.side[sides++] = side;
+    }
+    // sides of different chunks: as in launch_forward
+    const bool split = sides == 2 && cv[0] != cv[1] && items >= kItemsToSplit;
+    if (sides == 2 && !split) cv[0] = cv[0] < cv[1] ? cv[0] : cv[1];
+    for (int i = 0; i < (split ? 2 : 1); ++i) {
+        if (i) p.side[0] = p.side[1];
+        const dim3 grid(static_cast<unsigned>(blocks), split ? 1 : sides);
+        if (format == B2K_FMT_F32) pick_read<float>(p, cv[i], grid, st);
+        else if (format == B2K_FMT_F16) pick_read<__half>(p, cv[i], grid, st);
+        else pick_read<__nv_bfloat16>(p, cv[i], grid, st);
+        B2K_RETURN_IF_LAUNCH_FAILED(name);
+        b2k::note_launch();
+    }
     return B2K_OK;
 }
 

@@ -78,7 +78,7 @@ SHAPES = [  # tokens, q heads, k heads, dim, rotated, interleaved
     (7, 5, 1, 80, 80, False), (3, 6, 2, 96, 48, False), (9, 2, 2, 100, 50, False), (1, 1, 1, 256, 256, True),
     (2, 7, 1, 192, 64, False), (4, 2, 1, 576, 64, True), (3, 2, 2, 1024, 1024, False), (3, 1, 1, 1022, 510, True),
     (6, 2, 2, 127, 6, False), (6, 2, 2, 127, 126, True), (2, 1, 1, 2, 2, False), (3, 2, 1, 1, 0, False), (11, 9, 3, 72, 0, False),
-    (40, 33, 5, 32, 16, False), (257, 12, 4, 112, 112, False), (2, 3, 2, 24, 8, True),
+    (40, 33, 5, 32, 16, False), (9, 3, 2, 100, 100, False), (9, 3, 2, 50, 50, True), (5, 2, 1, 300, 100, False), (3, 1, 1, 516, 20, False), (257, 12, 4, 112, 112, False), (2, 3, 2, 24, 8, True),
 ]
 
 
@@ -177,6 +177,19 @@ def test_heads_of_different_sizes():
         dx, size, dw, dw_size = ref.norm_rotate_backward(f64(x), f64(w), c, s, f64(x), 1e-6, False, True)
         check(got[i].as_torch(), dx, size, "float16", 128)
         check(got[2 + i].as_torch(), dw, dw_size, "float16", 64 + x.shape[0] * x.shape[1])
+
+
+@pytest.mark.parametrize("dim,kdim", [(50, 1024), (1024, 50), (1022, 64), (36, 1000), (3, 1024)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_long_rows_beside_narrow_chunks(dim, kdim, dtype):
+    rng, q, k, qw, kw, _, _, _ = setup(5, 2, 3, dim, 0, dtype, "contiguous", "float32", 0, kdim=kdim)
+    qo, ko = headnorm.norm_rotate(q, k, qw, kw)
+    got = headnorm.norm_rotate_backward(q, k, qw, kw, None, None, None, q, k)
+    for i, (x, w, y) in enumerate(((q, qw, qo), (k, kw, ko))):
+        check(y.as_torch(), *ref.norm_rotate(f64(x), f64(w), None, None, 1e-6, False, True), dtype)
+        dx, size, dw, dw_size = ref.norm_rotate_backward(f64(x), f64(w), None, None, f64(x), 1e-6, False, True)
+        check(got[i].as_torch(), dx, size, dtype, 128)
+        check(got[2 + i].as_torch(), dw, dw_size, "float32", 64 + x.shape[0] * x.shape[1])
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])

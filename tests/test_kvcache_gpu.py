@@ -59,6 +59,7 @@ CACHES = [  # tokens, heads, dim, v dim, group (0: whole head), page size, pages
     (5, 2, 128, 128, 0, 16, 4, "token"), (33, 3, 64, 64, 32, 16, 9, "head"), (1, 1, 1, 1, 0, 1, 3, "token"),
     (70, 2, 96, 48, 16, 7, 30, "odd"), (9, 4, 100, 33, 0, 5, 8, "token"), (12, 2, 256, 512, 64, 64, 2, "head"),
     (3, 1, 576, 576, 0, 3, 40, "token"), (4, 2, 1024, 1024, 16, 16, 2, "token"), (31, 5, 72, 200, 0, 10, 12, "odd"),
+    (3500, 2, 128, 33, 0, 16, 230, "token"),      # large, with sides of different chunk widths: a launch each
     (8, 1, 80, 80, 16, 16, 4, "token"), (64, 8, 40, 40, 20, 16, 5, "token"), (6, 2, 1023, 7, 0, 4, 4, "token"),
 ]
 
@@ -152,6 +153,7 @@ READS = [  # lengths, heads, dim, v dim, group, page size, pages, head axis
     ([5, 0, 17, 1], 2, 128, 128, 0, 16, 6, "token"), ([40], 3, 64, 96, 32, 7, 9, "head"), ([1], 1, 1, 1, 0, 1, 3, "token"),
     ([0, 0], 1, 16, 16, 0, 16, 2, "token"), ([33, 64, 2, 0, 0, 9], 4, 72, 200, 0, 16, 11, "odd"),
     ([100, 3], 1, 576, 576, 64, 64, 3, "token"), ([12, 12], 2, 1024, 1024, 16, 5, 8, "head"), ([9], 5, 100, 33, 0, 4, 5, "token"),
+    ([3000, 0, 900], 2, 128, 33, 0, 16, 30, "token"),
     ([31, 30, 29], 2, 80, 40, 0, 10, 7, "token"), ([6, 5], 2, 1023, 8, 0, 3, 9, "odd"), ([200] * 40, 1, 64, 64, 0, 16, 30, "token"),
 ]
 
@@ -297,9 +299,10 @@ def test_step(tokens, qh, kh, dim, v_dim, rot, inter, group, dtype, wdtype, fmt,
         rng, q, k, qw, kw, cos, sin, pos = setup(tokens, qh, kh, dim, rot, dtype, how, wdtype, seed)
         v = layout((tokens, kh, v_dim), how, dtype, rng)
         groups = [group or d if d % (group or d) == 0 else d for d in (dim, v_dim)]
-        pools = [pool(30, 13, kh, d, g, fmt, scale, rng) for d, g in zip((dim, v_dim), groups)]
+        pages = 30 if tokens < 390 else 201
+        pools = [pool(pages, 13, kh, d, g, fmt, scale, rng) for d, g in zip((dim, v_dim), groups)]
         before = [values(*p, fmt, scale) for p in pools]
-        slots = rng.permutation(30 * 13)[:tokens]
+        slots = rng.permutation(pages * 13)[:tokens]
         if tokens > 3:
             slots[2] = -1
         q_out = torch.full((tokens, qh, dim), 5.0, dtype=TORCH[dtype], device="cuda")
@@ -315,7 +318,7 @@ def test_step(tokens, qh, kh, dim, v_dim, rot, inter, group, dtype, wdtype, fmt,
         vc, vs = ref.quantise(f64(v), groups[1], fmt, scale)                       # values are not computed with: equal
         np.testing.assert_array_equal(flat[1][0], vc[there])
         np.testing.assert_array_equal(flat[1][1], vs[there])
-        rest = np.setdiff1d(np.arange(30 * 13), slots)
+        rest = np.setdiff1d(np.arange(pages * 13), slots)
         for p, old in zip(pools, before):
             for a, b in zip(values(*p, fmt, scale), old):
                 np.testing.assert_array_equal(a.reshape(-1, *a.shape[2:])[rest], b.reshape(-1, *b.shape[2:])[rest])
