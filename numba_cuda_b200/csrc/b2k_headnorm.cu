@@ -58,6 +58,8 @@ int check_heads(const b2k_heads &h, const char *name, const char *what, int64_t 
     if (h.dim < 1) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s has no items in a head", name, what);
     if (h.dim > B2K_MAX_HEAD_DIM)
         return b2k::fail(B2K_ERR_TOO_LARGE, "%s: %s has heads of more than %d items", name, what, B2K_MAX_HEAD_DIM);
+    if (h.heads > INT_MAX / h.dim)
+        return b2k::fail(B2K_ERR_TOO_LARGE, "%s: a token of %s has more than 2^31 - 1 items", name, what);
     if (tokens == 0) return B2K_OK;
     if (h.data_dev == nullptr) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s is a null pointer", name, what);
     if (reinterpret_cast<uintptr_t>(h.data_dev) % itemsize)
@@ -533,7 +535,7 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
 }
 
 // Four blocks an SM where a row takes one unit a lane (128 registers; 32768 tokens x 40
-// heads of 128 bf16 items: 208 us, with three blocks of 146 registers 234 us).
+// heads of 128 bf16 items: 198 us, with three blocks of 146 registers 215 us).
 template <typename T, int VEC, int ITER>
 __global__ void __launch_bounds__(kThreads, ITER == 1 ? 4 : 1) heads_backward_kernel(const __grid_constant__ Params p) {
     extern __shared__ float block_sums[];             // one row of dim floats per warp
@@ -601,7 +603,8 @@ int resident_blocks() {
 template <typename T>
 static int pick_backward(const Params &p, const Plan &plan, bool launch, int blocks, size_t shared, cudaStream_t stream) {
 #define B2K_HEADS_CASE(V, I)                                                                              \
-    if constexpr (V * sizeof(T) <= 16) if (plan.vec == V && plan.iter == I) {                             \
+    if constexpr (V * sizeof(T) <= 16)                                                                    \
+    if (plan.vec == V && plan.iter == I) {                                                                \
         if (!launch) return resident_blocks<T, V, I>();                                                   \
         heads_backward_kernel<T, V, I><<<blocks, kThreads, shared, stream>>>(p);                          \
         return 0;                                                                                         \

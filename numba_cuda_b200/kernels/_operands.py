@@ -152,7 +152,11 @@ class _NoFast:
 class _Fast:
     """The extension ``_pyfast``, set up when it is first used (it needs the library)."""
 
+    ENTRIES = ("norm_rotate", "norm_rotate_backward", "cache_write", "cache_read", "norm_rotate_write")
+
     def __getattr__(self, name):
+        if name not in self.ENTRIES:
+            raise AttributeError(name)
         try:
             from .. import _pyfast as module
         except ImportError:
@@ -163,7 +167,7 @@ class _Fast:
                      "b2k_cache_write", "b2k_cache_read", "b2k_norm_rotate_write", "b2k_current_device")
             module.setup(torch.Tensor, _TORCH, {n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names},
                          stream_ptr, workspace)
-        for entry in ("norm_rotate", "norm_rotate_backward", "cache_write", "cache_read", "norm_rotate_write"):
+        for entry in self.ENTRIES:
             setattr(self, entry, getattr(module, entry))
         return self.__dict__[name]
 

@@ -127,6 +127,7 @@ def test_norm_rotate_refusals():
     assert call(_rotation(q=(4098, 64, 16, 4, 16))) == _lib.ERR_ALIGNMENT
     assert call(_rotation(q=(0, 64, 16, 4, 16))) == _lib.ERR_INVALID_ARG
     assert call(_rotation(q=(4096, 64, 16, 4, 1025)), _heads(dim=1025)) == _lib.ERR_TOO_LARGE
+    assert call(_rotation(q=(4096, 64, 16, 2 ** 30, 16)), _heads(heads=2 ** 30)) == _lib.ERR_TOO_LARGE
     assert call(_rotation(q=(4096, 64, 16, -4, 16))) == _lib.ERR_INVALID_ARG
     assert call(_rotation(q=(4096, 64, 16, 4, 0))) == _lib.ERR_INVALID_ARG
     assert call(_rotation(norm=2)) == _lib.ERR_INVALID_ARG
