@@ -403,47 +403,103 @@ __device__ __forceinline__ void gradient_of(const float (&x)[VEC], float (&g)[VE
     }
 }
 
-template <typename T, int VEC, int ITER, int WHICH, bool INTER>
-__device__ __forceinline__ void backward_role(const Params &p, uint32_t first_block, uint32_t blocks, float *block_sums) {
-    const Role &r = p.role[WHICH];
-    const Lanes g(p.lanes);
-    const uint32_t in_block = static_cast<uint32_t>(kThreads) >> p.lane_bits;
-    // w, sums and rows are kept in the order of the pairs
-    int oa[ITER], ob[ITER];
-    float wx[ITER][VEC], wy[ITER][VEC], sum_x[ITER][VEC] = {}, sum_y[ITER][VEC] = {};
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        unit_at<VEC>(r, g.lane + i * g.n, oa[i], ob[i]);
-        float wa[VEC] = {}, wb[VEC] = {};
-        if (oa[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa[i], wa);
-        if (ob[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob[i], wb);
-        in_pairs<VEC, INTER>(wa, wb, wx[i], wy[i]);
-    }
-    // A warp's groups take neighbouring items and stay together: see Lanes.  all_items < 2^31,
-    // and a step is at most the grid's groups, so nothing overflows.
-    const uint32_t in_warp = 32u >> p.lane_bits;
-    for (uint32_t base = first_block * in_block + threadIdx.x / 32 * in_warp; base < r.all_items; base += blocks * in_block) {
-        const uint32_t item = base + (threadIdx.x % 32 >> p.lane_bits);
+// What a group knows of an item: its rows and where they start.
+template <typename T>
+struct Item {
+    int64_t token;
+    int rows;                    // 0 behind the last item
+    const T *in, *grad;
+    T *out;
+    __device__ __forceinline__ void seek(const Role &r, uint32_t item) {
         const bool active = item < r.all_items;
         const uint32_t at_token = active ? r.items.quotient(item) : 0;
-        const int64_t token = at_token;
+        token = at_token;
         const int first = active ? static_cast<int>(item - at_token * r.items.d) * r.heads_per_item : 0;
-        const int rows = active ? min(r.heads - first, r.heads_per_item) : 0;
-        const T *in = static_cast<const T *>(r.in) + token * r.in_token + first * r.in_head;
-        const T *grad = static_cast<const T *>(r.grad) + token * r.grad_token + first * r.grad_head;
-        T *out = static_cast<T *>(r.out) + token * r.out_token + first * r.out_head;
+        rows = active ? min(r.heads - first, r.heads_per_item) : 0;
+        in = static_cast<const T *>(r.in) + token * r.in_token + first * r.in_head;
+        grad = static_cast<const T *>(r.grad) + token * r.grad_token + first * r.grad_head;
+        out = static_cast<T *>(r.out) + token * r.out_token + first * r.out_head;
+    }
+};
+
+// A lane's share of a role's weight and of its gradient, in the order of the pairs.
+template <int VEC, int ITER>
+struct Weights {
+    float x[ITER][VEC], y[ITER][VEC], sum_x[ITER][VEC], sum_y[ITER][VEC];
+};
+
+// The gradient of one row as loaded (x and g, two chunks a unit), stored to `out` if `there`.
+// A padding token's rows come as zeros.
+template <typename T, int VEC, int ITER, bool INTER>
+__device__ __forceinline__ void gradient_row(const Params &p, const Role &r, const Lanes &g, const int (&oa)[ITER],
+                                             const int (&ob)[ITER], const Chunk<T, VEC> (&xa)[ITER],
+                                             const Chunk<T, VEC> (&xb)[ITER], const Chunk<T, VEC> (&da)[ITER],
+                                             const Chunk<T, VEC> (&db)[ITER], const float (&c)[ITER][VEC],
+                                             const float (&s)[ITER][VEC], Weights<VEC, ITER> &w, T *out, bool padding,
+                                             bool there) {
+    float x[ITER][VEC], y[ITER][VEC], gx[ITER][VEC], gy[ITER][VEC];
+    float2 ss = make_float2(0.0f, 0.0f), dot = ss;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        float a[VEC], b[VEC];
+        widen(xa[i], a);
+        widen(xb[i], b);
+        in_pairs<VEC, INTER>(a, b, x[i], y[i]);
+        widen(da[i], a);
+        widen(db[i], b);
+        in_pairs<VEC, INTER>(a, b, gx[i], gy[i]);
+        const Turned t = turned_of<VEC, INTER>(r, g.lane + i * g.n, oa[i], ob[i]);
+        if (VEC > 1 && t.lo) turn_back<0, VEC / 2, VEC>(gx[i], gy[i], c[i], s[i]);
+        if (t.hi) turn_back<VEC / 2, VEC, VEC>(gx[i], gy[i], c[i], s[i]);
+        gradient_sums<VEC>(x[i], gx[i], w.x[i], ss, dot);
+        gradient_sums<VEC>(y[i], gy[i], w.y[i], ss, dot);
+    }
+    if (p.norm) {
+        // dx = r (h - n mean(h n)) with n = x r:  r h - x (r^3 sum(h x) / dim)
+        const float mean = g.sum(ss.x + ss.y) * r.inv_dim;
+        const float by = padding || !there ? 0.0f : rsqrtf(mean + p.eps);       // eps may be zero
+        const float pull = g.sum(dot.x + dot.y) * r.inv_dim * by * by * by;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            gradient_of<VEC>(x[i], gx[i], w.x[i], by, pull, w.sum_x[i]);
+            gradient_of<VEC>(y[i], gy[i], w.y[i], by, pull, w.sum_y[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        float a[VEC], b[VEC];
+        out_of_pairs<VEC, INTER>(gx[i], gy[i], a, b);
+        if (there && oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a);
+        if (there && ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b);
+    }
+}
+
+__device__ __forceinline__ bool is_padding(const Params &p, int64_t position) {
+    return p.positions != nullptr && (position < 0 || position >= p.table_rows);
+}
+__device__ __forceinline__ int64_t position_of(const Params &p, int64_t token) {
+    return p.positions != nullptr ? paging::load_index(p.positions, p.position_bytes, token) : 0;
+}
+
+// The rows of a warp's items `base`, `base + step`, ..., the next row loaded into registers
+// while one is worked on.  A warp's groups take neighbouring items and stay together: see
+// Lanes.  all_items < 2^31, and a step is at most the grid's groups, so nothing overflows.
+template <typename T, int VEC, int ITER, bool INTER>
+__device__ __forceinline__ void backward_rows(const Params &p, const Role &r, const Lanes &g, uint32_t base, uint32_t step,
+                                              const int (&oa)[ITER], const int (&ob)[ITER], Weights<VEC, ITER> &w) {
+    for (; base < r.all_items; base += step) {
+        Item<T> it;
+        it.seek(r, base + (threadIdx.x % 32 >> p.lane_bits));
         Batch<T, VEC, ITER, 1> x_now, g_now;
-        x_now.load(in, 0, rows, oa, ob, r.dim);
-        g_now.load(grad, 0, rows, oa, ob, r.dim);
-        int64_t position = 0;
-        if (p.positions != nullptr) position = paging::load_index(p.positions, p.position_bytes, token);
-        // a padding token's rows are taken as zeros all through, with by = 0 below
-        const bool padding = p.positions != nullptr && (position < 0 || position >= p.table_rows);
+        x_now.load(it.in, 0, it.rows, oa, ob, r.dim);
+        g_now.load(it.grad, 0, it.rows, oa, ob, r.dim);
+        const int64_t position = position_of(p, it.token);
+        const bool padding = is_padding(p, position);
         if (padding) {
             x_now = Batch<T, VEC, ITER, 1>{};
             g_now = Batch<T, VEC, ITER, 1>{};
         }
-        const int loads = padding ? 0 : rows;
+        const int loads = padding ? 0 : it.rows;
         float c[ITER][VEC], s[ITER][VEC];
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
@@ -454,63 +510,211 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
             load_angles<VEC, INTER>(p.cos_table + position * p.cos_stride, u, oa[i], ob[i], t, c[i]);
             load_angles<VEC, INTER>(p.sin_table + position * p.sin_stride, u, oa[i], ob[i], t, s[i]);
         }
-        const int most = __reduce_max_sync(0xFFFFFFFFu, rows);
+        const int most = __reduce_max_sync(0xFFFFFFFFu, it.rows);
 #pragma unroll 1
         for (int h = 0; h < most; ++h) {
-            // the next row is on its way while this one is worked on
             Batch<T, VEC, ITER, 1> x_next, g_next;
-            in += r.in_head;
-            grad += r.grad_head;
-            x_next.load(in, 0, loads - h - 1, oa, ob, r.dim);
-            g_next.load(grad, 0, loads - h - 1, oa, ob, r.dim);
-            float x[ITER][VEC], y[ITER][VEC], gx[ITER][VEC], gy[ITER][VEC];
-            float2 ss = make_float2(0.0f, 0.0f), dot = ss;
-#pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                float a[VEC], b[VEC];
-                widen(x_now.a[0][i], a);
-                widen(x_now.b[0][i], b);
-                in_pairs<VEC, INTER>(a, b, x[i], y[i]);
-                widen(g_now.a[0][i], a);
-                widen(g_now.b[0][i], b);
-                in_pairs<VEC, INTER>(a, b, gx[i], gy[i]);
-                const Turned t = turned_of<VEC, INTER>(r, g.lane + i * g.n, oa[i], ob[i]);
-                if (VEC > 1 && t.lo) turn_back<0, VEC / 2, VEC>(gx[i], gy[i], c[i], s[i]);
-                if (t.hi) turn_back<VEC / 2, VEC, VEC>(gx[i], gy[i], c[i], s[i]);
-                gradient_sums<VEC>(x[i], gx[i], wx[i], ss, dot);
-                gradient_sums<VEC>(y[i], gy[i], wy[i], ss, dot);
-            }
-            if (p.norm) {
-                // dx = r (h - n mean(h n)) with n = x r:  r h - x (r^3 sum(h x) / dim)
-                const bool none = padding || h >= rows;       // eps may be zero
-                const float mean = g.sum(ss.x + ss.y) * r.inv_dim;
-                const float by = none ? 0.0f : rsqrtf(mean + p.eps);
-                const float pull = g.sum(dot.x + dot.y) * r.inv_dim * by * by * by;
-#pragma unroll
-                for (int i = 0; i < ITER; ++i) {
-                    gradient_of<VEC>(x[i], gx[i], wx[i], by, pull, sum_x[i]);
-                    gradient_of<VEC>(y[i], gy[i], wy[i], by, pull, sum_y[i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                float a[VEC], b[VEC];
-                out_of_pairs<VEC, INTER>(gx[i], gy[i], a, b);
-                if (h < rows && oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a);
-                if (h < rows && ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b);
-            }
-            out += r.out_head;
+            it.in += r.in_head;
+            it.grad += r.grad_head;
+            x_next.load(it.in, 0, loads - h - 1, oa, ob, r.dim);
+            g_next.load(it.grad, 0, loads - h - 1, oa, ob, r.dim);
+            gradient_row<T, VEC, ITER, INTER>(p, r, g, oa, ob, x_now.a[0], x_now.b[0], g_now.a[0], g_now.b[0], c, s, w, it.out, padding,
+                                       h < it.rows);
+            it.out += r.out_head;
             x_now = x_next;
             g_now = g_next;
         }
     }
+}
+
+// The same with the rows of kStages - 1 steps ahead on their way into shared memory, across
+// the ends of items, with the next item's cosines and sines: registers no longer limit
+// the bytes in flight, and no warp waits for a position and then for its table rows.
+// Every thread copies what it will read itself, so there is nothing to synchronise but its
+// own copies.  32768 tokens x 40 heads of 128 bf16 items: 198 us with the next row in
+// registers, 174 us so, 177 us with four stages.  Needs 16-byte chunks, one unit a lane,
+// and items of at least kStages steps (then the loads are at most one item ahead).
+constexpr int kStages = 3;
+
+template <int VEC>
+struct Ring {
+    static constexpr int half = VEC * 2;             // bytes of VEC / 2 floats
+    static constexpr int rows = kStages * 4 * kThreads * 16, tables = 2 * 4 * kThreads * half;
+};
+
+// Shared memory of a block: the copies, and later one row of floats per warp for the
+// weight's sums (rows of one unit a lane have at most 64 * VEC items).
+template <typename T, int VEC, bool AHEAD>
+constexpr int shared_bytes() {
+    return AHEAD ? Ring<VEC>::rows + Ring<VEC>::tables : kThreads / 32 * B2K_MAX_HEAD_DIM * 4;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void *to_shared, const void *from) {
+    const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(to_shared));
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+template <typename T, int VEC, bool INTER>
+__device__ __forceinline__ void backward_rows_ahead(const Params &p, const Role &r, const Lanes &g, uint32_t base, uint32_t step,
+                                                    const int (&oa)[1], const int (&ob)[1], Weights<VEC, 1> &w, char *shared) {
+    using Slots = Ring<VEC>;
+    constexpr int H = VEC / 2;
+    const int hpi = r.heads_per_item;
+    const uint32_t in_warp = threadIdx.x % 32 >> p.lane_bits;
+    const Turned turned = turned_of<VEC, INTER>(r, g.lane, oa[0], ob[0]);
+    const int at_lo = INTER ? oa[0] / 2 : g.lane * VEC, at_hi = INTER ? ob[0] / 2 : g.lane * VEC + H;
+    const bool has_a = oa[0] < r.dim, has_b = ob[0] < r.dim;
+    // slots are [stage][array][thread], so neighbouring threads' 16 bytes are neighbours
+    char *const row_slot = shared + threadIdx.x * 16;
+    char *const table_slot = shared + Slots::rows + threadIdx.x * Slots::half;
+
+    // the load side: its item, row and position, and the position of the item after it
+    Item<T> ahead;
+    uint32_t ahead_base = base;
+    int ahead_h = 0, ahead_stage = 0, ahead_table = 0;
+    int64_t ahead_position = 0, after_position = 0;
+    const auto later_position = [&](uint32_t at) {
+        const uint32_t item = at + in_warp;
+        return item < r.all_items ? position_of(p, r.items.quotient(item)) : 0;
+    };
+    const auto load_step = [&]() {
+        if (ahead_base < r.all_items) {
+            if (ahead_h == 0 && p.positions != nullptr && !is_padding(p, ahead_position) && ahead.rows > 0) {
+                char *to = table_slot + ahead_table * 4 * kThreads * Slots::half;
+                const float *c = p.cos_table + ahead_position * p.cos_stride, *s = p.sin_table + ahead_position * p.sin_stride;
+                if (turned.lo) {
+                    copy_async<Slots::half>(to, c + at_lo);
+                    copy_async<Slots::half>(to + 2 * kThreads * Slots::half, s + at_lo);
+                }
+                if (turned.hi) {
+                    copy_async<Slots::half>(to + kThreads * Slots::half, c + at_hi);
+                    copy_async<Slots::half>(to + 3 * kThreads * Slots::half, s + at_hi);
+                }
+            }
+            if (ahead_h < ahead.rows) {
+                char *to = row_slot + ahead_stage * 4 * kThreads * 16;
+                if (has_a) {
+                    copy_async<16>(to, ahead.in + oa[0]);
+                    copy_async<16>(to + 2 * kThreads * 16, ahead.grad + oa[0]);
+                }
+                if (has_b) {
+                    copy_async<16>(to + kThreads * 16, ahead.in + ob[0]);
+                    copy_async<16>(to + 3 * kThreads * 16, ahead.grad + ob[0]);
+                }
+            }
+            ahead.in += r.in_head;
+            ahead.grad += r.grad_head;
+            if (++ahead_h == hpi) {
+                ahead_h = 0;
+                ahead_table ^= 1;
+                ahead_base += step;
+                ahead.seek(r, ahead_base + in_warp);
+                ahead_position = after_position;
+                after_position = later_position(ahead_base + step);
+            }
+        }
+        commit_copies();
+        ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
+    };
+
+    if (base >= r.all_items) return;
+    ahead.seek(r, base + in_warp);
+    ahead_position = later_position(base);
+    after_position = later_position(base + step);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) load_step();
+
+    int stage = 0, table = 0;
+    for (; base < r.all_items; base += step) {
+        // the load side is still in this item: see kStages
+        const int rows = ahead.rows;
+        T *out = ahead.out;
+        const bool padding = is_padding(p, ahead_position);
+#pragma unroll 1
+        for (int h = 0; h < hpi; ++h) {
+            wait_copies<kStages - 2>();
+            // read again for every row: 16 registers less
+            float c[1][VEC] = {}, s[1][VEC] = {};
+            {
+                const char *angles = table_slot + table * 4 * kThreads * Slots::half;
+                float lo[H], hi[H];
+                if (turned.lo) {
+                    load_floats<H>(reinterpret_cast<const float *>(angles), lo);
+                    load_floats<H>(reinterpret_cast<const float *>(angles + 2 * kThreads * Slots::half), hi);
+#pragma unroll
+                    for (int j = 0; j < H; ++j) {
+                        c[0][j] = lo[j];
+                        s[0][j] = hi[j];
+                    }
+                }
+                if (turned.hi) {
+                    load_floats<H>(reinterpret_cast<const float *>(angles + kThreads * Slots::half), lo);
+                    load_floats<H>(reinterpret_cast<const float *>(angles + 3 * kThreads * Slots::half), hi);
+#pragma unroll
+                    for (int j = 0; j < H; ++j) {
+                        c[0][H + j] = lo[j];
+                        s[0][H + j] = hi[j];
+                    }
+                }
+            }
+            const T *from = reinterpret_cast<const T *>(row_slot + stage * 4 * kThreads * 16);
+            constexpr int next = kThreads * 16 / sizeof(T);
+            const bool there = h < rows;
+            Chunk<T, VEC> xa[1] = {}, xb[1] = {}, da[1] = {}, db[1] = {};
+            if (there && !padding && has_a) {
+                xa[0] = load_chunk<T, VEC>(from);
+                da[0] = load_chunk<T, VEC>(from + 2 * next);
+            }
+            if (there && !padding && has_b) {
+                xb[0] = load_chunk<T, VEC>(from + next);
+                db[0] = load_chunk<T, VEC>(from + 3 * next);
+            }
+            load_step();                     // into the slot that the step before this one read
+            gradient_row<T, VEC, 1, INTER>(p, r, g, oa, ob, xa, xb, da, db, c, s, w, out, padding, there);
+            out += r.out_head;
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+        table ^= 1;
+    }
+    wait_copies<0>();
+}
+
+template <typename T, int VEC, int ITER, bool AHEAD, int WHICH, bool INTER>
+__device__ __forceinline__ void backward_role(const Params &p, uint32_t first_block, uint32_t blocks, char *shared) {
+    const Role &r = p.role[WHICH];
+    const Lanes g(p.lanes);
+    const uint32_t in_block = static_cast<uint32_t>(kThreads) >> p.lane_bits;
+    int oa[ITER], ob[ITER];
+    Weights<VEC, ITER> w;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        unit_at<VEC>(r, g.lane + i * g.n, oa[i], ob[i]);
+        float wa[VEC] = {}, wb[VEC] = {};
+        if (oa[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, oa[i], wa);
+        if (ob[i] < r.dim) load_weight<VEC>(r.weight, p.weight_format, ob[i], wb);
+        in_pairs<VEC, INTER>(wa, wb, w.x[i], w.y[i]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w.sum_x[i][j] = w.sum_y[i][j] = 0.0f;
+    }
+    const uint32_t base = first_block * in_block + threadIdx.x / 32 * (32u >> p.lane_bits), step = blocks * in_block;
+    if constexpr (AHEAD) backward_rows_ahead<T, VEC, INTER>(p, r, g, base, step, oa, ob, w, shared);
+    else backward_rows<T, VEC, ITER, INTER>(p, r, g, base, step, oa, ob, w);
     if (r.weight_grad == nullptr) return;
     // groups of a warp, then the block's warps in order
+    __syncthreads();                                     // the copies' memory is free now
+    float *block_sums = reinterpret_cast<float *>(shared);       // one row of dim floats per warp
     const int warp = threadIdx.x / 32;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         float a[VEC], b[VEC];
-        out_of_pairs<VEC, INTER>(sum_x[i], sum_y[i], a, b);
+        out_of_pairs<VEC, INTER>(w.sum_x[i], w.sum_y[i], a, b);
         for (int o = g.n; o < 32; o *= 2)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
@@ -529,23 +733,23 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
     float *row = p.partials + static_cast<int64_t>(blockIdx.x) * p.partial_stride;
     for (int d = threadIdx.x; d < r.dim; d += kThreads) {
         float v = 0.0f;
-        for (int w = 0; w < kThreads / 32; ++w) v += block_sums[w * r.dim + d];
+        for (int k = 0; k < kThreads / 32; ++k) v += block_sums[k * r.dim + d];
         row[d] = v;
     }
 }
 
 // Four blocks an SM where a row takes one unit a lane (128 registers; 32768 tokens x 40
-// heads of 128 bf16 items: 198 us, with three blocks of 146 registers 215 us).
-template <typename T, int VEC, int ITER>
+// heads of 128 bf16 items: 174 us, with three blocks 178 us).
+template <typename T, int VEC, int ITER, bool AHEAD>
 __global__ void __launch_bounds__(kThreads, ITER == 1 ? 4 : 1) heads_backward_kernel(const __grid_constant__ Params p) {
-    extern __shared__ float block_sums[];             // one row of dim floats per warp
+    extern __shared__ __align__(16) char shared[];
     const uint32_t blocks0 = p.blocks0, blocks1 = gridDim.x - blocks0;
     if (VEC > 1 && p.interleaved) {
-        if (blockIdx.x < blocks0) backward_role<T, VEC, ITER, 0, true>(p, blockIdx.x, blocks0, block_sums);
-        else backward_role<T, VEC, ITER, 1, true>(p, blockIdx.x - blocks0, blocks1, block_sums);
+        if (blockIdx.x < blocks0) backward_role<T, VEC, ITER, AHEAD, 0, true>(p, blockIdx.x, blocks0, shared);
+        else backward_role<T, VEC, ITER, AHEAD, 1, true>(p, blockIdx.x - blocks0, blocks1, shared);
     } else {
-        if (blockIdx.x < blocks0) backward_role<T, VEC, ITER, 0, false>(p, blockIdx.x, blocks0, block_sums);
-        else backward_role<T, VEC, ITER, 1, false>(p, blockIdx.x - blocks0, blocks1, block_sums);
+        if (blockIdx.x < blocks0) backward_role<T, VEC, ITER, AHEAD, 0, false>(p, blockIdx.x, blocks0, shared);
+        else backward_role<T, VEC, ITER, AHEAD, 1, false>(p, blockIdx.x - blocks0, blocks1, shared);
     }
 }
 
@@ -580,10 +784,9 @@ __global__ void __launch_bounds__(kSumThreads) weight_grad_kernel(const __grid_c
     else static_cast<__nv_bfloat16 *>(r.weight_grad)[at] = __float2bfloat16_rn(sum);
 }
 
-// Blocks of one instantiation that an SM holds at once: the grid is one full wave, since
-// a second, partial one would leave most SMs idle (4 blocks an SM where 3 fit: 313 us
-// instead of 226 us for 32768 tokens x 40 heads of 128 bf16 items).
-template <typename T, int VEC, int ITER>
+// Blocks of one instantiation that an SM holds at once: the grid is at most one wave, since
+// a second, partial one would leave most SMs idle (4 blocks an SM where 3 fit cost 40%).
+template <typename T, int VEC, int ITER, bool AHEAD>
 int resident_blocks() {
     static b2k::PerDeviceOnce once;
     static int found[b2k::kMaxDevices];
@@ -592,33 +795,42 @@ int resident_blocks() {
     once.run([&] {
         int n = 0;
         const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-            &n, heads_backward_kernel<T, VEC, ITER>, kThreads, kThreads / 32 * B2K_MAX_HEAD_DIM * sizeof(float));
+            &n, heads_backward_kernel<T, VEC, ITER, AHEAD>, kThreads, shared_bytes<T, VEC, AHEAD>());
         found[dev] = n < 1 ? 1 : n > kMostBlocksPerSm ? kMostBlocksPerSm : n;
         return e;
     });
     return found[dev] < 1 ? 1 : found[dev];
 }
 
-// Launches, or with `launch` off says how many blocks an SM holds.
+// Launches `blocks` blocks, or with none says how many an SM holds.
+template <typename T, int VEC, int ITER, bool AHEAD>
+int backward_shape(const Params &p, int blocks, cudaStream_t stream) {
+    if (blocks == 0) return resident_blocks<T, VEC, ITER, AHEAD>();
+    heads_backward_kernel<T, VEC, ITER, AHEAD><<<blocks, kThreads, shared_bytes<T, VEC, AHEAD>(), stream>>>(p);
+    return 0;
+}
+
 template <typename T>
-static int pick_backward(const Params &p, const Plan &plan, bool launch, int blocks, size_t shared, cudaStream_t stream) {
+static int pick_backward(const Params &p, const Plan &plan, int blocks, cudaStream_t stream) {
+    // copies ahead need items of at least kStages steps in every role
+    bool ahead = true;
+    for (const Role &r : p.role) ahead = ahead && (r.heads == 0 || r.heads_per_item >= kStages);
 #define B2K_HEADS_CASE(V, I)                                                                              \
     if constexpr (V * sizeof(T) <= 16)                                                                    \
-    if (plan.vec == V && plan.iter == I) {                                                                \
-        if (!launch) return resident_blocks<T, V, I>();                                                   \
-        heads_backward_kernel<T, V, I><<<blocks, kThreads, shared, stream>>>(p);                          \
-        return 0;                                                                                         \
-    }
+        if (plan.vec == V && plan.iter == I) {                                                            \
+            if constexpr (V * sizeof(T) == 16 && I == 1)                                                  \
+                if (ahead) return backward_shape<T, V, I, true>(p, blocks, stream);                       \
+            return backward_shape<T, V, I, false>(p, blocks, stream);                                     \
+        }
     B2K_HEADS_SHAPES(B2K_HEADS_CASE)
 #undef B2K_HEADS_CASE
     return 1;
 }
 
-static int backward_kernel(int64_t format, const Params &p, const Plan &plan, bool launch, int blocks, size_t shared,
-                           cudaStream_t stream) {
-    if (format == B2K_FMT_F32) return pick_backward<float>(p, plan, launch, blocks, shared, stream);
-    if (format == B2K_FMT_F16) return pick_backward<__half>(p, plan, launch, blocks, shared, stream);
-    return pick_backward<__nv_bfloat16>(p, plan, launch, blocks, shared, stream);
+static int backward_kernel(int64_t format, const Params &p, const Plan &plan, int blocks, cudaStream_t stream) {
+    if (format == B2K_FMT_F32) return pick_backward<float>(p, plan, blocks, stream);
+    if (format == B2K_FMT_F16) return pick_backward<__half>(p, plan, blocks, stream);
+    return pick_backward<__nv_bfloat16>(p, plan, blocks, stream);
 }
 
 }  // namespace headwise
@@ -699,25 +911,24 @@ int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, con
     const Plan plan = lay_out(p, vec, r);
     if (plan.iter == 0) return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: no kernel for this head size", name);
     if (int rc = count_items(p, kBackwardHeadsPerItem, kThreads, name)) return rc;
-    // blocks go to the two roles by their share of the rows' items, at least one to each
     const cudaStream_t st = b2k::as_stream(stream);
-    int64_t need[2], most = b2k::sm_count() * static_cast<int64_t>(backward_kernel(r->format, p, plan, false, 0, 0, st));
-    for (int i = 0; i < 2; ++i) need[i] = p.role[i].blocks;
-    if (need[0] + need[1] > most) {
-        const int64_t total = need[0] + need[1];
-        int64_t first = need[0] * most / total;
-        if (need[0] && first < 1) first = 1;
-        if (need[1] && first > most - 1) first = most - 1;
-        need[0] = first;
-        need[1] = need[1] ? most - first : 0;
+    const int64_t most = b2k::sm_count() * static_cast<int64_t>(backward_kernel(r->format, p, plan, 0, st));
+    int64_t need[2] = {p.role[0].blocks, p.role[1].blocks};
+    // one wave, and as many blocks as give each the same number of rounds: 2.2 rounds of a
+    // full wave take as long as 3 (4096 tokens x 40 heads of 128 bf16 items: 41 us)
+    for (int64_t rounds = std::max<int64_t>(1, (need[0] + need[1] + most - 1) / most);; ++rounds) {
+        const int64_t share[2] = {(need[0] + rounds - 1) / rounds, (need[1] + rounds - 1) / rounds};
+        if (share[0] + share[1] > most) continue;
+        need[0] = share[0];
+        need[1] = share[1];
+        break;
     }
     p.blocks0 = static_cast<int>(need[0]);
     const int blocks = static_cast<int>(need[0] + need[1]);
     const int dim = p.role[0].dim > p.role[1].dim ? p.role[0].dim : p.role[1].dim;
     p.partial_stride = dim;
     if (blocks > 0) {
-        const size_t shared = summed ? static_cast<size_t>(kThreads / 32) * dim * sizeof(float) : 0;
-        backward_kernel(r->format, p, plan, true, blocks, shared, st);
+        backward_kernel(r->format, p, plan, blocks, st);
         B2K_RETURN_IF_LAUNCH_FAILED(name);
         b2k::note_launch();
     }
