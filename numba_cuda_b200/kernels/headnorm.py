@@ -115,6 +115,11 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, position
     :param q_out, k_out: outputs; new arrays when not given (padding rows are then not
                  set).  An output may be its own input's memory; it must not overlap an
                  input in any other way.
+    :param stream: stream of the launch (0 = the default stream); arrays that other streams
+                 produce must be complete or ordered before it, as everywhere here.
+
+    Squares are summed in float32: a head whose squares add up to more than 3.4e38 gives
+    zeros.
     """
     status = fast.norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, q_out, k_out, stream)
     if status is not None:
