@@ -212,34 +212,45 @@ bool read_rotation(PyObject *const *args, PyObject *eps, PyObject *interleaved, 
     return true;
 }
 
-// k_codes, k_scales, v_codes, v_scales of args[0..4); the codes' type tells the format
+// k_codes, k_scales, v_codes, v_scales of args[0..4); the codes' types or `format` tell what they are
 bool read_cache(PyObject *const *args, PyObject *format, int device, b2k_cache &c) {
-    if (format != Py_None) return false;
+    int code = -1;
+    if (format != Py_None) {
+        if (!PyUnicode_CheckExact(format)) return false;
+        if (PyUnicode_CompareWithASCIIString(format, "e4m3") == 0) code = B2K_FMT_E4M3;
+        else if (PyUnicode_CompareWithASCIIString(format, "e5m2") == 0) code = B2K_FMT_E5M2;
+        else return false;
+    }
     c = b2k_cache{};
-    c.code_format = c.scale_format = -1;
     b2k_pages *side[2] = {&c.k, &c.v};
+    bool any = false;
     for (int i = 0; i < 2; ++i) {
         PyObject *codes = args[2 * i], *scales = args[2 * i + 1];
         if (codes == Py_None && scales == Py_None) continue;
         Array a, s;
         if (!read(codes, device, a) || !read(scales, device, s) || a.ndim != 4 || s.ndim != 4) return false;
-        if (a.format != B2K_FMT_E4M3 && a.format != B2K_FMT_E5M2) return false;
+        if (a.format == B2K_FMT_E4M3 || a.format == B2K_FMT_E5M2) {
+            if (code >= 0 && code != a.format) return false;
+            code = a.format;
+        } else if (a.format != B2K_FMT_U8) {
+            return false;
+        }
+        if (s.format == B2K_FMT_U8) s.format = B2K_FMT_E8M0;
         if (s.format != B2K_FMT_F32 && s.format != B2K_FMT_E8M0) return false;
         for (int j = 0; j < 3; ++j)
             if (a.size[j] != s.size[j]) return false;
         if ((a.stride[3] != 1 && a.size[3] > 1) || (s.stride[3] != 1 && s.size[3] > 1)) return false;
         if (s.size[3] < 1 || a.size[3] % s.size[3]) return false;
-        if (c.code_format >= 0 &&
-            (c.code_format != a.format || c.scale_format != s.format || c.pages != a.size[0] || c.page_size != a.size[1]))
-            return false;
-        c.code_format = a.format;
+        if (any && (c.scale_format != s.format || c.pages != a.size[0] || c.page_size != a.size[1])) return false;
+        any = true;
         c.scale_format = s.format;
         c.pages = a.size[0];
         c.page_size = a.size[1];
         *side[i] = b2k_pages{a.data, a.stride[0], a.stride[1], a.stride[2], s.data, s.stride[0], s.stride[1], s.stride[2],
                              a.size[2], a.size[3], a.size[3] / s.size[3]};
     }
-    return c.code_format >= 0;
+    c.code_format = code < 0 ? B2K_FMT_E4M3 : code;
+    return any;
 }
 
 bool fits(bool given, const b2k_heads &h, const b2k_pages &side) {

@@ -45,7 +45,7 @@ def slow(monkeypatch):
         monkeypatch.setattr(module, "fast", Nothing())
 
 
-def everything(dtype, wdtype, inter, seed, scale):
+def everything(dtype, wdtype, inter, seed, scale, fmt=None):
     """All five calls on one set of tensors; the results."""
     rng, q, k, qw, kw, cos, sin, pos = setup(37, 4, 2, 64, 32, dtype, "packed", wdtype, seed)
     v = layout((37, 2, 96), "packed", dtype, rng)
@@ -55,9 +55,10 @@ def everything(dtype, wdtype, inter, seed, scale):
     def pools():
         out = []
         for d in (64, 96):
-            out.append(torch.zeros(5, 16, 2, d, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn))
+            codes = torch.zeros(5, 16, 2, d, dtype=torch.uint8, device="cuda")
+            out.append(codes.view(torch.float8_e4m3fn) if fmt is None else codes)
             s = torch.zeros(5, 16, 2, d // 32, dtype=torch.float32 if scale == "f32" else torch.uint8, device="cuda")
-            out.append(s if scale == "f32" else s.view(torch.float8_e8m0fnu))
+            out.append(s if scale == "f32" or fmt else s.view(torch.float8_e8m0fnu))
         return out
 
     qo, ko = torch.zeros_like(q), torch.zeros_like(k)
@@ -66,25 +67,26 @@ def everything(dtype, wdtype, inter, seed, scale):
     dw = [None if w is None else torch.zeros_like(w) for w in (qw, kw)]
     headnorm.norm_rotate_backward(q, k, qw, kw, cos, sin, pos, qo, ko, interleaved=inter, dq=dq, dk=dk, dq_weight=dw[0], dk_weight=dw[1])
     a, b, only = pools(), pools(), pools()
-    kvcache.write(ko, v, *a, slots)
-    kvcache.write(ko, None, *only[:2], None, None, slots)
+    kvcache.write(ko, v, *a, slots, format=fmt)
+    kvcache.write(ko, None, *only[:2], None, None, slots, format=fmt)
     q2 = torch.zeros_like(q)
-    kvcache.norm_rotate_write(q, k, v, qw, kw, cos, sin, pos, *b, slots, interleaved=inter, q_out=q2)
+    kvcache.norm_rotate_write(q, k, v, qw, kw, cos, sin, pos, *b, slots, interleaved=inter, format=fmt, q_out=q2)
     table = torch.arange(6, dtype=torch.int32, device="cuda").view(2, 3) % 5
     out = [torch.zeros(80, 2, d, dtype=q.dtype, device="cuda") for d in (64, 96)]
-    kvcache.read(*b, table, torch.tensor([0, 30, 77], dtype=torch.int32, device="cuda"), *out)
+    kvcache.read(*b, table, torch.tensor([0, 30, 77], dtype=torch.int32, device="cuda"), *out, format=fmt)
     results = [qo, ko, dq, dk, *[w for w in dw if w is not None], q2, *a, *b, *only, *out]
     return [r.view(torch.uint8) if r.element_size() == 1 else r for r in results]
 
 
-@pytest.mark.parametrize("dtype,wdtype,inter,scale", [("bfloat16", "float32", False, "f32"), ("float16", None, True, "e8m0"),
-                                                      ("float32", "float32", True, "f32")])
-def test_same_results_as_the_python_code(made, monkeypatch, dtype, wdtype, inter, scale):
-    got = everything(dtype, wdtype, inter, 1, scale)
+@pytest.mark.parametrize("dtype,wdtype,inter,scale,fmt", [
+    ("bfloat16", "float32", False, "f32", None), ("float16", None, True, "e8m0", None), ("float32", "float32", True, "f32", None),
+    ("bfloat16", "bfloat16", False, "e8m0", "e5m2"), ("float32", None, False, "f32", "e4m3")])
+def test_same_results_as_the_python_code(made, monkeypatch, dtype, wdtype, inter, scale, fmt):
+    got = everything(dtype, wdtype, inter, 1, scale, fmt)
     assert [name for name, status in made if status == 0] == ["norm_rotate", "norm_rotate_backward", "cache_write",
                                                               "cache_write", "norm_rotate_write", "cache_read"]
     slow(monkeypatch)
-    for a, b in zip(got, everything(dtype, wdtype, inter, 1, scale)):
+    for a, b in zip(got, everything(dtype, wdtype, inter, 1, scale, fmt)):
         assert torch.equal(a, b)
 
 
@@ -132,7 +134,9 @@ def test_wrong_arguments_raise_what_the_python_code_raises(made):
             (ValueError, (x, None, codes, scales.repeat(1, 1, 1, 3), None, None, slots)), (ValueError, (x, None, codes[:2], scales, None, None, slots)),
             (ValueError, (x, x, codes, scales, codes[:2], scales[:2], slots)), (ValueError, (x, x[:2], codes, scales, codes, scales, slots)),
             (ValueError, (x, None, codes, scales.repeat(1, 1, 1, 4), None, None, slots)),          # blocks of 8 items
-            (TypeError, (x, x, codes, scales, codes.view(torch.uint8).view(torch.float8_e5m2), scales, slots))):
+            (TypeError, (x, x, codes, scales, codes.view(torch.uint8).view(torch.float8_e5m2), scales, slots)),
+            (TypeError, (x, None, codes, scales, None, None, slots, "e5m2")), (ValueError, (x, None, codes, scales, None, None, slots, "bf16")),
+            (TypeError, (x, x, codes, scales, codes, scales.to(torch.uint8), slots))):
         with pytest.raises(error):
             kvcache.write(*args)
     for error, args in (
