@@ -479,8 +479,8 @@ void set_rotation(Params &p, const b2k_rotation &rot);
 int widest(const Params &p, int which, int64_t format, const b2k_rotation *rot);
 // Lanes and unit layout of every role for chunks of `vec` items, or fewer.
 Plan lay_out(Params &p, int vec, const b2k_rotation *rot);
-// Items with up to `most` heads in each, and blocks of `threads` threads, of every role; an
-// error when they do not fit 31 bits.
-int count_items(Params &p, int most, int threads, const char *name);
+// Items with up to `most` heads in each, fewer where `busy` threads an SM would not have
+// work, and blocks of every role; an error when they do not fit 31 bits.
+int count_items(Params &p, int most, int busy, const char *name);
 
 }  // namespace headwise

@@ -243,9 +243,14 @@ void pick_forward(const Params &p, const Plan &plan, unsigned blocks, cudaStream
 #undef B2K_HEADS_CASE
 }
 
+// 1024 tokens x 40 heads of 128 bf16 items: 6.8 us, with 256 8.0, with 1024 8.3, with 2048
+// 12.4; 2048 tokens: 9.5, 11.3, 10.5, 12.8.
+constexpr int kForwardBusy = 512;
+
 // Roles whose sizes or strides allow different chunks get launches of their own when they
-// hold at least this many items together: a launch costs some 2.5 us of the host, single
-// items instead of chunks of 8 about 3 us for 2^20 items.
+// hold at least this many items together.  Cache write, 8 heads of 128 bf16 items for keys
+// and of 33 for values, in one launch and in two: 1.0 million items 8.3 and 10.4 us, 2.1
+// million 12.4 and 11.4, 7.7 million 30.9 and 20.5.
 constexpr int64_t kItemsToSplit = int64_t(1) << 20;
 
 // Launches over all items; the roles, tokens and tables of `p` are set.
@@ -270,7 +275,7 @@ int launch_forward(const Params &all, int64_t format, const b2k_rotation *rot, c
             if (split && vec[i] != width) p.role[i].heads = 0;
         const Plan plan = lay_out(p, width, rot);
         if (plan.iter == 0) return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: no kernel for this head size", name);
-        if (int rc = count_items(p, kHeadsPerItem, kThreads, name)) return rc;
+        if (int rc = count_items(p, kHeadsPerItem, kForwardBusy, name)) return rc;
         const unsigned blocks = p.role[0].blocks + p.role[1].blocks + p.role[2].blocks;
         if (format == B2K_FMT_F32) pick_forward<float, MODE>(p, plan, blocks, stream);
         else if (format == B2K_FMT_F16) pick_forward<__half, MODE>(p, plan, blocks, stream);

@@ -9,6 +9,8 @@
 // (8 + 8) heads of 128 bf16 items 40 us = 5.1 TB/s (issue slots 67% busy), about what a
 // plain copy of those bytes takes; with norm, rotation and 64 query heads beside it, 8192
 // tokens 63 us.
+#include <algorithm>
+
 #include "b2k_heads_forward.cuh"
 
 namespace {
@@ -203,6 +205,16 @@ void pick_read(const ReadParams &p, int cv, dim3 grid, cudaStream_t stream) {
     launch_read<T, 1>(p, grid, stream);
 }
 
+// Rows a block owns: smaller tiles where whole ones would leave SMs without a block (400
+// rows of 8 heads of 128 items: 41 us with tiles of 32, 10.4 us so), or where a row is long
+// work (16384 rows of 32 heads of 128 items: 81 us with tiles of 32, 70 us so; 6000 rows of 8
+// heads of 33 items beside 128: 24.7 and 18.6).
+int tile_rows(int64_t rows, int64_t chunks) {
+    int tile = kTileRows;
+    while (tile > 4 && (rows / tile < b2k::sm_count() || tile * chunks > 2048)) tile /= 2;
+    return tile;
+}
+
 int check_slots(const void *slots, int slot_bytes, int64_t tokens, const char *name) {
     return tokens ? check_indices(slots, slot_bytes, name, "slots") : B2K_OK;
 }
@@ -314,11 +326,6 @@ int b2k_cache_read(const b2k_cache *cache, int format, int64_t rows, const b2k_h
     p.offset_bytes = offset_bytes;
     p.e5m2 = cache->code_format == B2K_FMT_E5M2;
     p.e8m0 = cache->scale_format == B2K_FMT_E8M0;
-    // smaller tiles where whole ones would leave SMs without a block
-    p.tile = kTileRows;
-    while (p.tile > 4 && rows / p.tile < b2k::sm_count()) p.tile /= 2;
-    const int64_t blocks = (rows + p.tile - 1) / p.tile;
-    if (blocks > INT_MAX) return b2k::fail(B2K_ERR_TOO_LARGE, "%s: too many rows for one launch", name);
     const cudaStream_t st = b2k::as_stream(stream);
     int sides = 0, cv[2] = {};
     double items = 0;
@@ -333,7 +340,14 @@ int b2k_cache_read(const b2k_cache *cache, int format, int64_t rows, const b2k_h
     if (sides == 2 && !split) cv[0] = cv[0] < cv[1] ? cv[0] : cv[1];
     for (int i = 0; i < (split ? 2 : 1); ++i) {
         if (i) p.side[0] = p.side[1];
-        const dim3 grid(static_cast<unsigned>(blocks), split ? 1 : sides);
+        const int here = split ? 1 : sides;
+        int64_t chunks = 0;                                // of a row
+        for (int k = 0; k < here; ++k)
+            chunks = std::max<int64_t>(chunks, static_cast<int64_t>(p.side[k].heads) * p.side[k].dim / cv[i]);
+        p.tile = tile_rows(rows, chunks);
+        const int64_t blocks = (rows + p.tile - 1) / p.tile;
+        if (blocks > INT_MAX) return b2k::fail(B2K_ERR_TOO_LARGE, "%s: too many rows for one launch", name);
+        const dim3 grid(static_cast<unsigned>(blocks), here);
         if (format == B2K_FMT_F32) pick_read<float>(p, cv[i], grid, st);
         else if (format == B2K_FMT_F16) pick_read<__half>(p, cv[i], grid, st);
         else pick_read<__nv_bfloat16>(p, cv[i], grid, st);
