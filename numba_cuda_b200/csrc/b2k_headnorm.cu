@@ -645,40 +645,37 @@ __device__ __forceinline__ void backward_rows_ahead(const Params &p, const Role 
         for (int h = 0; h < hpi; ++h) {
             wait_copies<kStages - 2>();
             // read again for every row: 16 registers less
-            float c[1][VEC] = {}, s[1][VEC] = {};
-            {
-                const char *angles = table_slot + table * 4 * kThreads * Slots::half;
-                float lo[H], hi[H];
-                if (turned.lo) {
-                    load_floats<H>(reinterpret_cast<const float *>(angles), lo);
-                    load_floats<H>(reinterpret_cast<const float *>(angles + 2 * kThreads * Slots::half), hi);
+            float c[1][VEC], s[1][VEC];
+            const char *angles = table_slot + table * 4 * kThreads * Slots::half;
 #pragma unroll
-                    for (int j = 0; j < H; ++j) {
-                        c[0][j] = lo[j];
-                        s[0][j] = hi[j];
-                    }
-                }
-                if (turned.hi) {
-                    load_floats<H>(reinterpret_cast<const float *>(angles + kThreads * Slots::half), lo);
-                    load_floats<H>(reinterpret_cast<const float *>(angles + 3 * kThreads * Slots::half), hi);
+            for (int part = 0; part < 2; ++part) {
+                float cc[H], ss[H];
+                load_floats<H>(reinterpret_cast<const float *>(angles + part * kThreads * Slots::half), cc);
+                load_floats<H>(reinterpret_cast<const float *>(angles + (2 + part) * kThreads * Slots::half), ss);
 #pragma unroll
-                    for (int j = 0; j < H; ++j) {
-                        c[0][H + j] = lo[j];
-                        s[0][H + j] = hi[j];
-                    }
+                for (int i = 0; i < H; ++i) {
+                    c[0][part * H + i] = cc[i];
+                    s[0][part * H + i] = ss[i];
                 }
             }
             const T *from = reinterpret_cast<const T *>(row_slot + stage * 4 * kThreads * 16);
             constexpr int next = kThreads * 16 / sizeof(T);
             const bool there = h < rows;
-            Chunk<T, VEC> xa[1] = {}, xb[1] = {}, da[1] = {}, db[1] = {};
-            if (there && !padding && has_a) {
-                xa[0] = load_chunk<T, VEC>(from);
-                da[0] = load_chunk<T, VEC>(from + 2 * next);
-            }
-            if (there && !padding && has_b) {
-                xb[0] = load_chunk<T, VEC>(from + next);
-                db[0] = load_chunk<T, VEC>(from + 3 * next);
+            Chunk<T, VEC> xa[1], xb[1], da[1], db[1];
+            xa[0] = load_chunk<T, VEC>(from);
+            xb[0] = load_chunk<T, VEC>(from + next);
+            da[0] = load_chunk<T, VEC>(from + 2 * next);
+            db[0] = load_chunk<T, VEC>(from + 3 * next);
+            // What no copy has filled, angles too, holds anything: zeros instead.  One vote for
+            // the common row, where there is nothing of the kind, in place of a select for
+            // every register.
+            const bool row = there && !padding;
+            if (__any_sync(0xFFFFFFFFu, !(row && has_a && has_b))) {
+                if (!(row && has_a)) xa[0] = da[0] = Chunk<T, VEC>{};
+                if (!(row && has_b)) xb[0] = db[0] = Chunk<T, VEC>{};
+                if (!row)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) c[0][j] = s[0][j] = 0.0f;
             }
             load_step();                     // into the slot that the step before this one read
             gradient_row<T, VEC, 1, INTER>(p, r, g, oa, ob, xa, xb, da, db, c, s, w, out, padding, there);

@@ -236,6 +236,32 @@ def test_padding_tokens(index):
     assert not f64(dq.as_torch()).any() and not f64(dqw.as_torch()).any()
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_rows_that_are_not_there_add_nothing_whatever_shared_memory_holds(dtype):
+    """A call whose tables are NaN leaves NaNs in shared memory; padding tokens and the empty
+    places behind the last item of the next call must not pick them up."""
+    tokens = 4001
+    _, q, k, qw, kw, cos, sin, _ = setup(tokens, 16, 8, 64, 64, dtype, "contiguous", "float32", 0)
+    bad = torch.full_like(cos, float("nan"))
+    pos = torch.randint(0, 61, (tokens,), device="cuda")
+    for every in (1, 2, 3):
+        some = pos.clone()
+        some[::every] = -1
+        valid = (some >= 0).cpu()
+        headnorm.norm_rotate_backward(q, k, qw, kw, bad, bad, pos, q, k)
+        got = [g.as_torch() for g in headnorm.norm_rotate_backward(q, k, qw, kw, cos, sin, some, q, k)]
+        want = [g.as_torch() for g in headnorm.norm_rotate_backward(q[valid], k[valid], qw, kw, cos, sin, some[valid.cuda()], q[valid], k[valid])]
+        for g, w in zip(got[:2], want[:2]):
+            assert torch.equal(g[valid], w) and not g[~valid].any()
+        for g, w in zip(got[2:], want[2:]):
+            # the same rows in another order of addition: at most that many roundings
+            np.testing.assert_allclose(f64(g), f64(w), rtol=0, atol=tokens * 16 * 2 * U * float(w.abs().max() + 1))
+    headnorm.norm_rotate_backward(q, k, qw, kw, bad, bad, pos, q, k)
+    few = 33                                             # empty places in every role's last warp
+    got = headnorm.norm_rotate_backward(q[:few], k[:few], qw, kw, cos, sin, pos[:few], q[:few], k[:few])
+    assert all(torch.isfinite(g.as_torch()).all() for g in got)
+
+
 def test_no_tokens():
     _, q, k, qw, kw, cos, sin, pos = setup(4, 2, 2, 64, 64, "float32", "contiguous", "float32", 0)
     qo, ko = headnorm.norm_rotate(q[:0], k[:0], qw, kw, cos, sin, pos[:0])
