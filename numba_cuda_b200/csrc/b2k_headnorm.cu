@@ -434,7 +434,7 @@ struct Weights {
 
 // The gradient of one row as loaded (x and g, two chunks a unit), stored to `out` if `there`.
 // A padding token's rows come as zeros.
-template <typename T, int VEC, int ITER, bool INTER>
+template <typename T, int VEC, int ITER, bool INTER, bool AHEAD>
 __device__ __forceinline__ void gradient_row(const Params &p, const Role &r, const Lanes &g, const int (&oa)[ITER],
                                              const int (&ob)[ITER], const Chunk<T, VEC> (&xa)[ITER],
                                              const Chunk<T, VEC> (&xb)[ITER], const Chunk<T, VEC> (&da)[ITER],
@@ -462,7 +462,22 @@ __device__ __forceinline__ void gradient_row(const Params &p, const Role &r, con
         // dx = r (h - n mean(h n)) with n = x r:  r h - x (r^3 sum(h x) / dim)
         const float mean = g.sum(ss.x + ss.y) * r.inv_dim;
         const float by = padding || !there ? 0.0f : rsqrtf(mean + p.eps);       // eps may be zero
-        const float pull = g.sum(dot.x + dot.y) * r.inv_dim * by * by * by;
+        float pull = g.sum(dot.x + dot.y) * r.inv_dim * by * by * by;
+        // Squares beyond float32: the result is zeros, and so is the gradient; but the sum of h x can
+        // have passed the range too, and infinity times zero is no zero.  What is infinite or a NaN
+        // itself still makes the row NaNs.  A group alone takes this branch where copies run ahead
+        // (32768 tokens x 40 heads of 128 bf16 items: 170 us, with a vote of the warp 180), a warp
+        // where registers are short (32 + 2 heads: 192 us, 217 for a group alone, which spills).
+        const bool beyond = mean > FLT_MAX;
+        if (AHEAD ? beyond : __any_sync(0xFFFFFFFFu, beyond)) {
+            float none = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ITER; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) none += x[i][j] * 0.0f + y[i][j] * 0.0f;
+            none = AHEAD ? g.sum_alone(none) : g.sum(none);
+            if (beyond) pull = none;
+        }
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             gradient_of<VEC>(x[i], gx[i], w.x[i], by, pull, w.sum_x[i]);
@@ -522,7 +537,7 @@ __device__ __forceinline__ void backward_rows(const Params &p, const Role &r, co
             it.grad += r.grad_head;
             x_next.load(it.in, 0, loads - h - 1, oa, ob, r.dim);
             g_next.load(it.grad, 0, loads - h - 1, oa, ob, r.dim);
-            gradient_row<T, VEC, ITER, INTER>(p, r, g, oa, ob, x_now.a[0], x_now.b[0], g_now.a[0], g_now.b[0], c, s, w, it.out, padding,
+            gradient_row<T, VEC, ITER, INTER, false>(p, r, g, oa, ob, x_now.a[0], x_now.b[0], g_now.a[0], g_now.b[0], c, s, w, it.out, padding,
                                        h < it.rows);
             it.out += r.out_head;
             x_now = x_next;
@@ -678,7 +693,7 @@ __device__ __forceinline__ void backward_rows_ahead(const Params &p, const Role 
                     for (int j = 0; j < VEC; ++j) c[0][j] = s[0][j] = 0.0f;
             }
             load_step();                     // into the slot that the step before this one read
-            gradient_row<T, VEC, 1, INTER>(p, r, g, oa, ob, xa, xb, da, db, c, s, w, out, padding, there);
+            gradient_row<T, VEC, 1, INTER, true>(p, r, g, oa, ob, xa, xb, da, db, c, s, w, out, padding, there);
             out += r.out_head;
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }

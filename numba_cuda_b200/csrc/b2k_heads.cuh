@@ -197,6 +197,12 @@ struct Lanes {
             if (o < n) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
         return v;
     }
+    // for a group that is alone in a branch
+    __device__ float sum_alone(float v) const {
+        const unsigned group = (0xFFFFFFFFu >> (32 - n)) << (threadIdx.x & 31 & ~(n - 1));
+        for (int o = n / 2; o > 0; o >>= 1) v += __shfl_xor_sync(group, v, o);
+        return v;
+    }
     // over aligned runs of `span` lanes (a power of two) of the group
     __device__ float max(float v, int span) const {
 #pragma unroll

@@ -4,8 +4,9 @@ import pytest
 import torch
 
 import headwise_ref as ref
+from headwise_plan import Plan
 from numba_cuda_b200.kernels import headnorm, kvcache
-from test_headnorm_gpu import TORCH, angles, check, f64, setup
+from test_headnorm_gpu import TORCH, angles, check, f64, layout, setup
 from test_kvcache_gpu import pool
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +45,44 @@ def test_squares_beyond_float32_give_zeros(dtype, dim, rot, inter):
                               interleaved=inter)
     for t, h in rows:
         assert not (codes.flatten(0, 1)[t, h] & 0x7F).any() and (scales.flatten(0, 1)[t, h] == 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("dtype,dim,rot,inter", LARGE)
+def test_gradient_of_squares_beyond_float32_is_zero(dtype, dim, rot, inter):
+    """The result is zeros whatever the items are, so is its gradient; an infinity or a NaN still shows."""
+    rng, q, qw, cos, sin, pos, rows = large(dtype, dim, rot, "backward")
+    g = layout(tuple(q.shape), "contiguous", dtype, rng, 3.0)
+    dq, _, dw, _ = headnorm.norm_rotate_backward(q, None, qw, None, cos, sin, pos, g, None, interleaved=inter)
+    dq = dq.as_torch()
+    there = q.clone()
+    for t, h in rows:
+        assert not dq[t, h].any()
+        there[t, h] = 0.0
+        g[t, h] = 0.0
+    want = headnorm.norm_rotate_backward(there, None, qw, None, cos, sin, pos, g, None, interleaved=inter)
+    assert torch.equal(dq, want[0].as_torch()) and torch.equal(dw.as_torch(), want[2].as_torch())
+    q[2, 1, 1] = float("inf")
+    dq = headnorm.norm_rotate_backward(q, None, qw, None, cos, sin, pos, torch.ones_like(g), None, interleaved=inter)[0].as_torch()
+    assert dq[2, 1].isnan().all() and not dq[4, 2].any()
+
+
+@pytest.mark.parametrize("dtype,dim,rot,inter", [("bfloat16", 128, 128, False), ("bfloat16", 80, 40, True), ("float32", 64, 32, False)])
+def test_gradient_of_squares_beyond_float32_with_copies_ahead(dtype, dim, rot, inter):
+    """Groups of one warp of which some have such a head and others not."""
+    tokens, heads = 5001, 16
+    assert Plan(dtype, tokens, (heads,), (dim,), (rot,), inter, backward=True).ahead
+    rng, q, _, qw, _, cos, sin, pos = setup(tokens, heads, 1, dim, rot, dtype, "contiguous", "float32", 1)
+    g = layout(tuple(q.shape), "contiguous", dtype, rng, 3.0)
+    t, h = (torch.tensor(rng.integers(0, n, 3000), device="cuda") for n in (tokens, heads))
+    there, there_g = q.clone(), g.clone()
+    q[t, h] = torch.finfo(TORCH[dtype]).max * 0.99
+    there[t, h], there_g[t, h] = 0.0, 0.0
+    got = headnorm.norm_rotate_backward(q, None, qw, None, cos, sin, pos, g, None, interleaved=inter)
+    want = headnorm.norm_rotate_backward(there, None, qw, None, cos, sin, pos, there_g, None, interleaved=inter)
+    assert torch.equal(got[0].as_torch(), want[0].as_torch()) and torch.equal(got[2].as_torch(), want[2].as_torch())
+    assert not got[0].as_torch()[t, h].any()
+    q[t[0], h[0], 1] = float("-inf")
+    dq = headnorm.norm_rotate_backward(q, None, qw, None, cos, sin, pos, g, None, interleaved=inter)[0].as_torch()
+    assert dq[t[0], h[0]].isnan().all()
+    dq[t[0], h[0]] = 0.0
+    assert torch.equal(dq, want[0].as_torch())
