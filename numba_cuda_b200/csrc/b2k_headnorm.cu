@@ -488,8 +488,16 @@ __device__ __forceinline__ void gradient_row(const Params &p, const Role &r, con
     for (int i = 0; i < ITER; ++i) {
         float a[VEC], b[VEC];
         out_of_pairs<VEC, INTER>(gx[i], gy[i], a, b);
-        if (there && oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a);
-        if (there && ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b);
+        if (there && !padding && oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a);
+        if (there && !padding && ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b);
+    }
+    if (there && padding) {                 // not computed: a weight's infinity times zero is no zero
+        const float zeros[VEC] = {};
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            if (oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], zeros);
+            if (ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], zeros);
+        }
     }
 }
 

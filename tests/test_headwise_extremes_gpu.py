@@ -86,3 +86,18 @@ def test_gradient_of_squares_beyond_float32_with_copies_ahead(dtype, dim, rot, i
     assert dq[t[0], h[0]].isnan().all()
     dq[t[0], h[0]] = 0.0
     assert torch.equal(dq, want[0].as_torch())
+
+
+@pytest.mark.parametrize("dtype,tokens,qh,kh,dim,rot,inter", [
+    ("bfloat16", 4001, 16, 8, 128, 128, False), ("float32", 4001, 16, 8, 64, 32, True),          # with copies ahead
+    ("bfloat16", 40, 4, 2, 128, 128, False), ("float32", 40, 4, 2, 33, 10, True), ("float16", 40, 4, 2, 576, 64, False)])
+def test_padding_tokens_have_zero_gradients_whatever_the_weight(dtype, tokens, qh, kh, dim, rot, inter):
+    assert Plan(dtype, tokens, (qh, kh), (dim, dim), (rot, rot), inter, backward=True).ahead == (tokens > 4000)
+    rng, q, k, qw, kw, cos, sin, pos = setup(tokens, qh, kh, dim, rot, dtype, "contiguous", "float32", 1)
+    qw[dim - 1], kw[0] = float("nan"), float("inf")
+    pos[::3] = -1
+    pos[1] = 61
+    padding = ((pos < 0) | (pos >= 61)).cpu()
+    dq, dk, dqw, dkw = [g.as_torch() for g in headnorm.norm_rotate_backward(q, k, qw, kw, cos, sin, pos, q, k, interleaved=inter)]
+    assert not dq[padding].any() and not dk[padding].any()
+    assert torch.isfinite(dqw).all() and torch.isfinite(dkw).all()         # the weight itself is no part of its gradient
