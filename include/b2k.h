@@ -368,9 +368,9 @@ typedef struct b2k_heads {
  *                angle whose cosine and sine stand in row positions[token], column i of
  *                cos_dev and sin_dev (float32, `positions` rows of rotary_dim / 2 items,
  *                row strides in items)
- *   positions  : one index per token.  A token whose position is outside
- *                [0, table_rows) is padding: the forward calls leave its rows as they
- *                were, the backward call writes zeros. */
+ *   positions  : one index per token; may be NULL when rotary_dim = 0.  A token whose
+ *                position is outside [0, table_rows) is padding: the forward calls leave
+ *                its rows as they were, the backward call writes zeros. */
 typedef struct b2k_rotation {
     int64_t format, tokens;
     b2k_heads q, k;

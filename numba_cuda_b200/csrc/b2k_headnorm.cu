@@ -88,6 +88,9 @@ int check_indices(const void *p, int64_t bytes, const char *name, const char *wh
     return B2K_OK;
 }
 
+// Positions tell padding tokens even where nothing is rotated.
+static bool has_positions(const b2k_rotation &r) { return r.rotary_dim > 0 || r.positions_dev != nullptr; }
+
 int check_rotation(const b2k_rotation *r, const char *name) {
     if (r == nullptr) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: null arguments", name);
     if (int rc = check_tokens(r->format, r->tokens, name)) return rc;
@@ -112,15 +115,18 @@ int check_rotation(const b2k_rotation *r, const char *name) {
         for (const b2k_heads *h : {&r->q, &r->k})
             if (h->heads && r->rotary_dim > h->dim)
                 return b2k::fail(B2K_ERR_INVALID_ARG, "%s: rotary_dim is larger than a head", name);
-        if (r->table_rows < 0) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: negative table_rows", name);
         if (r->tokens > 0) {
             if (r->table_rows > 0 && (r->cos_dev == nullptr || r->sin_dev == nullptr))
                 return b2k::fail(B2K_ERR_INVALID_ARG, "%s: cos or sin is a null pointer", name);
             for (const void *t : {r->cos_dev, r->sin_dev})
                 if (reinterpret_cast<uintptr_t>(t) % 4)
                     return b2k::fail(B2K_ERR_ALIGNMENT, "%s: cos or sin is not aligned to its items", name);
-            if (int rc = check_indices(r->positions_dev, r->position_bytes, name, "positions")) return rc;
         }
+    }
+    if (has_positions(*r)) {
+        if (r->table_rows < 0) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: negative table_rows", name);
+        if (r->tokens > 0)
+            if (int rc = check_indices(r->positions_dev, r->position_bytes, name, "positions")) return rc;
     }
     return B2K_OK;
 }
@@ -209,6 +215,8 @@ void set_rotation(Params &p, const b2k_rotation &rot) {
         p.sin_table = rot.sin_dev;
         p.cos_stride = rot.table_rows > 1 ? rot.cos_stride : 0;
         p.sin_stride = rot.table_rows > 1 ? rot.sin_stride : 0;
+    }
+    if (has_positions(rot)) {
         p.table_rows = rot.table_rows;
         p.positions = rot.positions_dev;
         p.position_bytes = static_cast<int>(rot.position_bytes);

@@ -101,3 +101,29 @@ def test_padding_tokens_have_zero_gradients_whatever_the_weight(dtype, tokens, q
     dq, dk, dqw, dkw = [g.as_torch() for g in headnorm.norm_rotate_backward(q, k, qw, kw, cos, sin, pos, q, k, interleaved=inter)]
     assert not dq[padding].any() and not dk[padding].any()
     assert torch.isfinite(dqw).all() and torch.isfinite(dkw).all()         # the weight itself is no part of its gradient
+
+
+@pytest.mark.parametrize("dim", [64, 33])
+def test_tables_without_columns_still_tell_padding(dim):
+    """Nothing is rotated, and a token whose position is no row of the tables is padding."""
+    rng, q, k, qw, kw, _, _, _ = setup(6, 2, 2, dim, 0, "float32", "contiguous", "float32", 1)
+    empty = torch.zeros(5, 0, device="cuda")
+    pos = torch.tensor([0, -1, 4, 5, 2, 2 ** 40], device="cuda")
+    valid = torch.tensor([True, False, True, False, True, False])
+    qo = torch.full_like(q, 7.0)
+    headnorm.norm_rotate(q, None, qw, None, empty, empty, pos, q_out=qo)
+    assert (qo[~valid] == 7.0).all()
+    check(qo[valid], *ref.norm_rotate(f64(q[valid]), f64(qw), None, None, 1e-6, False, True), "float32")
+    dq, _, dw, _ = headnorm.norm_rotate_backward(q, None, qw, None, empty, empty, pos, q, None)
+    dx, size, dsum, dsize = ref.norm_rotate_backward(f64(q[valid]), f64(qw), None, None, f64(q[valid]), 1e-6, False, True)
+    check(dq.as_torch()[valid], dx, size, "float32", 128)
+    assert not dq.as_torch()[~valid].any()
+    check(dw.as_torch(), dsum, dsize, "float32", 64 + 12)
+    codes, scales = pool(2, 4, 2, dim, dim, "e4m3", "f32", rng)
+    before = codes.clone()
+    kvcache.norm_rotate_write(None, k, None, None, kw, empty, empty, pos, codes, scales, None, None, torch.arange(6, device="cuda"))
+    assert torch.equal(codes.flatten(0, 1)[1::2][:3], before.flatten(0, 1)[1::2][:3])
+    # tables without rows: padding only
+    qo.fill_(7.0)
+    headnorm.norm_rotate(q, None, qw, None, empty[:0], empty[:0], pos, q_out=qo)
+    assert (qo == 7.0).all()
