@@ -333,7 +333,7 @@ int count_items(Params &p, int most, int busy, const char *name) {
     const int64_t in_block = kThreads / p.lanes;
     int64_t blocks = 0;
     for (Role &r : p.role) {
-        const int64_t per_token = (r.heads + most - 1) / most;
+        const int64_t per_token = (static_cast<int64_t>(r.heads) + most - 1) / most;
         r.heads_per_item = per_token ? static_cast<int>((r.heads + per_token - 1) / per_token) : 1;      // even shares
         if (per_token && p.tokens > INT_MAX / per_token)
             return b2k::fail(B2K_ERR_TOO_LARGE, "%s: more than 2^31 - 1 groups of rows", name);

@@ -338,6 +338,10 @@ int b2k_cache_read(const b2k_cache *cache, int format, int64_t rows, const b2k_h
     // sides of different chunks: as in launch_forward
     const bool split = sides == 2 && cv[0] != cv[1] && items >= kItemsToSplit;
     if (sides == 2 && !split) cv[0] = cv[0] < cv[1] ? cv[0] : cv[1];
+    // a thread's chunk number stays an int one step past the last chunk of a row
+    for (int i = 0; i < sides; ++i)
+        if (static_cast<int64_t>(p.side[i].heads) * p.side[i].dim / cv[split ? i : 0] > INT_MAX - kThreads)
+            return b2k::fail(B2K_ERR_TOO_LARGE, "%s: a row has more than 2^31 - %d chunks", name, kThreads + 1);
     for (int i = 0; i < (split ? 2 : 1); ++i) {
         if (i) p.side[0] = p.side[1];
         const int here = split ? 1 : sides;

@@ -1,6 +1,7 @@
 """Head-wise calls at the edges of their arguments, without a GPU."""
 from numba_cuda_b200 import _lib
-from test_headwise_host import _heads, _rotation
+from numba_cuda_b200.kernels import _operands as ops
+from test_headwise_host import _cache, _heads, _rotation
 
 
 def test_positions_are_checked_where_nothing_is_rotated():
@@ -14,3 +15,16 @@ def test_positions_are_checked_where_nothing_is_rotated():
     assert call(pb=2) == _lib.ERR_INVALID_ARG
     assert call(rows=-1) == _lib.ERR_INVALID_ARG
     assert call(tokens=0, pos=0, pb=0) == 0
+
+
+def test_rows_whose_last_chunk_has_no_successor_in_32_bits():
+    """A thread of the cache read counts a row's chunks in steps of a block's threads."""
+    L = _lib.lib()
+    heads, dim = 2099202, 1023                                  # 2^31 - 2 single items
+    side = (4096, 0, 0, dim, 8192, 0, 0, 1, heads, dim, dim)
+    out = ops.HEADS.pack(4096, heads * dim, dim, heads, dim)
+    for k, v in ((1, 0), (0, 1)):
+        cache = _cache(pages=1, size=1, k=side if k else (0,) * 11, v=side if v else (0,) * 11)
+        got = L.b2k_cache_read(cache, _lib.FMT_F16, 1, out if k else ops.NO_HEADS, out if v else ops.NO_HEADS, 4096, 1, 1, 4,
+                               4096, 1, 4, None)
+        assert got == _lib.ERR_TOO_LARGE
