@@ -212,8 +212,9 @@ bool read_rotation(PyObject *const *args, PyObject *eps, PyObject *interleaved, 
     return true;
 }
 
-// k_codes, k_scales, v_codes, v_scales of args[0..4); the codes' types or `format` tell what they are
-bool read_cache(PyObject *const *args, PyObject *format, int device, b2k_cache &c) {
+// k_codes, k_scales, v_codes, v_scales of args[0..4); the codes' types or `format` tell what they
+// are.  `given` says which sides are there.
+bool read_cache(PyObject *const *args, PyObject *format, int device, b2k_cache &c, bool (&given)[2]) {
     int code = -1;
     if (format != Py_None) {
         if (!PyUnicode_CheckExact(format)) return false;
@@ -226,7 +227,8 @@ bool read_cache(PyObject *const *args, PyObject *format, int device, b2k_cache &
     bool any = false;
     for (int i = 0; i < 2; ++i) {
         PyObject *codes = args[2 * i], *scales = args[2 * i + 1];
-        if (codes == Py_None && scales == Py_None) continue;
+        given[i] = codes != Py_None || scales != Py_None;
+        if (!given[i]) continue;
         Array a, s;
         if (!read(codes, device, a) || !read(scales, device, s) || a.ndim != 4 || s.ndim != 4) return false;
         if (a.format == B2K_FMT_E4M3 || a.format == B2K_FMT_E5M2) {
@@ -253,8 +255,9 @@ bool read_cache(PyObject *const *args, PyObject *format, int device, b2k_cache &
     return any;
 }
 
-bool fits(bool given, const b2k_heads &h, const b2k_pages &side) {
-    return given ? h.heads == side.heads && h.dim == side.dim && side.dim > 0 : side.codes_dev == nullptr && side.heads == 0;
+// An array and its side of the cache: both are there and alike, or neither is.
+bool fits(bool given, const b2k_heads &h, bool side_given, const b2k_pages &side) {
+    return given == side_given && (!given || (h.heads == side.heads && h.dim == side.dim && side.dim > 0));
 }
 
 bool read_stream(PyObject *o, void *&stream) {
@@ -345,13 +348,14 @@ PyObject *norm_rotate_backward(PyObject *, PyObject *const *args, Py_ssize_t n) 
 PyObject *cache_write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     int device;
     b2k_cache cache;
+    bool side[2];
     b2k_heads h[2] = {};
     Array a[2], at;
     void *stream;
-    if (!ready(n, 9, device) || !read_cache(args + 2, args[7], device, cache)) return pass();
+    if (!ready(n, 9, device) || !read_cache(args + 2, args[7], device, cache, side)) return pass();
     const bool has[2] = {args[0] != Py_None, args[1] != Py_None};
     for (int i = 0; i < 2; ++i)
-        if ((has[i] && !read_heads(args[i], device, a[i], h[i])) || !fits(has[i], h[i], i ? cache.v : cache.k)) return pass();
+        if ((has[i] && !read_heads(args[i], device, a[i], h[i])) || !fits(has[i], h[i], side[i], i ? cache.v : cache.k)) return pass();
     if (has[0] && has[1] && (a[0].size[0] != a[1].size[0] || a[0].format != a[1].format)) return pass();
     const Array &first = has[0] ? a[0] : a[1];
     if (!(has[0] || has[1]) || !read_vector(args[6], device, first.size[0], at) || !is_index(at.format) ||
@@ -365,13 +369,14 @@ PyObject *cache_write(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *cache_read(PyObject *, PyObject *const *args, Py_ssize_t n) {
     int device;
     b2k_cache cache;
+    bool side[2];
     b2k_heads h[2] = {};
     Array a[2], table, at;
     void *stream;
-    if (!ready(n, 10, device) || !read_cache(args, args[8], device, cache)) return pass();
+    if (!ready(n, 10, device) || !read_cache(args, args[8], device, cache, side)) return pass();
     const bool has[2] = {args[6] != Py_None, args[7] != Py_None};
     for (int i = 0; i < 2; ++i)
-        if ((has[i] && !read_heads(args[6 + i], device, a[i], h[i])) || !fits(has[i], h[i], i ? cache.v : cache.k)) return pass();
+        if ((has[i] && !read_heads(args[6 + i], device, a[i], h[i])) || !fits(has[i], h[i], side[i], i ? cache.v : cache.k)) return pass();
     if (has[0] && has[1] && (a[0].size[0] != a[1].size[0] || a[0].format != a[1].format)) return pass();
     const Array &first = has[0] ? a[0] : a[1];
     if (!(has[0] || has[1]) || !read(args[4], device, table) || table.ndim != 2 || !is_index(table.format) ||
@@ -389,15 +394,16 @@ PyObject *norm_rotate_write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     int device;
     Rotation t;
     b2k_cache cache;
+    bool side[2];
     b2k_heads v{}, q_out;
     Array av, at;
     void *stream;
     if (!ready(n, 19, device) || !read_rotation(args, args[13], args[14], args[15], device, t) ||
-        !read_cache(args + 8, args[16], device, cache) || !read_result(args[17], t.has_q, t.q, device, q_out))
+        !read_cache(args + 8, args[16], device, cache, side) || !read_result(args[17], t.has_q, t.q, device, q_out))
         return pass();
     const bool has_v = args[7] != Py_None;
     if (has_v && (!read_heads(args[7], device, av, v) || av.size[0] != t.r.tokens || av.format != t.r.format)) return pass();
-    if (!fits(t.has_k, t.r.k, cache.k) || !fits(has_v, v, cache.v) || !read_vector(args[12], device, t.r.tokens, at) ||
+    if (!fits(t.has_k, t.r.k, side[0], cache.k) || !fits(has_v, v, side[1], cache.v) || !read_vector(args[12], device, t.r.tokens, at) ||
         !is_index(at.format) || !read_stream(args[18], stream))
         return pass();
     return PyLong_FromLong(g_call.norm_rotate_write(&t.r, &v, &q_out, &cache, at.data, index_bytes(at), stream));
