@@ -283,6 +283,16 @@ bool ready(Py_ssize_t given, Py_ssize_t wanted, int &device) {
     return device >= 0;
 }
 
+// Makes the call `f` without the interpreter lock: a launch waits when the GPU's queue is full.  The
+// arguments are held by the caller of the entry point meanwhile.
+template <typename F>
+int unlocked(F f) {
+    PyThreadState *state = PyEval_SaveThread();
+    const int status = f();
+    PyEval_RestoreThread(state);
+    return status;
+}
+
 // (q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, q_out, k_out, stream)
 PyObject *norm_rotate(PyObject *, PyObject *const *args, Py_ssize_t n) {
     int device;
@@ -293,7 +303,7 @@ PyObject *norm_rotate(PyObject *, PyObject *const *args, Py_ssize_t n) {
         !read_result(args[10], t.has_q, t.q, device, q_out) || !read_result(args[11], t.has_k, t.k, device, k_out) ||
         !read_stream(args[12], stream))
         return pass();
-    return PyLong_FromLong(g_call.norm_rotate(&t.r, &q_out, &k_out, stream));
+    return PyLong_FromLong(unlocked([&] { return g_call.norm_rotate(&t.r, &q_out, &k_out, stream); }));
 }
 
 // (q, k, q_weight, k_weight, cos, sin, positions, q_grad, k_grad, eps, interleaved, norm, dq, dk, dq_weight, dk_weight, stream)
@@ -338,8 +348,9 @@ PyObject *norm_rotate_backward(PyObject *, PyObject *const *args, Py_ssize_t n) 
         }
         scratch = scratch_of.data;
     }
-    const int status =
-        g_call.norm_rotate_backward(&t.r, &q_grad, &k_grad, &dq, &dk, sums[0], sums[1], scratch, bytes, stream);
+    const int status = unlocked([&] {
+        return g_call.norm_rotate_backward(&t.r, &q_grad, &k_grad, &dq, &dk, sums[0], sums[1], scratch, bytes, stream);
+    });
     Py_XDECREF(held);
     return PyLong_FromLong(status);
 }
@@ -361,8 +372,9 @@ PyObject *cache_write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (!(has[0] || has[1]) || !read_vector(args[6], device, first.size[0], at) || !is_index(at.format) ||
         !read_stream(args[8], stream))
         return pass();
-    return PyLong_FromLong(
-        g_call.cache_write(&cache, first.format, first.size[0], &h[0], &h[1], at.data, index_bytes(at), stream));
+    return PyLong_FromLong(unlocked([&] {
+        return g_call.cache_write(&cache, first.format, first.size[0], &h[0], &h[1], at.data, index_bytes(at), stream);
+    }));
 }
 
 // (k_codes, k_scales, v_codes, v_scales, page_table, offsets, k_out, v_out, format, stream)
@@ -383,9 +395,10 @@ PyObject *cache_read(PyObject *, PyObject *const *args, Py_ssize_t n) {
         (table.stride[1] != 1 && table.size[1] > 1) || !read_vector(args[5], device, table.size[0] + 1, at) ||
         !is_index(at.format) || !read_stream(args[9], stream))
         return pass();
-    return PyLong_FromLong(g_call.cache_read(&cache, first.format, first.size[0], &h[0], &h[1], table.data, table.stride[0],
-                                             table.size[1], index_bytes(table), at.data, table.size[0], index_bytes(at),
-                                             stream));
+    return PyLong_FromLong(unlocked([&] {
+        return g_call.cache_read(&cache, first.format, first.size[0], &h[0], &h[1], table.data, table.stride[0], table.size[1],
+                                 index_bytes(table), at.data, table.size[0], index_bytes(at), stream);
+    }));
 }
 
 // (q, k, q_weight, k_weight, cos, sin, positions, v, k_codes, k_scales, v_codes, v_scales, slots, eps, interleaved, norm,
@@ -406,7 +419,8 @@ PyObject *norm_rotate_write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (!fits(t.has_k, t.r.k, side[0], cache.k) || !fits(has_v, v, side[1], cache.v) || !read_vector(args[12], device, t.r.tokens, at) ||
         !is_index(at.format) || !read_stream(args[18], stream))
         return pass();
-    return PyLong_FromLong(g_call.norm_rotate_write(&t.r, &v, &q_out, &cache, at.data, index_bytes(at), stream));
+    return PyLong_FromLong(
+        unlocked([&] { return g_call.norm_rotate_write(&t.r, &v, &q_out, &cache, at.data, index_bytes(at), stream); }));
 }
 
 template <typename F>

@@ -86,3 +86,11 @@ def test_a_cache_without_its_array_is_left_to_the_python_code(tmp_path, name, ca
     assert getattr(fast, name)(*args) is None
     args[cache:cache + 2] = None, None
     assert getattr(fast, name)(*args) == 0
+
+
+@pytest.mark.parametrize("name", list(calls()))
+def test_the_interpreter_lock_is_free_during_a_call(tmp_path, name):
+    """A launch can wait for room in the GPU's queue.  The entry point here is the interpreter's own
+    question whether this thread holds the lock."""
+    fast = load(tmp_path, ctypes.pythonapi.PyGILState_Check)
+    assert getattr(fast, name)(*calls()[name]) == 0
