@@ -17,7 +17,7 @@
 namespace {
 
 // Set once by setup().
-PyObject *g_tensor_type, *g_formats, *g_stream_ptr, *g_workspace, *g_no_arguments;
+PyObject *g_tensor_type, *g_formats, *g_stream_ptr, *g_workspace, *g_forward_mode, *g_level, *g_no_arguments;
 
 // An attribute or a method without arguments of the tensor type.  Where it is implemented
 // in C, its function is called directly: looking six of them up for each of ten tensors
@@ -279,6 +279,9 @@ PyObject *pass() {                  // let the Python code look at it
 
 bool ready(Py_ssize_t given, Py_ssize_t wanted, int &device) {
     if (g_tensor_type == nullptr || given != wanted) return false;
+    // inside a level of forward differentiation a tensor may carry a tangent: the Python code looks
+    PyObject *level = PyDict_GetItemWithError(g_forward_mode, g_level);             // borrowed
+    if (level == nullptr || PyLong_AsLong(level) != -1 || PyErr_Occurred()) return false;
     device = g_call.current_device();
     return device >= 0;
 }
@@ -434,10 +437,11 @@ bool address(PyObject *dict, const char *name, F &f) {
     return !PyErr_Occurred();
 }
 
-// setup(tensor type, {dtype: format}, {entry point: address}, stream_ptr, workspace)
+// setup(tensor type, {dtype: format}, {entry point: address}, stream_ptr, workspace, names of torch.autograd.forward_ad)
 PyObject *setup(PyObject *, PyObject *args) {
-    PyObject *type, *formats, *addresses, *stream, *workspace;
-    if (!PyArg_ParseTuple(args, "OO!O!OO", &type, &PyDict_Type, &formats, &PyDict_Type, &addresses, &stream, &workspace))
+    PyObject *type, *formats, *addresses, *stream, *workspace, *forward;
+    if (!PyArg_ParseTuple(args, "OO!O!OOO!", &type, &PyDict_Type, &formats, &PyDict_Type, &addresses, &stream, &workspace,
+                          &PyDict_Type, &forward))
         return nullptr;
     Entry e;
     if (!address(addresses, "b2k_norm_rotate", e.norm_rotate) ||
@@ -456,6 +460,8 @@ PyObject *setup(PyObject *, PyObject *args) {
     Py_XSETREF(g_stream_ptr, stream);
     Py_INCREF(workspace);
     Py_XSETREF(g_workspace, workspace);
+    Py_INCREF(forward);
+    Py_XSETREF(g_forward_mode, forward);
     Py_INCREF(type);
     Py_XSETREF(g_tensor_type, type);
     Py_RETURN_NONE;
@@ -477,6 +483,7 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_pyfast", nullptr, -1, g_methods
 
 PyMODINIT_FUNC PyInit__pyfast(void) {
     g_no_arguments = PyTuple_New(0);
-    if (g_no_arguments == nullptr) return nullptr;
+    g_level = PyUnicode_InternFromString("_current_level");
+    if (g_no_arguments == nullptr || g_level == nullptr) return nullptr;
     return PyModule_Create(&g_module);
 }

@@ -12,6 +12,7 @@ import struct
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from ..api import auto_device, is_cuda_array
@@ -33,6 +34,11 @@ CACHE = struct.Struct("26q")
 NO_HEADS = HEADS.pack(0, 0, 0, 0, 0)
 
 
+def _in_forward_mode() -> bool:
+    """Whether a level of forward differentiation is open, where a tensor may carry a tangent."""
+    return getattr(forward_ad, "_current_level", 0) != -1
+
+
 #: An operand is the tuple (pointer, shape, strides in items, format, device, owner); the
 #: owner keeps the memory alive until the launch.  Plain tuples, and a first branch for the
 #: common argument, because a small call's time is the host's: an attribute of a tensor
@@ -42,12 +48,16 @@ def operand(x, what, written=False, stream=0):
     if isinstance(x, _Tensor):
         fmt = _TORCH.get(x.dtype)
         device = x.get_device()
-        if fmt is not None and device >= 0 and not x.requires_grad:
+        if fmt is not None and device >= 0 and not x.requires_grad and not _in_forward_mode():
             return x.data_ptr(), x.shape, x.stride(), fmt, device, x
         if fmt is None:
             raise TypeError(f"{what}: unsupported type {x.dtype}")
         if x.requires_grad:
             raise ValueError(f"{what} requires grad: the call is not recorded for autograd, pass x.detach()")
+        if _in_forward_mode() and forward_ad.unpack_dual(x).tangent is not None:
+            raise ValueError(f"{what} carries a tangent: the call gives none, pass forward_ad.unpack_dual(x).primal")
+        if device >= 0:
+            return x.data_ptr(), x.shape, x.stride(), fmt, device, x
         if written:
             raise ValueError(f"{what} must be in device memory")
         with torch.cuda.stream(_torch_stream(stream)):      # its memory goes back in this stream's order
@@ -166,7 +176,7 @@ class _Fast:
             names = ("b2k_norm_rotate", "b2k_norm_rotate_backward_scratch_bytes", "b2k_norm_rotate_backward",
                      "b2k_cache_write", "b2k_cache_read", "b2k_norm_rotate_write", "b2k_current_device")
             module.setup(torch.Tensor, _TORCH, {n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names},
-                         stream_ptr, workspace)
+                         stream_ptr, workspace, vars(forward_ad))
         for entry in self.ENTRIES:
             setattr(self, entry, getattr(module, entry))
         return self.__dict__[name]

@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import headwise_ref as ref
 from headwise_plan import Plan
@@ -127,3 +128,21 @@ def test_tables_without_columns_still_tell_padding(dim):
     qo.fill_(7.0)
     headnorm.norm_rotate(q, None, qw, None, empty[:0], empty[:0], pos, q_out=qo)
     assert (qo == 7.0).all()
+
+
+def test_tensors_inside_forward_differentiation():
+    """A tensor with a tangent is refused; others give what they give outside."""
+    rng, q, k, qw, kw, cos, sin, pos = setup(9, 4, 2, 64, 32, "float32", "contiguous", "float32", 1)
+    out, inside = (torch.empty_like(q), torch.empty_like(k)), (torch.empty_like(q), torch.empty_like(k))
+    headnorm.norm_rotate(q, k, qw, kw, cos, sin, pos, q_out=out[0], k_out=out[1])
+    codes, scales = pool(3, 4, 2, 64, 64, "e4m3", "f32", rng)
+    with forward_ad.dual_level():
+        headnorm.norm_rotate(q, k, qw, kw, cos, sin, pos, q_out=inside[0], k_out=inside[1])
+        dual = forward_ad.make_dual(k, torch.ones_like(k))
+        for call in (lambda: headnorm.norm_rotate(q, dual, qw, kw, cos, sin, pos, q_out=out[0], k_out=out[1]),
+                     lambda: headnorm.norm_rotate(q, k, qw, kw, cos, sin, pos, q_out=out[0], k_out=dual),
+                     lambda: kvcache.write(dual, None, codes, scales, None, None, pos),
+                     lambda: kvcache.read(codes, scales, None, None, pos[None], torch.tensor([0, 1]), dual, None)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+    assert torch.equal(out[0], inside[0]) and torch.equal(out[1], inside[1])

@@ -39,8 +39,9 @@ class Tensor:
         return 0
 
 
-def load(tmp_path, entry, **more):
-    """A copy of the extension with every entry point at the address `entry`."""
+def load(tmp_path, entry, level=-1):
+    """A copy of the extension with every entry point at the address `entry`, inside `level` of forward
+    differentiation (-1: none)."""
     path = str(tmp_path / "_pyfast.so")
     shutil.copy(_build.build_pyfast(), path)
     loader = importlib.machinery.ExtensionFileLoader("_pyfast", path)
@@ -49,7 +50,8 @@ def load(tmp_path, entry, **more):
     address = {name: ctypes.cast(entry, ctypes.c_void_p).value for name in NAMES}
     address["b2k_current_device"] = ctypes.cast(_DEVICE, ctypes.c_void_p).value
     address["b2k_norm_rotate_backward_scratch_bytes"] = ctypes.cast(_SCRATCH, ctypes.c_void_p).value
-    module.setup(Tensor, FORMATS, address, lambda stream: 0, lambda n, stream: Tensor((n,), "u8"), **more)
+    module.setup(Tensor, FORMATS, address, lambda stream: 0, lambda n, stream: Tensor((n,), "u8"),
+                 {"_current_level": level})
     return module
 
 
@@ -94,3 +96,9 @@ def test_the_interpreter_lock_is_free_during_a_call(tmp_path, name):
     question whether this thread holds the lock."""
     fast = load(tmp_path, ctypes.pythonapi.PyGILState_Check)
     assert getattr(fast, name)(*calls()[name]) == 0
+
+
+@pytest.mark.parametrize("name", list(calls()))
+def test_forward_differentiation_is_left_to_the_python_code(tmp_path, name):
+    entry = ctypes.CFUNCTYPE(ctypes.c_int)(lambda: 0)
+    assert getattr(load(tmp_path, entry, level=0), name)(*calls()[name]) is None

@@ -1,7 +1,12 @@
 """Head-wise calls at the edges of their arguments, without a GPU."""
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
 from numba_cuda_b200 import _lib
-from numba_cuda_b200.kernels import _operands as ops
-from test_headwise_host import _cache, _heads, _rotation
+from numba_cuda_b200.kernels import _operands as ops, headnorm, kvcache
+from test_headwise_host import _cache, _fake, _heads, _rotation
 
 
 def test_positions_are_checked_where_nothing_is_rotated():
@@ -28,3 +33,20 @@ def test_rows_whose_last_chunk_has_no_successor_in_32_bits():
         got = L.b2k_cache_read(cache, _lib.FMT_F16, 1, out if k else ops.NO_HEADS, out if v else ops.NO_HEADS, 4096, 1, 1, 4,
                                4096, 1, 4, None)
         assert got == _lib.ERR_TOO_LARGE
+
+
+def test_tensors_with_a_tangent_are_refused():
+    """The results would have none, without a word."""
+    x, w = torch.ones(3, 2, 16), torch.ones(16)
+    q, slots = _fake((3, 2, 16), np.float32), _fake((3,), np.int64)
+    codes, scales = _fake((5, 4, 2, 16), np.uint8), _fake((5, 4, 2, 1), np.float32)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        dual_w = forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: headnorm.norm_rotate(dual, None), lambda: headnorm.norm_rotate(q, None, dual_w),
+                     lambda: headnorm.norm_rotate(q, None, q_out=dual),
+                     lambda: headnorm.norm_rotate_backward(q, None, None, None, None, None, None, dual, None),
+                     lambda: kvcache.write(dual, None, codes, scales, None, None, slots),
+                     lambda: kvcache.norm_rotate_write(None, q, dual, None, None, None, None, None, codes, scales, codes, scales, slots)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
