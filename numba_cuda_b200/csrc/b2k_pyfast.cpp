@@ -17,7 +17,7 @@
 namespace {
 
 // Set once by setup().
-PyObject *g_tensor_type, *g_formats, *g_stream_ptr, *g_workspace, *g_forward_mode, *g_level, *g_no_arguments;
+PyObject *g_tensor_type, *g_formats, *g_stream_ptr, *g_workspace, *g_forward_mode, *g_level, *g_written, *g_no_arguments;
 
 // An attribute or a method without arguments of the tensor type.  Where it is implemented
 // in C, its function is called directly: looking six of them up for each of ten tensors
@@ -296,6 +296,24 @@ int unlocked(F f) {
     return status;
 }
 
+// The status of a call; after a good one autograd is told which tensors (or None) it has written.
+PyObject *done(int status, std::initializer_list<PyObject *> outputs) {
+    if (status == 0) {
+        Py_ssize_t n = 0;
+        for (PyObject *o : outputs) n += o != Py_None;
+        PyObject *tensors = PyTuple_New(n);
+        if (tensors == nullptr) return nullptr;
+        n = 0;
+        for (PyObject *o : outputs)
+            if (o != Py_None) PyTuple_SET_ITEM(tensors, n++, Py_NewRef(o));
+        PyObject *none = PyObject_CallOneArg(g_written, tensors);
+        Py_DECREF(tensors);
+        if (none == nullptr) return nullptr;
+        Py_DECREF(none);
+    }
+    return PyLong_FromLong(status);
+}
+
 // (q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, q_out, k_out, stream)
 PyObject *norm_rotate(PyObject *, PyObject *const *args, Py_ssize_t n) {
     int device;
@@ -306,7 +324,7 @@ PyObject *norm_rotate(PyObject *, PyObject *const *args, Py_ssize_t n) {
         !read_result(args[10], t.has_q, t.q, device, q_out) || !read_result(args[11], t.has_k, t.k, device, k_out) ||
         !read_stream(args[12], stream))
         return pass();
-    return PyLong_FromLong(unlocked([&] { return g_call.norm_rotate(&t.r, &q_out, &k_out, stream); }));
+    return done(unlocked([&] { return g_call.norm_rotate(&t.r, &q_out, &k_out, stream); }), {args[10], args[11]});
 }
 
 // (q, k, q_weight, k_weight, cos, sin, positions, q_grad, k_grad, eps, interleaved, norm, dq, dk, dq_weight, dk_weight, stream)
@@ -355,7 +373,7 @@ PyObject *norm_rotate_backward(PyObject *, PyObject *const *args, Py_ssize_t n) 
         return g_call.norm_rotate_backward(&t.r, &q_grad, &k_grad, &dq, &dk, sums[0], sums[1], scratch, bytes, stream);
     });
     Py_XDECREF(held);
-    return PyLong_FromLong(status);
+    return done(status, {args[12], args[13], args[14], args[15]});
 }
 
 // (k, v, k_codes, k_scales, v_codes, v_scales, slots, format, stream)
@@ -375,9 +393,10 @@ PyObject *cache_write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (!(has[0] || has[1]) || !read_vector(args[6], device, first.size[0], at) || !is_index(at.format) ||
         !read_stream(args[8], stream))
         return pass();
-    return PyLong_FromLong(unlocked([&] {
+    const int status = unlocked([&] {
         return g_call.cache_write(&cache, first.format, first.size[0], &h[0], &h[1], at.data, index_bytes(at), stream);
-    }));
+    });
+    return done(status, {args[2], args[3], args[4], args[5]});
 }
 
 // (k_codes, k_scales, v_codes, v_scales, page_table, offsets, k_out, v_out, format, stream)
@@ -398,10 +417,11 @@ PyObject *cache_read(PyObject *, PyObject *const *args, Py_ssize_t n) {
         (table.stride[1] != 1 && table.size[1] > 1) || !read_vector(args[5], device, table.size[0] + 1, at) ||
         !is_index(at.format) || !read_stream(args[9], stream))
         return pass();
-    return PyLong_FromLong(unlocked([&] {
+    const int status = unlocked([&] {
         return g_call.cache_read(&cache, first.format, first.size[0], &h[0], &h[1], table.data, table.stride[0], table.size[1],
                                  index_bytes(table), at.data, table.size[0], index_bytes(at), stream);
-    }));
+    });
+    return done(status, {args[6], args[7]});
 }
 
 // (q, k, q_weight, k_weight, cos, sin, positions, v, k_codes, k_scales, v_codes, v_scales, slots, eps, interleaved, norm,
@@ -422,8 +442,9 @@ PyObject *norm_rotate_write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (!fits(t.has_k, t.r.k, side[0], cache.k) || !fits(has_v, v, side[1], cache.v) || !read_vector(args[12], device, t.r.tokens, at) ||
         !is_index(at.format) || !read_stream(args[18], stream))
         return pass();
-    return PyLong_FromLong(
-        unlocked([&] { return g_call.norm_rotate_write(&t.r, &v, &q_out, &cache, at.data, index_bytes(at), stream); }));
+    const int status =
+        unlocked([&] { return g_call.norm_rotate_write(&t.r, &v, &q_out, &cache, at.data, index_bytes(at), stream); });
+    return done(status, {args[17], args[8], args[9], args[10], args[11]});
 }
 
 template <typename F>
@@ -437,11 +458,12 @@ bool address(PyObject *dict, const char *name, F &f) {
     return !PyErr_Occurred();
 }
 
-// setup(tensor type, {dtype: format}, {entry point: address}, stream_ptr, workspace, names of torch.autograd.forward_ad)
+// setup(tensor type, {dtype: format}, {entry point: address}, stream_ptr, workspace, names of torch.autograd.forward_ad,
+//       function to call with a tuple of written tensors)
 PyObject *setup(PyObject *, PyObject *args) {
-    PyObject *type, *formats, *addresses, *stream, *workspace, *forward;
-    if (!PyArg_ParseTuple(args, "OO!O!OOO!", &type, &PyDict_Type, &formats, &PyDict_Type, &addresses, &stream, &workspace,
-                          &PyDict_Type, &forward))
+    PyObject *type, *formats, *addresses, *stream, *workspace, *forward, *written;
+    if (!PyArg_ParseTuple(args, "OO!O!OOO!O", &type, &PyDict_Type, &formats, &PyDict_Type, &addresses, &stream, &workspace,
+                          &PyDict_Type, &forward, &written))
         return nullptr;
     Entry e;
     if (!address(addresses, "b2k_norm_rotate", e.norm_rotate) ||
@@ -460,6 +482,8 @@ PyObject *setup(PyObject *, PyObject *args) {
     Py_XSETREF(g_stream_ptr, stream);
     Py_INCREF(workspace);
     Py_XSETREF(g_workspace, workspace);
+    Py_INCREF(written);
+    Py_XSETREF(g_written, written);
     Py_INCREF(forward);
     Py_XSETREF(g_forward_mode, forward);
     Py_INCREF(type);

@@ -149,6 +149,18 @@ def workspace(nbytes, stream):
         return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
 
 
+#: Raises the version counters of tensors that a call has written through their addresses:
+#: autograd then notices that a tensor it saved is not what it was.
+_increment_version = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
+
+
+def written(*arrays) -> None:
+    """Note that a call has written these arrays (``None`` and arrays of other kinds among them)."""
+    tensors = tuple(x for x in arrays if isinstance(x, _Tensor))
+    if tensors:
+        _increment_version(tensors)
+
+
 class _NoFast:
     """Stands for the extension where it was not built: every call takes the Python code."""
 
@@ -176,7 +188,7 @@ class _Fast:
             names = ("b2k_norm_rotate", "b2k_norm_rotate_backward_scratch_bytes", "b2k_norm_rotate_backward",
                      "b2k_cache_write", "b2k_cache_read", "b2k_norm_rotate_write", "b2k_current_device")
             module.setup(torch.Tensor, _TORCH, {n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names},
-                         stream_ptr, workspace, vars(forward_ad))
+                         stream_ptr, workspace, vars(forward_ad), _increment_version)
         for entry in self.ENTRIES:
             setattr(self, entry, getattr(module, entry))
         return self.__dict__[name]
@@ -184,4 +196,5 @@ class _Fast:
 
 fast = _Fast()
 
-__all__ = ["operand", "heads", "vector", "indices", "pack_heads", "index_bytes", "on_one_device", "like", "workspace", "fast"]
+__all__ = ["operand", "heads", "vector", "indices", "pack_heads", "index_bytes", "on_one_device", "like", "workspace",
+           "written", "fast"]

@@ -18,7 +18,7 @@ from __future__ import annotations
 from .. import _lib
 from ..devicearray import stream_ptr
 from ._operands import (HEAD_FORMATS, ROTATION, fast, heads, index_bytes, indices, like, on_one_device, operand, pack_heads,
-                        vector, workspace)
+                        vector, workspace, written)
 
 
 def _table(x, what, stream):
@@ -130,6 +130,7 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, position
     k_out, ko = result(k_out, k, "k_out", stream)
     on_one_device([*ops, qo, ko])
     _lib.check(_lib.lib().b2k_norm_rotate(packed, pack_heads(qo), pack_heads(ko), stream_ptr(stream)))
+    written(q_out, k_out)
     return q_out, k_out
 
 
@@ -178,6 +179,7 @@ def norm_rotate_backward(q, k, q_weight, k_weight, cos, sin, positions, q_grad, 
         weights[0][1][0] if weights[0][1] is not None else None,
         weights[1][1][0] if weights[1][1] is not None else None,
         scratch.data_ptr() if scratch is not None else None, need, stream_ptr(stream)))
+    written(dq, dk, dq_weight, dk_weight)
     return outs[0][0], outs[1][0], weights[0][0], weights[1][0]
 
 

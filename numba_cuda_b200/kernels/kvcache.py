@@ -23,7 +23,7 @@ from __future__ import annotations
 from .. import _lib
 from ..casts import _format_code
 from ..devicearray import stream_ptr
-from ._operands import CACHE, INDEX_FORMATS, fast, heads, index_bytes, indices, on_one_device, operand, pack_heads
+from ._operands import CACHE, INDEX_FORMATS, fast, heads, index_bytes, indices, on_one_device, operand, pack_heads, written
 from .headnorm import result, rotation
 
 _CODES = (_lib.FMT_E4M3, _lib.FMT_E5M2)
@@ -131,6 +131,7 @@ def write(k, v, k_codes, k_scales, v_codes, v_scales, slots, format=None, stream
     on_one_device((k, v, at, *ops))
     _lib.check(_lib.lib().b2k_cache_write(packed, fmt, tokens, pack_heads(k), pack_heads(v), at[0], index_bytes(at),
                                           stream_ptr(stream)))
+    written(k_codes, k_scales, v_codes, v_scales)
 
 
 def read(k_codes, k_scales, v_codes, v_scales, page_table, offsets, k_out, v_out, format=None, stream=0):
@@ -165,6 +166,7 @@ def read(k_codes, k_scales, v_codes, v_scales, page_table, offsets, k_out, v_out
     on_one_device((ko, vo, table, at, *ops))
     _lib.check(_lib.lib().b2k_cache_read(packed, fmt, rows, pack_heads(ko), pack_heads(vo), table[0], table[2][0], width,
                                          index_bytes(table), at[0], sequences, index_bytes(at), stream_ptr(stream)))
+    written(k_out, v_out)
     return k_out, v_out
 
 
@@ -194,6 +196,7 @@ def norm_rotate_write(q, k, v, q_weight, k_weight, cos, sin, positions, k_codes,
     on_one_device((*ops, v, qo, at, *more))
     _lib.check(_lib.lib().b2k_norm_rotate_write(packed, pack_heads(v), pack_heads(qo), packed_cache, at[0], index_bytes(at),
                                                 stream_ptr(stream)))
+    written(q_out, k_codes, k_scales, v_codes, v_scales)
     return q_out
 
 

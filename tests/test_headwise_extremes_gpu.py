@@ -6,7 +6,7 @@ from torch.autograd import forward_ad
 
 import headwise_ref as ref
 from headwise_plan import Plan
-from numba_cuda_b200.kernels import headnorm, kvcache
+from numba_cuda_b200.kernels import _operands, headnorm, kvcache
 from test_headnorm_gpu import TORCH, angles, check, f64, layout, setup
 from test_kvcache_gpu import pool
 
@@ -146,3 +146,42 @@ def test_tensors_inside_forward_differentiation():
             with pytest.raises(ValueError, match="tangent"):
                 call()
     assert torch.equal(out[0], inside[0]) and torch.equal(out[1], inside[1])
+
+
+@pytest.mark.parametrize("fast", [True, False])
+def test_autograd_notices_what_a_call_has_written(fast, monkeypatch):
+    """Every output's version counter rises, so a tensor that another operation saved for its backward
+    is not taken for what it was; an input's does not."""
+    if not fast:
+        for module in (headnorm, kvcache):
+            monkeypatch.setattr(module, "fast", _operands._NoFast)
+    rng, q, k, qw, kw, cos, sin, pos = setup(9, 4, 2, 64, 32, "float32", "contiguous", "float32", 1)
+    v = layout((9, 2, 64), "contiguous", "float32", rng)
+    pools = [a for _ in range(2) for a in pool(3, 4, 2, 64, 64, "e4m3", "f32", rng)]
+    qo, ko, dq, dk, out = torch.empty_like(q), torch.empty_like(k), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    dw = torch.empty_like(qw), torch.empty_like(kw)
+    inputs = (q, k, v, qw, kw, cos, sin, pos)
+    slots = torch.arange(9, device="cuda")
+    table, offsets = torch.zeros(1, 3, dtype=torch.int64, device="cuda"), torch.tensor([0, 9], device="cuda")
+    for call, outputs in (
+            (lambda: headnorm.norm_rotate(q, k, qw, kw, cos, sin, pos, q_out=qo, k_out=ko), (qo, ko)),
+            (lambda: headnorm.norm_rotate(q, None, qw, None, cos, sin, pos, q_out=qo), (qo,)),
+            (lambda: headnorm.norm_rotate_backward(q, k, qw, kw, cos, sin, pos, qo, ko, dq=dq, dk=dk, dq_weight=dw[0], dk_weight=dw[1]),
+             (dq, dk, *dw)),
+            (lambda: kvcache.write(k, v, *pools, slots), pools), (lambda: kvcache.write(None, v, None, None, *pools[2:], slots), pools[2:]),
+            (lambda: kvcache.norm_rotate_write(q, k, v, qw, kw, cos, sin, pos, *pools, slots, q_out=qo), (qo, *pools)),
+            (lambda: kvcache.read(*pools, table, offsets, out, ko), (out, ko))):
+        before, still = [o._version for o in outputs], [x._version for x in inputs]
+        call()
+        assert all(o._version > b for o, b in zip(outputs, before))
+        assert [x._version for x in inputs] == still
+    # in place over a tensor that a product keeps for its backward
+    leaf = torch.ones_like(q, requires_grad=True)
+    product = (leaf * qo).sum()
+    headnorm.norm_rotate(qo, None, qw, None, cos, sin, pos, q_out=qo)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    with torch.inference_mode():                       # tensors without a counter
+        made = torch.empty(9, 4, 64, device="cuda")
+        headnorm.norm_rotate(q, None, qw, None, cos, sin, pos, q_out=made)
+    headnorm.norm_rotate(q, None, qw, None, cos, sin, pos, q_out=made)

@@ -39,10 +39,10 @@ class Tensor:
         return 0
 
 
-def load(tmp_path, entry, level=-1):
+def load(tmp_path, entry, level=-1, written=lambda tensors: None):
     """A copy of the extension with every entry point at the address `entry`, inside `level` of forward
-    differentiation (-1: none)."""
-    path = str(tmp_path / "_pyfast.so")
+    differentiation (-1: none); `written` is told what a call has written."""
+    path = str(tmp_path / f"_pyfast{len(list(tmp_path.iterdir()))}.so")        # a file in use stays as it is
     shutil.copy(_build.build_pyfast(), path)
     loader = importlib.machinery.ExtensionFileLoader("_pyfast", path)
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_pyfast", loader))
@@ -51,7 +51,7 @@ def load(tmp_path, entry, level=-1):
     address["b2k_current_device"] = ctypes.cast(_DEVICE, ctypes.c_void_p).value
     address["b2k_norm_rotate_backward_scratch_bytes"] = ctypes.cast(_SCRATCH, ctypes.c_void_p).value
     module.setup(Tensor, FORMATS, address, lambda stream: 0, lambda n, stream: Tensor((n,), "u8"),
-                 {"_current_level": level})
+                 {"_current_level": level}, written)
     return module
 
 
@@ -102,3 +102,23 @@ def test_the_interpreter_lock_is_free_during_a_call(tmp_path, name):
 def test_forward_differentiation_is_left_to_the_python_code(tmp_path, name):
     entry = ctypes.CFUNCTYPE(ctypes.c_int)(lambda: 0)
     assert getattr(load(tmp_path, entry, level=0), name)(*calls()[name]) is None
+
+
+@pytest.mark.parametrize("name", list(calls()))
+def test_written_tensors_are_told(tmp_path, name):
+    """After a call that was made, and after no other."""
+    told, args = [], list(calls()[name])
+    outputs = {"norm_rotate": (10, 11), "norm_rotate_backward": (12, 13, 14, 15), "cache_write": (2, 3, 4, 5),
+               "cache_read": (6, 7), "norm_rotate_write": (17, 8, 9, 10, 11)}[name]
+    for i in outputs:
+        args[i] = Tensor(args[i].shape, args[i].dtype, args[i].ptr)
+    for status in (0, 7):
+        entry = ctypes.CFUNCTYPE(ctypes.c_int)(lambda: status)
+        assert getattr(load(tmp_path, entry, written=told.append), name)(*args) == status
+    assert len(told) == 1 and len(told[0]) == len(outputs)
+    assert all(t is args[i] for t, i in zip(told[0], outputs))
+
+    def broken(tensors):
+        raise RuntimeError("not told")
+    with pytest.raises(RuntimeError, match="not told"):
+        getattr(load(tmp_path, ctypes.CFUNCTYPE(ctypes.c_int)(lambda: 0), written=broken), name)(*args)
