@@ -19,9 +19,11 @@ from ..api import auto_device, is_cuda_array
 from ..devicearray import DeviceNDArray, _torch_stream, bfloat16_dtype, stream_ptr
 
 _Tensor = torch.Tensor
-_TORCH = {torch.float32: _lib.FMT_F32, torch.float16: _lib.FMT_F16, torch.bfloat16: _lib.FMT_BF16,
-          torch.uint16: _lib.FMT_BF16, torch.uint8: _lib.FMT_U8, torch.int32: _lib.FMT_I32, torch.int64: _lib.FMT_I64,
-          torch.float8_e4m3fn: _lib.FMT_E4M3, torch.float8_e5m2: _lib.FMT_E5M2, torch.float8_e8m0fnu: _lib.FMT_E8M0}
+#: Types by torch's names; a torch of fewer types has no tensors of the others.
+_TORCH = {getattr(torch, name): fmt for name, fmt in (
+    ("float32", _lib.FMT_F32), ("float16", _lib.FMT_F16), ("bfloat16", _lib.FMT_BF16), ("uint16", _lib.FMT_BF16),
+    ("uint8", _lib.FMT_U8), ("int32", _lib.FMT_I32), ("int64", _lib.FMT_I64), ("float8_e4m3fn", _lib.FMT_E4M3),
+    ("float8_e5m2", _lib.FMT_E5M2), ("float8_e8m0fnu", _lib.FMT_E8M0)) if hasattr(torch, name)}
 _NUMPY = {"float32": _lib.FMT_F32, "float16": _lib.FMT_F16, "bfloat16": _lib.FMT_BF16, "uint16": _lib.FMT_BF16,
           "uint8": _lib.FMT_U8, "int32": _lib.FMT_I32, "int64": _lib.FMT_I64, "float8_e4m3fn": _lib.FMT_E4M3,
           "float8_e5m2": _lib.FMT_E5M2, "float8_e8m0fnu": _lib.FMT_E8M0}

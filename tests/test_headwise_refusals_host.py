@@ -1,4 +1,8 @@
 """Head-wise calls at the edges of their arguments, without a GPU."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -50,3 +54,14 @@ def test_tensors_with_a_tangent_are_refused():
                      lambda: kvcache.norm_rotate_write(None, q, dual, None, None, None, None, None, codes, scales, codes, scales, slots)):
             with pytest.raises(ValueError, match="tangent"):
                 call()
+
+
+def test_the_package_imports_with_a_torch_of_fewer_types():
+    """Types that a torch does not have are types that no tensor of it has."""
+    code = ("import torch\n"
+            "for name in ('float8_e8m0fnu', 'float8_e5m2', 'float8_e4m3fn'):\n"
+            "    delattr(torch, name)\n"
+            "import numba_cuda_b200 as cuda\n"
+            "from numba_cuda_b200.kernels import _operands\n"
+            "assert torch.bfloat16 in _operands._TORCH and cuda.casts.cast and cuda.reduce and cuda.kernels.kvcache.read\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
