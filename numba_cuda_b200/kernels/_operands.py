@@ -151,9 +151,22 @@ def workspace(nbytes, stream):
         return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
 
 
-#: Raises the version counters of tensors that a call has written through their addresses:
-#: autograd then notices that a tensor it saved is not what it was.
-_increment_version = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
+def _version_counters():
+    """torch's function that raises the version counters of a tuple of tensors."""
+    many = getattr(torch._C, "_increment_version", None)
+    try:
+        many((torch.empty(0),))
+        return many
+    except TypeError:                                       # an older torch takes one at a time
+        def each(tensors):
+            for x in tensors:
+                torch.autograd.graph.increment_version(x)
+        return each
+
+
+#: Called for tensors that a call has written through their addresses: autograd then notices
+#: that a tensor it saved is not what it was.
+_increment_version = _version_counters()
 
 
 def written(*arrays) -> None:

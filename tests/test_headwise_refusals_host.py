@@ -65,3 +65,18 @@ def test_the_package_imports_with_a_torch_of_fewer_types():
             "from numba_cuda_b200.kernels import _operands\n"
             "assert torch.bfloat16 in _operands._TORCH and cuda.casts.cast and cuda.reduce and cuda.kernels.kvcache.read\n")
     subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+def test_version_counters_rise_with_a_torch_that_takes_one_tensor_at_a_time():
+    code = ("import torch\n"
+            "many = torch._C._increment_version\n"
+            "def one(x):\n"
+            "    if not isinstance(x, torch.Tensor):\n"
+            "        raise TypeError('one tensor')\n"
+            "    many((x,))\n"
+            "torch._C._increment_version = torch.autograd.graph.increment_version = one\n"
+            "from numba_cuda_b200.kernels import _operands\n"
+            "a, b = torch.zeros(2), torch.zeros(3)\n"
+            "_operands.written(a, None, b)\n"
+            "assert (a._version, b._version) == (1, 1)\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
