@@ -405,7 +405,8 @@ typedef struct b2k_cache {
 } b2k_cache;
 
 /* Forward.  q_out / k_out have the shapes of q / k and may be the same memory; any
- * other overlap of an output with an input is not allowed. */
+ * other overlap of an output with an input, or of two outputs, is not allowed (two that
+ * start at one address are refused, here and in the calls below). */
 B2K_API int b2k_norm_rotate(const b2k_rotation *r, const b2k_heads *q_out, const b2k_heads *k_out, void *stream);
 
 /* Gradients of b2k_norm_rotate at r->q, r->k for the outputs' gradients q_grad, k_grad:

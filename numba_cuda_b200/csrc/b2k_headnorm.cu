@@ -73,6 +73,11 @@ int check_heads(const b2k_heads &h, const char *name, const char *what, int64_t 
     return B2K_OK;
 }
 
+int check_apart(const void *a, const void *b, const char *name, const char *what) {
+    if (a != nullptr && a == b) return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s are the same memory", name, what);
+    return B2K_OK;
+}
+
 int check_like(const b2k_heads &h, const b2k_heads &like, const char *name, const char *what) {
     if (h.heads != like.heads || (h.heads && h.dim != like.dim))
         return b2k::fail(B2K_ERR_INVALID_ARG, "%s: %s has another shape than its input", name, what);
@@ -943,6 +948,9 @@ int b2k_norm_rotate_backward(const b2k_rotation *r, const b2k_heads *q_grad, con
     const Plan plan = lay_out(p, vec, r);
     if (plan.iter == 0) return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: no kernel for this head size", name);
     if (int rc = count_items(p, kBackwardHeadsPerItem, kBackwardBusy, name)) return rc;
+    if (r->tokens > 0)
+        if (int rc = check_apart(p.role[0].out, p.role[1].out, name, "dq and dk")) return rc;
+    if (int rc = check_apart(dq_weight_dev, dk_weight_dev, name, "the weights' gradients")) return rc;
     const cudaStream_t st = b2k::as_stream(stream);
     const int64_t most = b2k::sm_count() * static_cast<int64_t>(backward_kernel(r->format, p, plan, 0, st));
     int64_t need[2] = {p.role[0].blocks, p.role[1].blocks};

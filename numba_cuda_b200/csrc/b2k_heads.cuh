@@ -469,6 +469,8 @@ struct Plan {
 int item_bytes(int64_t format);                      // 0 for a format that arrays of heads cannot have
 int check_heads(const b2k_heads &h, const char *name, const char *what, int64_t tokens, int itemsize, bool written);
 int check_like(const b2k_heads &h, const b2k_heads &like, const char *name, const char *what);
+// Two outputs that start at one address would overwrite each other.
+int check_apart(const void *a, const void *b, const char *name, const char *what);
 int check_tokens(int64_t format, int64_t tokens, const char *name);
 int check_rotation(const b2k_rotation *r, const char *name);
 int check_cache(const b2k_cache *c, const char *name);

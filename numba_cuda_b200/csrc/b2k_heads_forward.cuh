@@ -287,6 +287,7 @@ int launch_forward(const Params &all, int64_t format, const b2k_rotation *rot, c
         const Plan plan = lay_out(p, width, rot);
         if (plan.iter == 0) return b2k::fail(B2K_ERR_UNSUPPORTED, "%s: no kernel for this head size", name);
         if (int rc = count_items(p, kHeadsPerItem, kForwardBusy, name)) return rc;
+        if (int rc = check_apart(all.role[0].out, all.role[1].out, name, "q_out and k_out")) return rc;
         const unsigned blocks = p.role[0].blocks + p.role[1].blocks + p.role[2].blocks;
         if (format == B2K_FMT_F32) pick_forward<float, MODE>(p, plan, blocks, stream);
         else if (format == B2K_FMT_F16) pick_forward<__half, MODE>(p, plan, blocks, stream);

@@ -215,6 +215,11 @@ int tile_rows(int64_t rows, int64_t chunks) {
     return tile;
 }
 
+int check_sides_apart(const Params &p, const char *name) {
+    if (int rc = check_apart(p.role[1].codes, p.role[2].codes, name, "the codes of keys and values")) return rc;
+    return check_apart(p.role[1].scales, p.role[2].scales, name, "the scales of keys and values");
+}
+
 int check_slots(const void *slots, int slot_bytes, int64_t tokens, const char *name) {
     return tokens ? check_indices(slots, slot_bytes, name, "slots") : B2K_OK;
 }
@@ -243,6 +248,7 @@ int b2k_cache_write(const b2k_cache *cache, int format, int64_t tokens, const b2
         set_pages(p, p.role[1 + i], *cache, *side[i]);
     }
     if (tokens == 0 || cache->pages == 0) return B2K_OK;
+    if (int rc = check_sides_apart(p, name)) return rc;
     p.tokens = tokens;
     p.slots = slots_dev;
     p.slot_bytes = slot_bytes;
@@ -277,6 +283,8 @@ int b2k_norm_rotate_write(const b2k_rotation *r, const b2k_heads *v, const b2k_h
         set_input(p.role[2], *v, r->tokens);
         set_pages(p, p.role[2], *cache, cache->v);
     }
+    if (cache->pages > 0)
+        if (int rc = check_sides_apart(p, name)) return rc;
     p.tokens = r->tokens;
     p.slots = slots_dev;
     p.slot_bytes = slot_bytes;
@@ -311,6 +319,7 @@ int b2k_cache_read(const b2k_cache *cache, int format, int64_t rows, const b2k_h
                              r.group};
     }
     if (rows == 0 || seqs == 0 || (k_out->heads == 0 && v_out->heads == 0)) return B2K_OK;
+    if (int rc = check_apart(p.side[0].out, p.side[1].out, name, "k_out and v_out")) return rc;
     if (int rc = check_indices(offsets_dev, offset_bytes, name, "offsets")) return rc;
     if (table_width > 0)
         if (int rc = check_indices(table_dev, table_bytes, name, "the page table")) return rc;

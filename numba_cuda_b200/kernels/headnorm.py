@@ -114,7 +114,7 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, position
     :param norm: ``False`` leaves the norm out.
     :param q_out, k_out: outputs; new arrays when not given (padding rows are then not
                  set).  An output may be its own input's memory; it must not overlap an
-                 input in any other way.
+                 input in any other way, nor another output.
     :param stream: stream of the launch (0 = the default stream); arrays that other streams
                  produce must be complete or ordered before it, as everywhere here.
 

@@ -80,3 +80,29 @@ def test_version_counters_rise_with_a_torch_that_takes_one_tensor_at_a_time():
             "_operands.written(a, None, b)\n"
             "assert (a._version, b._version) == (1, 1)\n")
     subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+def test_two_outputs_in_one_memory_are_refused():
+    """Keys and values would overwrite each other.  Inputs may share theirs, and so may outputs of no tokens."""
+    L = _lib.lib()
+    a, b, none = _heads(ptr=1 << 20), _heads(ptr=1 << 21), ops.NO_HEADS
+    rotation = _rotation(qw=4096, kw=4096)
+
+    def refused(status):
+        return status == _lib.ERR_INVALID_ARG and b"same memory" in L.b2k_last_error()
+
+    assert refused(L.b2k_norm_rotate(rotation, a, a, None))
+    assert L.b2k_norm_rotate(_rotation(tokens=0), a, a, None) == 0
+    need = L.b2k_norm_rotate_backward_scratch_bytes(rotation)
+    assert refused(L.b2k_norm_rotate_backward(rotation, a, a, a, a, 4096, 8192, 4096, need, None))
+    assert refused(L.b2k_norm_rotate_backward(rotation, a, a, a, b, 4096, 4096, 4096, need, None))
+    side = (4096, 1024, 64, 16, 8192, 64, 4, 1, 4, 16, 16)
+    codes, scales = (1 << 16, *side[1:]), (*side[:4], 1 << 16, *side[5:])
+    for v in (side, codes, scales):
+        cache = _cache(k=side, v=v)
+        assert refused(L.b2k_cache_write(cache, _lib.FMT_F32, 2, a, b, 4096, 8, None))
+        assert refused(L.b2k_norm_rotate_write(rotation, b, a, cache, 4096, 8, None))
+    assert refused(L.b2k_cache_read(_cache(), _lib.FMT_F32, 2, a, a, 4096, 3, 3, 4, 4096, 2, 4, None))
+    empty = _cache(pages=0, k=(0, *side[1:4], 0, *side[5:]), v=(0, *side[1:4], 0, *side[5:]))
+    assert L.b2k_cache_write(empty, _lib.FMT_F32, 2, a, b, 4096, 8, None) == 0
+    assert L.b2k_cache_read(_cache(), _lib.FMT_F32, 0, a, a, 4096, 3, 3, 4, 4096, 2, 4, None) == 0
