@@ -615,8 +615,10 @@ __device__ __forceinline__ void backward_rows_ahead(const Params &p, const Role 
     char *const row_slot = shared + threadIdx.x * 16;
     char *const table_slot = shared + Slots::rows + threadIdx.x * Slots::half;
 
+    if (base >= r.all_items) return;
     // the load side: its item, row and position, and the position of the item after it
     Item<T> ahead;
+    ahead.seek(r, base + in_warp);
     uint32_t ahead_base = base;
     int ahead_h = 0, ahead_stage = 0, ahead_table = 0;
     int64_t ahead_position = 0, after_position = 0;
@@ -664,8 +666,6 @@ __device__ __forceinline__ void backward_rows_ahead(const Params &p, const Role 
         ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
     };
 
-    if (base >= r.all_items) return;
-    ahead.seek(r, base + in_warp);
     ahead_position = later_position(base);
     after_position = later_position(base + step);
 #pragma unroll
