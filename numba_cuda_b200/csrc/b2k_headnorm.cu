@@ -445,15 +445,14 @@ struct Weights {
     float x[ITER][VEC], y[ITER][VEC], sum_x[ITER][VEC], sum_y[ITER][VEC];
 };
 
-// The gradient of one row as loaded (x and g, two chunks a unit), stored to `out` if `there`.
-// A padding token's rows come as zeros.
+// The gradient of one row as loaded (x and g, two chunks a unit), stored to `out` if `there`; a
+// row that is not comes as zeros.
 template <typename T, int VEC, int ITER, bool INTER, bool AHEAD>
 __device__ __forceinline__ void gradient_row(const Params &p, const Role &r, const Lanes &g, const int (&oa)[ITER],
                                              const int (&ob)[ITER], const Chunk<T, VEC> (&xa)[ITER],
                                              const Chunk<T, VEC> (&xb)[ITER], const Chunk<T, VEC> (&da)[ITER],
                                              const Chunk<T, VEC> (&db)[ITER], const float (&c)[ITER][VEC],
-                                             const float (&s)[ITER][VEC], Weights<VEC, ITER> &w, T *out, bool padding,
-                                             bool there) {
+                                             const float (&s)[ITER][VEC], Weights<VEC, ITER> &w, T *out, bool there) {
     float x[ITER][VEC], y[ITER][VEC], gx[ITER][VEC], gy[ITER][VEC];
     float2 ss = make_float2(0.0f, 0.0f), dot = ss;
 #pragma unroll
@@ -474,7 +473,7 @@ __device__ __forceinline__ void gradient_row(const Params &p, const Role &r, con
     if (p.norm) {
         // dx = r (h - n mean(h n)) with n = x r:  r h - x (r^3 sum(h x) / dim)
         const float mean = g.sum(ss.x + ss.y) * r.inv_dim;
-        const float by = padding || !there ? 0.0f : rsqrtf(mean + p.eps);       // eps may be zero
+        const float by = !there ? 0.0f : rsqrtf(mean + p.eps);       // eps may be zero
         float pull = g.sum(dot.x + dot.y) * r.inv_dim * by * by * by;
         // Squares beyond float32: the result is zeros, and so is the gradient; but the sum of h x can
         // have passed the range too, and infinity times zero is no zero.  What is infinite or a NaN
@@ -501,16 +500,19 @@ __device__ __forceinline__ void gradient_row(const Params &p, const Role &r, con
     for (int i = 0; i < ITER; ++i) {
         float a[VEC], b[VEC];
         out_of_pairs<VEC, INTER>(gx[i], gy[i], a, b);
-        if (there && !padding && oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a);
-        if (there && !padding && ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b);
+        if (there && oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], a);
+        if (there && ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], b);
     }
-    if (there && padding) {                 // not computed: a weight's infinity times zero is no zero
-        const float zeros[VEC] = {};
+}
+
+// A padding token's row: not computed, since a weight's infinity times zero is no zero.
+template <typename T, int VEC, int ITER>
+__device__ __forceinline__ void zero_row(T *out, const int (&oa)[ITER], const int (&ob)[ITER], int dim) {
+    const float zeros[VEC] = {};
 #pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            if (oa[i] < r.dim) store_chunk<T, VEC>(out + oa[i], zeros);
-            if (ob[i] < r.dim) store_chunk<T, VEC>(out + ob[i], zeros);
-        }
+    for (int i = 0; i < ITER; ++i) {
+        if (oa[i] < dim) store_chunk<T, VEC>(out + oa[i], zeros);
+        if (ob[i] < dim) store_chunk<T, VEC>(out + ob[i], zeros);
     }
 }
 
@@ -558,8 +560,9 @@ __device__ __forceinline__ void backward_rows(const Params &p, const Role &r, co
             it.grad += r.grad_head;
             x_next.load(it.in, 0, loads - h - 1, oa, ob, r.dim);
             g_next.load(it.grad, 0, loads - h - 1, oa, ob, r.dim);
-            gradient_row<T, VEC, ITER, INTER, false>(p, r, g, oa, ob, x_now.a[0], x_now.b[0], g_now.a[0], g_now.b[0], c, s, w, it.out, padding,
-                                       h < it.rows);
+            gradient_row<T, VEC, ITER, INTER, false>(p, r, g, oa, ob, x_now.a[0], x_now.b[0], g_now.a[0], g_now.b[0], c, s, w, it.out,
+                                                     !padding && h < it.rows);
+            if (padding && h < it.rows) zero_row<T, VEC, ITER>(it.out, oa, ob, r.dim);
             it.out += r.out_head;
             x_now = x_next;
             g_now = g_next;
@@ -712,9 +715,10 @@ __device__ __forceinline__ void backward_rows_ahead(const Params &p, const Role 
                 if (!row)
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) c[0][j] = s[0][j] = 0.0f;
+                if (there && padding) zero_row<T, VEC, 1>(out, oa, ob, r.dim);
             }
             load_step();                     // into the slot that the step before this one read
-            gradient_row<T, VEC, 1, INTER, true>(p, r, g, oa, ob, xa, xb, da, db, c, s, w, out, padding, there);
+            gradient_row<T, VEC, 1, INTER, true>(p, r, g, oa, ob, xa, xb, da, db, c, s, w, out, row);
             out += r.out_head;
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }
