@@ -1,4 +1,6 @@
 """Head-wise calls at the ends of their ranges."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -185,3 +187,39 @@ def test_autograd_notices_what_a_call_has_written(fast, monkeypatch):
         made = torch.empty(9, 4, 64, device="cuda")
         headnorm.norm_rotate(q, None, qw, None, cos, sin, pos, q_out=made)
     headnorm.norm_rotate(q, None, qw, None, cos, sin, pos, q_out=made)
+
+
+def test_calls_of_several_threads_at_once():
+    """The lock is free during a call, so threads are inside the library at the same time: each gets its own
+    results, and the message of its own error."""
+    sets = [setup(500 + 300 * i, 8, 4, 64, 64, "bfloat16", "contiguous", "float32", i)[1:] for i in range(4)]
+    want = [[g.as_torch() for g in (*headnorm.norm_rotate(*s), *headnorm.norm_rotate_backward(*s, s[0], s[1]))] for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        q, k, qw, kw, cos, sin, pos = sets[i]
+        st = torch.cuda.Stream()
+        out = [torch.empty_like(t) for t in (q, k, q, k, qw, kw)]
+        for n in range(40):
+            headnorm.norm_rotate(q, k, qw, kw, cos, sin, pos, q_out=out[0], k_out=out[1], stream=st)
+            headnorm.norm_rotate_backward(q, k, qw, kw, cos, sin, pos, q, k, dq=out[2], dk=out[3], dq_weight=out[4],
+                                          dk_weight=out[5], stream=st)
+            try:
+                headnorm.norm_rotate(q, k, qw, kw, cos, sin, pos, eps=-1.0 if i % 2 else 1e-6, q_out=out[0], k_out=out[i % 2],
+                                     stream=st)
+                wrong.append((i, "no error"))
+            except ValueError as e:
+                if ("eps" if i % 2 else "shape") not in str(e):
+                    wrong.append((i, str(e)))
+            if n % 10 == 0:
+                st.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(out, want[i])):
+                    wrong.append((i, "results"))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sets))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
