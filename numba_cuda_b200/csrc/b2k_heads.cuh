@@ -327,30 +327,32 @@ __device__ __forceinline__ void load_angles(const float *row, int u, int oa, int
     }
 }
 
-// (x, y) -> scale (x k0 - y k1, y k2 + x k3): rotation, weights and norm of a pair in one
-// step, with k0 = w_x cos, k1 = w_y sin, k2 = w_y cos, k3 = w_x sin.  Pairs that are not
-// rotated are scaled by their weights k0, k2 alone: a product with a zero sine would
-// carry an infinity over to the partner.
+// (x, y) -> (x' k0 - y' k1, y' k2 + x' k3), x' = scale x, y' = scale y: norm, weights and rotation
+// of a pair in one step, with k0 = w_x cos, k1 = w_y sin, k2 = w_y cos, k3 = w_x sin.  The scale goes
+// first: normed items are at most sqrt(dim), so that no product here leaves float32's range where
+// the result does not, and the zero scale of a head whose squares did gives zeros.  Pairs that are
+// not rotated take their weights k0, k2 alone: a product with a zero sine would carry an infinity
+// over to the partner.
 template <int FROM, int TO, int VEC>
 __device__ __forceinline__ void turn(float (&x)[VEC], float (&y)[VEC], const float (&k0)[VEC], const float (&k1)[VEC],
                                      const float (&k2)[VEC], const float (&k3)[VEC], float scale, bool turned) {
     if constexpr (TO - FROM == 1) {
+        x[FROM] *= scale;
+        y[FROM] *= scale;
         const float u = turned ? x[FROM] * k0[FROM] - y[FROM] * k1[FROM] : x[FROM] * k0[FROM];
         const float v = turned ? y[FROM] * k2[FROM] + x[FROM] * k3[FROM] : y[FROM] * k2[FROM];
-        x[FROM] = u * scale;
-        y[FROM] = v * scale;
+        x[FROM] = u;
+        y[FROM] = v;
     } else {
         const float2 by = make_float2(scale, scale);
 #pragma unroll
         for (int j = FROM; j < TO; j += 2) {
-            const float2 xx = make_float2(x[j], x[j + 1]), yy = make_float2(y[j], y[j + 1]);
+            const float2 xx = mul2(make_float2(x[j], x[j + 1]), by), yy = mul2(make_float2(y[j], y[j + 1]), by);
             float2 u = mul2(xx, make_float2(k0[j], k0[j + 1])), v = mul2(yy, make_float2(k2[j], k2[j + 1]));
             if (turned) {
                 u = fma2(make_float2(-yy.x, -yy.y), make_float2(k1[j], k1[j + 1]), u);
                 v = fma2(xx, make_float2(k3[j], k3[j + 1]), v);
             }
-            u = mul2(u, by);
-            v = mul2(v, by);
             x[j] = u.x;
             x[j + 1] = u.y;
             y[j] = v.x;

@@ -180,17 +180,6 @@ __device__ __forceinline__ void forward_role(const Params &p, uint32_t block, un
 #pragma unroll
                     for (int i = 0; i < ITER; ++i) ss = squares<VEC>(a[i], b[i], ss);
                     by = rsqrtf(g.sum(ss) * r.inv_dim + p.eps);
-                    // squares beyond float32: zeros before the products of turn(), which could
-                    // pass the range too and would give infinity * 0
-                    if (by == 0.0f) {
-#pragma unroll
-                        for (int i = 0; i < ITER; ++i)
-#pragma unroll
-                            for (int j = 0; j < VEC; ++j) {
-                                a[i][j] *= 0.0f;
-                                b[i][j] *= 0.0f;
-                            }
-                    }
                 }
 #pragma unroll
                 for (int i = 0; i < ITER; ++i) {

@@ -223,3 +223,15 @@ def test_calls_of_several_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("dim,rot,inter", [(64, 64, False), (64, 32, True), (33, 10, False), (64, 0, False)])
+@pytest.mark.parametrize("items,weights", [(1e15, 1e25), (1e-17, 1e-25)])
+def test_weights_and_items_far_from_one(dim, rot, inter, items, weights):
+    """Their product leaves float32's range, the normed item's product with the weight does not."""
+    _, q, _, qw, _, cos, sin, pos = setup(5, 3, 1, dim, rot, "float32", "contiguous", "float32", 1)
+    q *= items
+    qw *= weights
+    c, s = angles(cos, sin, pos)
+    got = headnorm.norm_rotate(q, None, qw, None, cos, sin, pos, eps=0.0, interleaved=inter)[0].as_torch()
+    check(got, *ref.norm_rotate(f64(q), f64(qw), c, s, 0.0, inter, True), "float32")
