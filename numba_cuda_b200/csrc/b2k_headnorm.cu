@@ -10,9 +10,10 @@
 // HBM bounds them (2 and 3 items moved per item of the rows).  Sums are kept in float32
 // and a value is rounded once, when it is stored.  Measured with bf16 items, 32 + 8 heads
 // of 128: forward, 16384 tokens, 62 us = 5.6 TB/s (a copy of the same bytes 60 us);
-// backward, 32768 tokens, 172 us = 6.0 TB/s (a copy 164 us).  The reference's users
-// would write this as a last-axis reduction of their own; its library reduce stops at
-// one axis (numba/cuda/kernels/reduction.py:217-218).
+// backward, 32768 tokens, 178 to 188 us on different GPUs = 5.4 to 5.7 TB/s with inputs that
+// change from call to call (173 us on three sets of inputs in turn; a copy 164 us).  The
+// reference's users would write this as a last-axis reduction of their own; its library reduce
+// stops at one axis (numba/cuda/kernels/reduction.py:217-218).
 #include <algorithm>
 
 #include "b2k_heads_forward.cuh"
@@ -357,7 +358,9 @@ int count_items(Params &p, int most, int busy, const char *name) {
 // in order: no atomics, so equal calls give equal bits.
 constexpr int kMostBlocksPerSm = 8;
 constexpr int kBackwardHeadsPerItem = 8;
-constexpr int kBackwardBusy = 1024;       // 1024 tokens x 40 heads of 128 bf16 items: 15.7 us, with 512 18.5, with 2048 18.7
+// 1024 tokens x 40 heads of 128 bf16 items: 15.7 us, with 512 18.5, with 2048 18.7.  Not measured
+// for other types and heads.
+constexpr int kBackwardBusy = 1024;
 
 // The inverse rotation of a unit's pairs.
 template <int FROM, int TO, int VEC>
@@ -574,8 +577,8 @@ __device__ __forceinline__ void backward_rows(const Params &p, const Role &r, co
 // the ends of items, with the next item's cosines and sines: registers no longer limit
 // the bytes in flight, and no warp waits for a position and then for its table rows.
 // Every thread copies what it will read itself, so there is nothing to synchronise but its
-// own copies.  32768 tokens x 40 heads of 128 bf16 items: 198 us with the next row in
-// registers, 172 us so, 177 us with four stages.  Needs 16-byte chunks, one unit a lane,
+// own copies.  32768 tokens x 40 heads of 128 bf16 items, three sets of inputs in turn: 198 us
+// with the next row in registers, 172 us so, 177 us with four stages.  Needs 16-byte chunks, one unit a lane,
 // and items of at least kStages steps (then the loads are at most one item ahead).
 constexpr int kStages = 3;
 
@@ -780,7 +783,7 @@ __device__ __forceinline__ void backward_role(const Params &p, uint32_t first_bl
 }
 
 // Four blocks an SM where a row takes one unit a lane (128 registers; 32768 tokens x 40
-// heads of 128 bf16 items: 172 us, with three blocks 178 us).
+// heads of 128 bf16 items, three sets of inputs in turn: 172 us, with three blocks 178 us).
 template <typename T, int VEC, int ITER, bool AHEAD>
 __global__ void __launch_bounds__(kThreads, ITER == 1 ? 4 : 1) heads_backward_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(16) char shared[];

@@ -220,9 +220,10 @@ __device__ __forceinline__ void forward_roles(const Params &p, unsigned *group_m
     if constexpr (MODE != kRotate) forward_role<T, VEC, ITER, MODE, 2, INTER>(p, block - p.role[1].blocks, group_max);
 }
 
-// Five blocks an SM where a row takes one unit a lane (102 registers): left alone the
-// compiler takes a few more and four fit (rotation of 16384 tokens x 40 heads of 128 bf16
-// items 66 us instead of 62 us).
+// Five blocks an SM where a row takes one unit a lane (96 registers): left alone the compiler
+// takes a few more and four fit (rotation of 16384 tokens x 40 heads of 128 bf16 items 66 us
+// instead of 62 us).  The joined step of 16-bit items spills 56 bytes under this bound; four
+// blocks were not measured for it.
 template <typename T, int VEC, int ITER, int MODE>
 __global__ void __launch_bounds__(kThreads, ITER == 1 ? 5 : 1) heads_forward_kernel(const __grid_constant__ Params p) {
     __shared__ unsigned group_max[MODE == kRotate ? 1 : kThreads * ((2 * VEC * ITER + 15) / 16)];
@@ -244,7 +245,7 @@ void pick_forward(const Params &p, const Plan &plan, unsigned blocks, cudaStream
 }
 
 // 1024 tokens x 40 heads of 128 bf16 items: 6.8 us, with 256 8.0, with 1024 8.3, with 2048
-// 12.4; 2048 tokens: 9.5, 11.3, 10.5, 12.8.
+// 12.4; 2048 tokens: 9.5, 11.3, 10.5, 12.8.  Not measured for other types and heads.
 constexpr int kForwardBusy = 512;
 
 // Roles whose sizes or strides allow different chunks get launches of their own when they

@@ -6,7 +6,7 @@
 //
 // Writing is the forward row kernel (b2k_heads_forward.cuh) with its store replaced: the
 // group's largest magnitude by shuffles, the scale, the codes.  Measured: 32768 tokens x
-// (8 + 8) heads of 128 bf16 items 40 us = 5.1 TB/s (issue slots 67% busy), about what a
+// (8 + 8) heads of 128 bf16 items 40 to 42 us = 4.9 to 5.1 TB/s (issue slots 67% busy), about what a
 // plain copy of those bytes takes; with norm, rotation and 64 query heads beside it, 8192
 // tokens 63 us.
 #include <algorithm>

@@ -116,10 +116,13 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, position
                  set).  An output may be its own input's memory; it must not overlap an
                  input in any other way, nor another output.
     :param stream: stream of the launch (0 = the default stream); arrays that other streams
-                 produce must be complete or ordered before it, as everywhere here.
+                 produce must be complete or ordered before it, and arrays stay in use until
+                 the launch has run, as everywhere here.
 
     Squares are summed in float32: a head whose squares add up to more than 3.4e38 gives
-    zeros.
+    zeros (NaN where an item itself is infinite).  The calls are not recorded for autograd:
+    tensors that require grad or carry a forward tangent are refused, and the version
+    counters of the tensors that a call has written rise.
     """
     status = fast.norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm, q_out, k_out, stream)
     if status is not None:
@@ -141,8 +144,10 @@ def norm_rotate_backward(q, k, q_weight, k_weight, cos, sin, positions, q_grad, 
 
     The weights' gradients are sums over all tokens and heads, accumulated in float32 in
     an order that depends on the shapes only, and are stored in the weights' type.  A
-    padding token has zero gradients and adds nothing to the sums.  ``dq`` and ``dk`` may be
-    the memory of ``q_grad`` and ``k_grad``."""
+    padding token has zero gradients and adds nothing to the sums, whatever the weights are; so
+    has a head whose squares add up to more than 3.4e38.  The sum of gradient x weight x item over
+    a head is taken in float32 too.  ``dq`` and ``dk`` may be the memory of ``q_grad`` and
+    ``k_grad``."""
     status = fast.norm_rotate_backward(q, k, q_weight, k_weight, cos, sin, positions, q_grad, k_grad, eps, interleaved,
                                        norm, dq, dk, dq_weight, dk_weight, stream)
     if status is not None:
