@@ -155,7 +155,7 @@ def _version_counters():
     """torch's function that raises the version counters of a tuple of tensors."""
     many = getattr(torch._C, "_increment_version", None)
     try:
-        many((torch.empty(0),))
+        many((torch.empty(0, device="cpu"),))
         return many
     except TypeError:                                       # an older torch takes one at a time
         def each(tensors):

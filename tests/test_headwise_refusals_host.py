@@ -106,3 +106,14 @@ def test_two_outputs_in_one_memory_are_refused():
     empty = _cache(pages=0, k=(0, *side[1:4], 0, *side[5:]), v=(0, *side[1:4], 0, *side[5:]))
     assert L.b2k_cache_write(empty, _lib.FMT_F32, 2, a, b, 4096, 8, None) == 0
     assert L.b2k_cache_read(_cache(), _lib.FMT_F32, 0, a, a, 4096, 3, 3, 4, 4096, 2, 4, None) == 0
+
+
+def test_the_import_makes_no_tensor_on_the_default_device():
+    code = ("import torch\n"
+            "torch.set_default_device('cuda')\n"
+            "from numba_cuda_b200.kernels import _operands\n"
+            "assert not torch.cuda.is_initialized()\n"
+            "a = torch.zeros(2, device='cpu')\n"
+            "_operands.written(a)\n"
+            "assert a._version == 1\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
