@@ -10,7 +10,7 @@
 // HBM bounds them (2 and 3 items moved per item of the rows).  Sums are kept in float32
 // and a value is rounded once, when it is stored.  Measured with bf16 items, 32 + 8 heads
 // of 128: forward, 16384 tokens, 62 us = 5.6 TB/s (a copy of the same bytes 60 us);
-// backward, 32768 tokens, 178 to 188 us on different GPUs = 5.4 to 5.7 TB/s with inputs that
+// backward, 32768 tokens, 176 to 188 us on different GPUs = 5.4 to 5.8 TB/s with inputs that
 // change from call to call (173 us on three sets of inputs in turn; a copy 164 us).  The
 // reference's users would write this as a last-axis reduction of their own; its library reduce
 // stops at one axis (numba/cuda/kernels/reduction.py:217-218).
